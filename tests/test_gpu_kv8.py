@@ -1,0 +1,257 @@
+"""The 8-bit key/value cache and attention from it, on the GPU, against the definition in 64 bits."""
+
+import pytest
+import torch
+
+from attention_cases import BLOCK, RING, attention64, cache64, coded64, kv8_attention64, near
+from triune_b200 import ops
+
+pytestmark = pytest.mark.gpu
+KINDS = ["int8", "e4m3"]
+
+
+def rows(B, T, G, D, seed=0, loud=True):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(B, T, G, D, generator=gen, device="cuda")
+    if loud:
+        x[..., 3] *= 9.0  # a channel that is larger than the others
+    return x.bfloat16()
+
+
+def filled(B, G, D, n, kind, seed=0, capacity=None, chunk=None):
+    """-> (cache of n tokens, keys and values [B, n, G, D])"""
+    cache = ops.kv8_cache(B, G, capacity or n, D, kind, device="cuda")
+    k, v = rows(B, n, G, D, seed), rows(B, n, G, D, seed + 1, False)
+    chunk = chunk or n
+    for p in range(0, n, max(1, chunk)):
+        ops.kv8_append(cache, k[:, p : p + chunk], v[:, p : p + chunk], p)
+    return cache, k, v
+
+
+def bits(cache):
+    return {n: t.view(torch.uint8) for n, t in cache.items()}
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n", [1, 63, 64, 65, 128, 200, 1000])
+@pytest.mark.parametrize("G,D", [(1, 64), (3, 128), (2, 8), (2, 80)])
+def test_what_the_cache_holds(kind, n, G, D):
+    cache, k, v = filled(2, G, D, n, kind)
+    full = n // BLOCK
+    got = ops.kv8_expand(cache, n, D)
+    for x, y, name in zip(got, (k, v), ("k", "v")):
+        for b in range(2):
+            held = cache64(y[b].transpose(0, 1), kind, n)  # codes times scale in fp32, rounded to bf16: twice on the way
+            assert torch.equal(x[b].transpose(0, 1), held.float().bfloat16())
+            scale = coded64(y[b, : full * BLOCK].transpose(0, 1).unflatten(1, (full, BLOCK)), kind)[1] if full else cache[name + "s"][b, :, :0]
+            assert torch.equal(cache[name + "s"][b, :, :full].double(), scale.double())
+        slots = torch.arange(max(0, n - RING), n, device="cuda")
+        assert torch.equal(cache[name + "t"][:, :, slots % RING, :D].transpose(1, 2), y[:, slots])
+        assert not cache[name + "t"][..., D:].any() and not cache[name + "8"].view(torch.uint8)[..., D:].any()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D", [64, 128])
+def test_contents_do_not_depend_on_the_portions(kind, D):
+    n = 500
+    whole, k, v = filled(2, 2, D, n, kind)
+    for chunk in (1, 7, 64, 65, 100, 190, 333):
+        assert all(torch.equal(a, bits(whole)[x]) for x, a in bits(filled(2, 2, D, n, kind, chunk=chunk)[0]).items()), chunk
+    # up to 64 tokens are taken back and others come in their place
+    for back in (1, 30, 64):
+        new_k, new_v = rows(2, back + 40, 2, D, 77), rows(2, back + 40, 2, D, 78)
+        cache = filled(2, 2, D, n, kind, capacity=640)[0]
+        ops.kv8_append(cache, new_k, new_v, n - back)
+        k2, v2 = torch.cat((k[:, : n - back], new_k), 1), torch.cat((v[:, : n - back], new_v), 1)
+        fresh = ops.kv8_cache(2, 2, 640, D, kind, device="cuda")
+        ops.kv8_append(fresh, k2, v2, 0)
+        m = k2.shape[1]
+        assert all(torch.equal(a, b) for a, b in zip(ops.kv8_expand(cache, m, D), ops.kv8_expand(fresh, m, D)))
+        assert torch.equal(cache["kt"], fresh["kt"])
+
+
+def attend(B, G, rep, D, T, starts, kind, seed=0, chunk=None, on_device=True, append=True):
+    """Decodes T tokens per sequence after ``starts`` ones, together, and compares every sequence."""
+    longest = max(max(starts), 0) + T
+    cache, k, v = filled(B, G, D, longest, kind, seed, capacity=longest + 70)
+    for b, n in enumerate(starts):  # each sequence as it was before its new tokens
+        if n >= 0:
+            one = ops.kv8_cache(1, G, longest + 70, D, kind, device="cuda")
+            if n:
+                ops.kv8_append(one, k[b : b + 1, :n], v[b : b + 1, :n], 0)
+            for x in cache:
+                cache[x].view(torch.uint8)[b] = one[x].view(torch.uint8)[0]
+    pos = torch.tensor(starts, device="cuda") if on_device else starts[0]
+    q = rows(B, T, G * rep, D, seed + 5, False)
+    at = lambda x: torch.stack([x[b, max(n, 0) : max(n, 0) + T] for b, n in enumerate(starts)])  # noqa: E731
+    if append:
+        out = ops.kv8_attention(q, cache, pos, at(k), at(v))
+    else:
+        ops.kv8_append(cache, at(k), at(v), pos)
+        out = ops.kv8_attention(q, cache, pos)
+    for b, n in enumerate(starts):
+        if n < 0:
+            assert not out[b].any()
+            continue
+        near(out[b], kv8_attention64(q[b], k[b].transpose(0, 1), v[b].transpose(0, 1), kind, n), f"sequence {b}")
+    return out
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D", [8, 64, 72, 128])
+@pytest.mark.parametrize("T,rep", [(1, 1), (1, 4), (1, 8), (4, 1), (3, 5), (9, 2), (20, 3)])
+def test_steps_and_drafted_tokens(kind, D, T, rep):
+    attend(5, 2, rep, D, T, [0, 1, 63, 200, 517], kind)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n", [5000, 40000])
+def test_long_caches(kind, n):
+    attend(1, 2, 4, 128, 1, [n], kind, on_device=False)
+    attend(2, 1, 2, 64, 2, [n, 3], kind)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("T", [64, 100, 300])
+def test_portions_of_prompts(kind, T):
+    """As steps, but for weights, which lose up to 2^-8 of themselves, and values, which are rounded to bf16 (2^-8) when they are expanded: keys
+    too, which moves scores by 2^-8 of the sum of their terms' magnitudes."""
+    for on_device, starts in ((False, [130]), (True, [0, 130, -1, 77])):
+        B, G, rep, D = len(starts), 2, 2, 64
+        longest = max(starts) + T
+        cache, k, v = filled(B, G, D, longest, kind, capacity=longest)
+        q = rows(B, T, G * rep, D, 5, False) * 0.25
+        pos = torch.tensor(starts, device="cuda") if on_device else starts[0]
+        at = lambda x: torch.stack([x[b, max(n, 0) : max(n, 0) + T] for b, n in enumerate(starts)])  # noqa: E731
+        for b, n in enumerate(starts):
+            one = ops.kv8_cache(1, G, longest, D, kind, device="cuda")
+            ops.kv8_append(one, k[b : b + 1, : max(n, 0)], v[b : b + 1, : max(n, 0)], 0)
+            for x in cache:
+                cache[x].view(torch.uint8)[b] = one[x].view(torch.uint8)[0]
+        out = ops.kv8_attention(q, cache, pos, at(k), at(v))
+        for b, n in enumerate(starts):
+            if n < 0:
+                assert not out[b].any()
+                continue
+            K, V = (cache64(x[b].transpose(0, 1), kind, n + T).float().bfloat16() for x in (k, v))
+            near(out[b : b + 1], attention64(q[b : b + 1], K.transpose(0, 1)[None], V.transpose(0, 1)[None])["o"], f"sequence {b}")
+
+
+def test_appending_first_is_the_same_and_scale_and_bound_are_the_callers():
+    a = attend(3, 2, 2, 64, 3, [10, 61, 300], "int8")
+    assert torch.equal(a, attend(3, 2, 2, 64, 3, [10, 61, 300], "int8", append=False))
+    cache, k, v = filled(1, 2, 64, 3000, "int8", capacity=4096)
+    q = rows(1, 1, 4, 64, 3, False)
+    for most in (None, 3000, 100000, 1):
+        out = ops.kv8_attention(q, cache, torch.tensor([2999], device="cuda"), scale=0.3, most=most)
+        near(out[0], kv8_attention64(q[0], k[0].transpose(0, 1), v[0].transpose(0, 1), "int8", 2999, 0.3))
+
+
+def test_queries_of_any_size_and_keys_far_from_one():
+    for factor in (1e-30, 1e-5, 3e4, 1e15):
+        cache = ops.kv8_cache(1, 1, 300, 64, "int8", device="cuda")
+        k, v = rows(1, 200, 1, 64, 1, False), rows(1, 200, 1, 64, 2, False)
+        k, v = (k.float() / factor).bfloat16(), (v.float() * factor).bfloat16()
+        q = (rows(1, 1, 2, 64, 3, False).float() * factor).bfloat16()
+        ops.kv8_append(cache, k, v, 0)
+        out = ops.kv8_attention(q, cache, 199)
+        near(out[0], kv8_attention64(q[0], k[0].transpose(0, 1), v[0].transpose(0, 1), "int8", 199))
+
+
+def test_blocks_whose_scales_differ_and_blocks_of_zeros():
+    cache = ops.kv8_cache(1, 1, 400, 64, "int8", device="cuda")
+    k, v = rows(1, 330, 1, 64, 1, False), rows(1, 330, 1, 64, 2, False)
+    for m, f in enumerate((0.0, 1e-6, 1.0, 1e6, 0.0)):
+        v[:, 64 * m : 64 * m + 64] *= f
+    k[:, 64:128] = 0
+    ops.kv8_append(cache, k, v, 0)
+    q = rows(1, 1, 3, 64, 3, False)
+    near(ops.kv8_attention(q, cache, 329)[0], kv8_attention64(q[0], k[0].transpose(0, 1), v[0].transpose(0, 1), "int8", 329))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("T", [1, 5, 100])
+def test_idle_sequences_and_tokens_past_the_capacity_leave_the_rest_alone(kind, T):
+    B, G, D, C = 3, 2, 64, 128
+    cache, k, v = filled(B, G, D, 100, kind, capacity=C)
+    before = {n: t.clone() for n, t in bits(cache).items()}
+    q, nk, nv = rows(B, T, 4, D, 3, False), rows(B, T, G, D, 4), rows(B, T, G, D, 5)
+    out = ops.kv8_attention(q, cache, torch.tensor([-1, C, -5], device="cuda"), nk, nv)
+    assert all(torch.equal(before[n], t) for n, t in bits(cache).items())
+    assert not out[0].any() and not out[2].any() and bool(torch.isnan(out[1]).all())
+    out = ops.kv8_attention(q, cache, torch.tensor([100, C - 2, -1], device="cuda"), nk, nv)
+    assert bool(torch.isnan(out[1, 2:]).all()) and not torch.isnan(out[1, :2]).any() and not torch.isnan(out[0, : C - 100]).any()
+    assert all(torch.equal(before[n][2], t[2]) for n, t in bits(cache).items())
+
+
+@pytest.mark.parametrize("what", [float("nan"), float("inf")])
+def test_tokens_that_are_no_numbers(what):
+    for T in (4, 100):
+        cache, k, v = filled(1, 1, 64, 70, "int8", capacity=256)
+        q, nk, nv = rows(1, T, 2, 64, 3, False), rows(1, T, 1, 64, 4), rows(1, T, 1, 64, 5)
+        clean = ops.kv8_attention(q, {n: t.clone() for n, t in cache.items()}, 70, nk, nv)
+        nv[0, 2, 0, 7] = what
+        out = ops.kv8_attention(q, cache, 70, nk, nv)
+        assert torch.equal(out[:, :2], clean[:, :2]) if T == 4 else True  # 70 + 100 fill the block, which reads as NaN throughout
+        assert bool(torch.isnan(out[:, 2:, :, 7]).all()) or what == float("inf") and not torch.isfinite(out[:, 2:, :, 7]).any()
+    cache, k, v = filled(1, 1, 64, 200, "int8")
+    assert torch.isfinite(ops.kv8_attention(q[:, :1], cache, 199)).all()
+    v[0, 70, 0, 1] = what
+    ops.kv8_append(cache, k, v, 0)
+    got = ops.kv8_expand(cache, 200, 64)[1][0, :, 0]
+    assert bool(torch.isnan(got[64:128]).all()) and torch.isfinite(got[:64]).all() and torch.isfinite(got[128:]).all()
+    assert bool(torch.isnan(ops.kv8_attention(q[:, :1], cache, 199)).all())
+
+
+def test_offsets_past_32_bits():
+    """5 sequences of 2^17 tokens, 32 heads of 128: codes of 2.7 GB, the last of them past 2^31."""
+    B, G, D, C = 5, 32, 128, 1 << 17
+    cache = ops.kv8_cache(B, G, C, D, "int8", device="cuda")
+    assert cache["k8"].numel() > 2 ** 31
+    k, v = rows(B, 200, G, D, 1), rows(B, 200, G, D, 2, False)
+    pos = torch.tensor([-1, -1, -1, -1, C - 200], device="cuda")
+    ops.kv8_append(cache, k, v, pos)  # block by block: C - 200 is 56 past a block's start, so this block holds older (zero) tokens too
+    full = torch.zeros(G, C, D, device="cuda", dtype=torch.bfloat16)
+    full[:, C - 200 :] = v[4].transpose(0, 1)
+    got = ops.kv8_expand(cache, torch.tensor([0, 0, 0, 0, C], device="cuda"), D)[1]
+    assert torch.equal(got[4, C - 256 :].transpose(0, 1), cache64(full[:, C - 256 :], "int8", 256).float().bfloat16())
+    q = rows(B, 1, G, D, 3, False)
+    out = ops.kv8_attention(q, cache, torch.tensor([-1, -1, -1, -1, C - 1], device="cuda"))
+    keys = torch.zeros(1, C, D, device="cuda", dtype=torch.bfloat16)
+    keys[:, C - 200 :] = k[4, :, 31:].transpose(0, 1)
+    near(out[4, :, 31:], kv8_attention64(q[4, :, 31:], keys, full[31:], "int8", C - 1))
+
+
+@pytest.mark.parametrize("T", [1, 3, 80])
+def test_captured_steps_follow_positions_on_the_device(T):
+    B, G, D = 2, 2, 64
+    n, steps = 100, 6
+    k, v, q = (rows(B, n + T * steps, h, D, s, False) for h, s in ((G, 1), (G, 2), (4, 3)))
+
+    def fresh():
+        cache = ops.kv8_cache(B, G, n + T * steps, D, "e4m3", device="cuda")
+        ops.kv8_append(cache, k[:, :n], v[:, :n], 0)
+        return cache
+
+    want, cache = [], fresh()
+    for i in range(steps):
+        at = slice(n + T * i, n + T * i + T)
+        want.append(ops.kv8_attention(q[:, at], cache, torch.tensor([n + T * i], device="cuda"), k[:, at], v[:, at]))
+    caches = [fresh(), fresh()]
+    graphs = []
+    for c in caches:  # two captures, replayed in turn
+        pos = torch.tensor([n, n], device="cuda")
+        at = [x[:, n : n + T].clone() for x in (q, k, v)]
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = ops.kv8_attention(at[0], c, pos, at[1], at[2])
+            pos += T
+        pos.fill_(n)
+        graphs.append((g, at, out, pos))  # the captured steps read and move the positions
+    for i in range(steps):
+        for g, at, out, _ in graphs:
+            for x, y in zip(at, (q, k, v)):
+                x.copy_(y[:, n + T * i : n + T * i + T])
+            g.replay()
+            assert torch.equal(out, want[i])
+    assert all(torch.equal(a, bits(caches[0])[x]) for x, a in bits(cache).items())

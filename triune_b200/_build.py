@@ -89,8 +89,8 @@ def _build_module(so: Path, sources, force: bool, verbose: bool, ptxas_info: boo
         if not stale:
             continue
         if src.suffix == ".cu":
-            # the heterogeneous-layer kernels keep the accurate functions: large angles, chained exponentials, 32-bit models
-            fast = [] if "hybrid" in src.parts else ["--use_fast_math"]
+            # these keep the accurate functions: large angles, chained exponentials, 32-bit models; codes that are the same as a division gives
+            fast = [] if {"hybrid", "attention"} & set(src.parts) else ["--use_fast_math"]
             cmd = (
                 [nvcc, "-c", str(src), "-o", str(obj)]
                 + NVCC_ARCH

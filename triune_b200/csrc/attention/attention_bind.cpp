@@ -1,0 +1,218 @@
+// Python bindings of softmax attention and of the 8-bit key/value cache.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include <cmath>
+
+#include "kv8.cuh"
+
+namespace {
+using torch::Tensor;
+using OptTensor = c10::optional<Tensor>;
+
+constexpr int64_t MOST_ROWS = 65535ll * 128;  // queries or keys of a sequence: tiles along a grid's second dimension
+
+cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
+bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
+
+// [B, rows, heads, D] bf16 as the kernels read it: 16-byte pieces of every row in place. Other layouts are copied (`held` keeps the copy).
+tb::AttentionView view_of(const Tensor& x, const Tensor& like, const char* name, Tensor& held) {
+  TORCH_CHECK(x.is_cuda() && x.get_device() == like.get_device(), name, " must be on the device of the queries");
+  TORCH_CHECK(x.scalar_type() == at::kBFloat16 && x.dim() == 4, name, " must be bfloat16 [batch, tokens, heads, head_dim]");
+  bool fits = (reinterpret_cast<uintptr_t>(x.data_ptr()) & 15) == 0 && (x.size(3) == 1 || x.stride(3) == 1);
+  for (int i = 0; i < 3; ++i) fits = fits && (x.size(i) <= 1 || (x.stride(i) > 0 && x.stride(i) % 8 == 0));  // nothing that is expanded
+  held = fits ? x : x.clone(at::MemoryFormat::Contiguous);
+  auto step = [&](int i) { return held.size(i) <= 1 ? 0ll : (long long)held.stride(i); };
+  return tb::AttentionView{held.data_ptr(), step(1), step(2), step(0)};
+}
+
+const long long* numbers(const OptTensor& t, int64_t batch, const Tensor& like, const char* name) {
+  if (!has(t)) return nullptr;
+  TORCH_CHECK(t->is_cuda() && t->get_device() == like.get_device() && t->scalar_type() == at::kLong && t->is_contiguous() && t->numel() == batch, name,
+              " must be int64 [batch] on the device of the queries");
+  return reinterpret_cast<const long long*>(t->data_ptr<int64_t>());
+}
+
+int* status_of(const Tensor& t) {
+  TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kInt && t.numel() == 1, "status: one CUDA int32");
+  return t.data_ptr<int>();
+}
+
+tb::AttentionShape shape_of(const Tensor& q, const Tensor& k, const Tensor& v, double scale, bool causal, int64_t window, const OptTensor& lengths,
+                            const OptTensor& starts, int64_t start) {
+  TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.sizes() == k.sizes() && q.size(0) == k.size(0) && q.size(3) == k.size(3),
+              "attention: queries [B, T, H, D], keys and values [B, S, G, D]");
+  const int64_t T = q.size(1), S = k.size(1), H = q.size(2), G = k.size(2), D = q.size(3);
+  TORCH_CHECK(D % 8 == 0 && D >= 8 && D <= 128, "attention: head sizes are multiples of 8 up to 128");
+  TORCH_CHECK(G > 0 && H % G == 0, "attention: query heads must be a multiple of the key/value heads");
+  TORCH_CHECK(T <= MOST_ROWS && S <= MOST_ROWS && q.size(0) * H < (1ll << 31), "attention: too many rows");
+  TORCH_CHECK(std::isfinite(scale) && scale > 0, "attention: the scale must be positive");
+  tb::AttentionShape a{(int)q.size(0), (int)T, (int)S, (int)H, (int)G, (int)D, (float)scale, causal, (int)std::min<int64_t>(window, 1 << 30)};
+  a.lengths = numbers(lengths, a.B, q, "key_lengths");
+  a.starts = numbers(starts, a.B, q, "query_start");
+  a.start = start;
+  return a;
+}
+
+tb::Kv8Cache cache_of(const Tensor& k8, const Tensor& v8, const Tensor& ks, const Tensor& vs, const Tensor& kt, const Tensor& vt, const Tensor& like) {
+  const bool e4m3 = k8.scalar_type() == at::kFloat8_e4m3fn;
+  TORCH_CHECK(e4m3 || k8.scalar_type() == at::kChar, "kv8: codes are int8 or float8_e4m3fn");
+  TORCH_CHECK(k8.dim() == 4 && v8.sizes() == k8.sizes() && v8.scalar_type() == k8.scalar_type(), "kv8: codes [B, G, capacity, pitch]");
+  const int64_t B = k8.size(0), G = k8.size(1), C = k8.size(2), P = k8.size(3);
+  TORCH_CHECK((P == 64 || P == 128) && C % tb::KV8_BLOCK == 0 && C < (1ll << 30), "kv8: pitch 64 or 128, capacity a multiple of 64");
+  for (const Tensor* t : {&ks, &vs})
+    TORCH_CHECK(t->scalar_type() == at::kFloat && t->dim() == 3 && t->size(0) == B && t->size(1) == G && t->size(2) == C / tb::KV8_BLOCK,
+                "kv8: scales fp32 [B, G, capacity / 64]");
+  for (const Tensor* t : {&kt, &vt})
+    TORCH_CHECK(t->scalar_type() == at::kBFloat16 && t->dim() == 4 && t->size(0) == B && t->size(1) == G && t->size(2) == tb::KV8_RING && t->size(3) == P,
+                "kv8: ring bf16 [B, G, 128, pitch]");
+  for (const Tensor* t : {&k8, &v8, &ks, &vs, &kt, &vt})
+    TORCH_CHECK(t->is_cuda() && t->get_device() == like.get_device() && t->is_contiguous() && (reinterpret_cast<uintptr_t>(t->data_ptr()) & 15) == 0,
+                "kv8: the cache must be contiguous, 16-byte aligned and on the device of the rows");
+  return tb::Kv8Cache{(uint8_t*)k8.data_ptr(), (uint8_t*)v8.data_ptr(), ks.data_ptr<float>(), vs.data_ptr<float>(), (__nv_bfloat16*)kt.data_ptr(),
+                      (__nv_bfloat16*)vt.data_ptr(), (int)B, (int)G, (int)C, (int)P, e4m3};
+}
+
+tb::Kv8Pos pos_of(int64_t host, const OptTensor& dev, int64_t batch, const Tensor& like) {
+  if (!has(dev)) return tb::Kv8Pos{host, nullptr, 0};
+  TORCH_CHECK(dev->is_cuda() && dev->get_device() == like.get_device() && dev->scalar_type() == at::kLong && dev->is_contiguous() &&
+                  (dev->numel() == 1 || dev->numel() == batch),
+              "kv8: positions are int64, one or one per sequence, on the device of the rows");
+  return tb::Kv8Pos{0, reinterpret_cast<const long long*>(dev->data_ptr<int64_t>()), dev->numel() == 1 ? 0 : 1};
+}
+
+void check_rows(const tb::Kv8Cache& c, const Tensor& x, int64_t heads, const char* name) {
+  TORCH_CHECK(x.dim() == 4 && x.size(0) == c.B && x.size(2) == heads && x.size(3) % 8 == 0 && x.size(3) >= 8 && x.size(3) <= c.P, "kv8: ", name,
+              " [B, T, heads, D] must fit the cache (D a multiple of 8)");
+  TORCH_CHECK(x.size(1) < (1ll << 30), "kv8: too many tokens");
+}
+
+void append_rows(const tb::Kv8Cache& c, const Tensor& k, const Tensor& v, const tb::Kv8Pos& pos) {
+  check_rows(c, k, c.G, "keys");
+  TORCH_CHECK(v.sizes() == k.sizes(), "kv8: keys and values differ in shape");
+  Tensor hk, hv;
+  const tb::AttentionView kv = view_of(k, k, "keys", hk), vv = view_of(v, k, "values", hv);
+  if (k.numel() > 0) tb::launch_kv8_append(c, kv, vv, (int)k.size(1), (int)k.size(3), pos, cur_stream());
+}
+
+// -> (out, lse). lse is empty where it is not asked for.
+std::vector<Tensor> attention_fwd(const Tensor& q, const Tensor& k, const Tensor& v, double scale, bool causal, int64_t window, const OptTensor& lengths,
+                                  const OptTensor& starts, int64_t start, bool want_lse, const Tensor& status) {
+  tb::AttentionFwd f{};
+  f.a = shape_of(q, k, v, scale, causal, window, lengths, starts, start);
+  c10::cuda::CUDAGuard guard(q.device());
+  Tensor hq, hk, hv;
+  f.q = view_of(q, q, "queries", hq);
+  f.k = view_of(k, q, "keys", hk);
+  f.v = view_of(v, q, "values", hv);
+  Tensor out = torch::empty(q.sizes(), q.options()), lse, part;
+  const auto f32 = q.options().dtype(at::kFloat);
+  if (want_lse) lse = torch::empty({f.a.B, f.a.H, tb::attention_rows(f.a.T)}, f32);
+  if (out.numel() == 0) return {out, lse};
+  if (f.a.S == 0) {
+    out.zero_();
+    if (want_lse) lse.fill_(INFINITY);
+    return {out, lse};
+  }
+  const long long bytes = tb::attention_fwd_scratch(f.a);
+  if (bytes > 0) part = torch::empty({bytes / 4}, f32);
+  f.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
+  f.lse = want_lse ? lse.data_ptr<float>() : nullptr;
+  f.part = bytes > 0 ? part.data_ptr<float>() : nullptr;
+  f.status = status_of(status);
+  tb::launch_attention_fwd(f, cur_stream());
+  return {out, lse};
+}
+
+// -> (dq, dk, dv)
+std::vector<Tensor> attention_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out, const Tensor& dout, const Tensor& lse, double scale,
+                                  bool causal, int64_t window, const OptTensor& lengths, const OptTensor& starts, int64_t start, const Tensor& status) {
+  tb::AttentionBwd f{};
+  f.a = shape_of(q, k, v, scale, causal, window, lengths, starts, start);
+  TORCH_CHECK(out.sizes() == q.sizes() && dout.sizes() == q.sizes(), "attention: outputs and their gradients have the queries' shape");
+  TORCH_CHECK(lse.is_cuda() && lse.get_device() == q.get_device() && lse.scalar_type() == at::kFloat && lse.is_contiguous() &&
+                  lse.numel() == (int64_t)f.a.B * f.a.H * tb::attention_rows(f.a.T) && (reinterpret_cast<uintptr_t>(lse.data_ptr()) & 15) == 0,
+              "attention: the forward pass's sums");
+  c10::cuda::CUDAGuard guard(q.device());
+  Tensor held[5];
+  f.q = view_of(q, q, "queries", held[0]);
+  f.k = view_of(k, q, "keys", held[1]);
+  f.v = view_of(v, q, "values", held[2]);
+  f.out = view_of(out, q, "outputs", held[3]);
+  f.dout = view_of(dout, q, "gradients", held[4]);
+  Tensor dq = torch::empty(q.sizes(), q.options()), dk = torch::empty(k.sizes(), k.options()), dv = torch::empty(v.sizes(), v.options());
+  if (dq.numel() == 0 || dk.numel() == 0) return {dq.zero_(), dk.zero_(), dv.zero_()};
+  Tensor delta = torch::empty(lse.sizes(), lse.options());
+  f.lse = lse.data_ptr<float>();
+  f.delta = delta.data_ptr<float>();
+  f.dq = reinterpret_cast<__nv_bfloat16*>(dq.data_ptr());
+  f.dk = reinterpret_cast<__nv_bfloat16*>(dk.data_ptr());
+  f.dv = reinterpret_cast<__nv_bfloat16*>(dv.data_ptr());
+  f.status = status_of(status);
+  tb::launch_attention_bwd(f, cur_stream());
+  return {dq, dk, dv};
+}
+
+void kv8_append(const Tensor& k8, const Tensor& v8, const Tensor& ks, const Tensor& vs, const Tensor& kt, const Tensor& vt, const Tensor& k, const Tensor& v,
+                int64_t host, const OptTensor& dev) {
+  const tb::Kv8Cache c = cache_of(k8, v8, ks, vs, kt, vt, k);
+  c10::cuda::CUDAGuard guard(k.device());
+  append_rows(c, k, v, pos_of(host, dev, c.B, k));
+}
+
+// -> k, v [B, G, rows, D]
+std::vector<Tensor> kv8_expand(const Tensor& k8, const Tensor& v8, const Tensor& ks, const Tensor& vs, const Tensor& kt, const Tensor& vt, int64_t rows,
+                               int64_t D, int64_t host, const OptTensor& dev) {
+  const tb::Kv8Cache c = cache_of(k8, v8, ks, vs, kt, vt, k8);
+  TORCH_CHECK(rows >= 0 && rows <= c.C && D % 8 == 0 && D >= 8 && D <= c.P, "kv8: rows and head size must fit the cache");
+  c10::cuda::CUDAGuard guard(k8.device());
+  Tensor k = torch::empty({c.B, c.G, rows, D}, kt.options()), v = torch::empty_like(k);
+  if (k.numel() > 0)
+    tb::launch_kv8_expand(c, reinterpret_cast<__nv_bfloat16*>(k.data_ptr()), reinterpret_cast<__nv_bfloat16*>(v.data_ptr()), (int)rows, (int)D,
+                          pos_of(host, dev, c.B, k8), cur_stream());
+  return {k, v};
+}
+
+// Appends k and v (where given), then attends. `most`: tokens a sequence may hold then; a bound that the work is split by.
+Tensor kv8_attention(const Tensor& k8, const Tensor& v8, const Tensor& ks, const Tensor& vs, const Tensor& kt, const Tensor& vt, const Tensor& q,
+                     const OptTensor& k, const OptTensor& v, int64_t host, const OptTensor& dev, double scale, int64_t most) {
+  const tb::Kv8Cache c = cache_of(k8, v8, ks, vs, kt, vt, q);
+  TORCH_CHECK(q.dim() == 4 && q.size(2) % c.G == 0, "kv8: query heads must be a multiple of the cache's");
+  check_rows(c, q, q.size(2), "queries");
+  TORCH_CHECK(std::isfinite(scale) && scale > 0, "kv8: the scale must be positive");
+  c10::cuda::CUDAGuard guard(q.device());
+  tb::Kv8Attention a{};
+  a.c = c;
+  Tensor hq, part;
+  a.q = view_of(q, q, "queries", hq);
+  a.T = (int)q.size(1);
+  a.H = (int)q.size(2);
+  a.D = (int)q.size(3);
+  a.pos = pos_of(host, dev, c.B, q);
+  a.scale = (float)scale;
+  a.most = (int)std::max<int64_t>(0, std::min<int64_t>(most, c.C));
+  Tensor out = torch::empty(q.sizes(), q.options());
+  if (has(k)) {
+    TORCH_CHECK(has(v) && k->dim() == 4 && k->size(1) == q.size(1) && k->size(3) == q.size(3) && k->get_device() == q.get_device(),
+                "kv8: new keys and values come with the queries' tokens");
+    append_rows(c, *k, *v, a.pos);
+  }
+  if (out.numel() == 0) return out;
+  a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
+  const long long bytes = tb::kv8_attention_scratch(a);
+  if (bytes > 0) part = torch::empty({bytes / 4}, q.options().dtype(at::kFloat));
+  a.part = bytes > 0 ? part.data_ptr<float>() : nullptr;
+  tb::launch_kv8_attention(a, cur_stream());
+  return out;
+}
+
+}  // namespace
+
+void register_attention(pybind11::module& m) {
+  m.def("attention_fwd", &attention_fwd);
+  m.def("attention_bwd", &attention_bwd);
+  m.def("kv8_append", &kv8_append);
+  m.def("kv8_expand", &kv8_expand);
+  m.def("kv8_attention", &kv8_attention);
+}

@@ -1,0 +1,521 @@
+// Backward pass: the probabilities are computed again from the scores and the saved logarithms of their sums. With
+//   P = exp(S - lse),  dP = dO V^T,  delta_i = dO_i . O_i,  dS = P (dP - delta):
+//   dQ = scale dS K,   dK = scale dS^T Q,   dV = P^T dO     (dK, dV summed over the query heads of a shared head).
+//
+// Two kernels, each of which keeps its sums in TMEM and writes every gradient once: one per 128 queries (dQ; it also forms delta),
+// one per 128 keys (dK, dV). S and dP are formed in both, so there are seven tile products instead of the five of a kernel that
+// adds dQ up in global memory: no atomics, the same bits every time, no fp32 copy of dQ, and every product that reads P or dS
+// takes it from TMEM as its first operand (rows = lanes), so neither passes through shared memory.
+// Both: warp 0 TMA producer, warp 1 tcgen05.mma, warps 4-11 softmax; a thread has one row and half of its 128 columns, and keeps
+// the fp32 probabilities in registers between S and dP. P and dS are rounded to bf16 for the products (2^-8 of each term at
+// most, which averages out over the sums); dS is formed from the unrounded P.
+// The tensor cores work on the next tile's scores while the softmax warps form dS, and on dP while they form P.
+// TMEM: columns 0-127 S (P or its transpose over it), 128-255 dP (dS over it), 256-383 and 384-511 the sums.
+#include "../common/per_device.h"
+#include "attention_tiles.cuh"
+
+namespace tb {
+namespace {
+
+constexpr int BW_THREADS = 384;
+
+struct BwdParams {
+  AttentionShape a;
+  AttentionView out, dout;
+  const float* lse;
+  float* delta;
+  __nv_bfloat16 *dq, *dk, *dv;
+  float scale2;
+  int* status;
+};
+
+// 64 columns of a row from TMEM columns `at` on
+__device__ __forceinline__ void load_half(uint32_t at, uint32_t (&x)[32], uint32_t (&y)[32]) {
+  tmem_ld_32x32b_x32(at, x);
+  tmem_ld_32x32b_x32(at + 32, y);
+  tmem_ld_wait_regs(x);
+  asm volatile("" : "+r"(y[0]), "+r"(y[1]), "+r"(y[2]), "+r"(y[3]), "+r"(y[4]), "+r"(y[5]), "+r"(y[6]), "+r"(y[7]), "+r"(y[8]), "+r"(y[9]), "+r"(y[10]),
+               "+r"(y[11]), "+r"(y[12]), "+r"(y[13]), "+r"(y[14]), "+r"(y[15])::"memory");
+  asm volatile("" : "+r"(y[16]), "+r"(y[17]), "+r"(y[18]), "+r"(y[19]), "+r"(y[20]), "+r"(y[21]), "+r"(y[22]), "+r"(y[23]), "+r"(y[24]), "+r"(y[25]),
+               "+r"(y[26]), "+r"(y[27]), "+r"(y[28]), "+r"(y[29]), "+r"(y[30]), "+r"(y[31])::"memory");
+}
+
+// D += A B, A: 128 x 128 bf16 in TMEM as two halves of 64 columns, each in the first 32 TMEM columns of its half of `a`; B: rows
+// `b` of a [128][64 DB] tile
+template <int DB>
+__device__ __forceinline__ void rows_product(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+#pragma unroll
+  for (int k = 0; k < AT_M / 16; ++k)
+    umma_bf16_ts(d, a + (k >> 2) * 64 + (k & 3) * 8, make_smem_desc(b + k * 2048, AT_BOX, 1024), idesc, add || k > 0);
+}
+
+// D = A B^T over the head dimension
+__device__ __forceinline__ void scores_product(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int steps) {
+  for (int k = 0; k < steps; ++k) {
+    const uint32_t off = (k >> 2) * AT_BOX + (k & 3) * 32;
+    umma_bf16(d, make_smem_desc(a + off, 16, 1024), make_smem_desc(b + off, 16, 1024), idesc, k > 0);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- queries
+template <int DB>
+__global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
+                                                                     const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                                                                     const BwdParams p) {
+  constexpr int TILE = DB * AT_BOX;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  uint8_t *sQ = smem, *sG = sQ + TILE, *sK = sG + TILE, *sV = sK + 2 * TILE;  // G: dO
+  __shared__ __align__(8) uint64_t bars[12];
+  uint64_t *q_full = bars, *kv_full = bars + 1, *kv_empty = bars + 3, *s_full = bars + 5, *s_read = bars + 6, *dp_full = bars + 7, *ds_ready = bars + 8,
+           *done = bars + 9, *k_clean = bars + 10, *end_full = bars + 11;
+  __shared__ uint32_t tmem_slot;
+  __shared__ float part[AT_M];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int h = blockIdx.x % p.a.H, b = blockIdx.x / p.a.H, kvh = h / (p.a.H / p.a.G);
+  const int q0 = (gridDim.y - 1 - blockIdx.y) * AT_M;
+  const Visible vis(p.a, b);
+  const int2 range = vis.tiles(q0, min(p.a.T, q0 + AT_M) - 1);
+  const int n = range.y - range.x;
+  // the tile, if any, in which the sequence ends before the tile does: its other keys may hold anything and are set to zero. It is
+  // the last of all and has barriers of its own, whose only phase the warps that wait for nothing else cannot miss.
+  const int ragged = vis.length % AT_M != 0 && vis.length < p.a.S ? vis.length / AT_M - range.x : -1;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(kv_full + i, 1);
+      mbar_init(kv_empty + i, 1);
+    }
+    mbar_init(s_full, 1);
+    mbar_init(s_read, 256);
+    mbar_init(dp_full, 1);
+    mbar_init(ds_ready, 256);
+    mbar_init(done, 1);
+    mbar_init(k_clean, 64);
+    mbar_init(end_full, 1);
+    mbar_fence_init();
+  }
+  if (warp == 2) {
+    tmem_alloc(&tmem_slot, 512);
+    tmem_relinquish();
+  }
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0 && n > 0) {
+      prefetch_tmap(&tmQ);
+      prefetch_tmap(&tmG);
+      prefetch_tmap(&tmK);
+      prefetch_tmap(&tmV);
+      mbar_expect_tx(q_full, 2 * TILE);
+      for (int d = 0; d < DB; ++d) {
+        tma_load_4d(sQ + d * AT_BOX, &tmQ, q_full, d * 64, q0, h, b);
+        tma_load_4d(sG + d * AT_BOX, &tmG, q_full, d * 64, q0, h, b);
+      }
+      bool ok = true;
+      for (int u = 0; u < n && ok; ++u) {
+        const int s = u & 1;
+        if (u >= 2) ok = mbar_wait(kv_empty + s, ((u >> 1) & 1) ^ 1);
+        if (!ok) break;
+        uint64_t* full = u == ragged ? end_full : kv_full + s;
+        mbar_expect_tx(full, 2 * TILE);
+        for (int d = 0; d < DB; ++d) {
+          tma_load_4d(sK + s * TILE + d * AT_BOX, &tmK, full, d * 64, (range.x + u) * AT_M, kvh, b);
+          tma_load_4d(sV + s * TILE + d * AT_BOX, &tmV, full, d * 64, (range.x + u) * AT_M, kvh, b);
+        }
+      }
+      if (!ok && p.status) *p.status = ST_TIMEOUT_EMPTY;
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && n > 0) {
+      const uint32_t id_s = make_idesc(128, 128, 1, 1, 0, 0), id_q = make_idesc(128, 64 * DB, 1, 1, 0, 1);
+      const int ks = (p.a.D + 15) / 16;
+      const uint32_t q = smem_u32(sQ), g = smem_u32(sG), k = smem_u32(sK), v = smem_u32(sV);
+      auto arrived = [&](int u) { return u == ragged ? mbar_wait(end_full, 0) && mbar_wait(k_clean, 0) : mbar_wait(kv_full + (u & 1), (u >> 1) & 1); };
+      bool ok = mbar_wait(q_full, 0) && arrived(0);
+      if (ok) {
+        tc_fence_after_sync();
+        scores_product(tmem, q, k, id_s, ks);
+        umma_commit(s_full);
+        scores_product(tmem + 128, g, v, id_s, ks);
+        umma_commit(dp_full);
+        for (int u = 0; u < n && ok; ++u) {
+          const int s = u & 1, t = s ^ 1;
+          const bool next = u + 1 < n;
+          if (next) {
+            ok = mbar_wait(s_read, u & 1) && arrived(u + 1);
+            if (!ok) break;
+            tc_fence_after_sync();
+            scores_product(tmem, q, k + t * TILE, id_s, ks);
+            umma_commit(s_full);
+          }
+          ok = mbar_wait(ds_ready, u & 1);
+          if (!ok) break;
+          tc_fence_after_sync();
+          rows_product<DB>(tmem + 256, tmem + 128, k + s * TILE, id_q, u > 0);
+          umma_commit(kv_empty + s);
+          if (next) {
+            scores_product(tmem + 128, g, v + t * TILE, id_s, ks);
+            umma_commit(dp_full);
+          }
+        }
+        if (ok) umma_commit(done);
+      }
+      if (!ok && p.status) *p.status = ST_TIMEOUT_FULL;
+    }
+  } else if (warp < 4) {
+    if (ragged >= 0 && ragged < n) {
+      const int s = ragged & 1, keep = vis.length % AT_M;
+      const bool ok = mbar_wait(end_full, 0);
+      if (ok)
+        for (int i = threadIdx.x - 64; i < TILE / 16; i += 64)
+          if (((i >> 3) & (AT_M - 1)) >= keep) reinterpret_cast<uint4*>(sK + s * TILE)[i] = make_uint4(0, 0, 0, 0);
+      fence_proxy_async_smem();
+      mbar_arrive(k_clean);
+      if (!ok && p.status) *p.status = ST_TIMEOUT_FULL;
+    }
+  } else {
+    const int half = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane, t = q0 + row;
+    const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+    const uint32_t tS = tmem + lane_base + half * 64, tP = tS + 128;
+    const int padded = (p.a.T + AT_M - 1) / AT_M * AT_M;
+    const long long at = ((long long)b * p.a.H + h) * padded + t;
+    const float lse = p.lse[at];
+    // delta: each half of the row's columns by one of its two threads
+    float dot = 0.f;
+    if (t < p.a.T) {
+      const uint4* o = reinterpret_cast<const uint4*>((const __nv_bfloat16*)p.out.p + b * p.out.sb + t * p.out.sr + h * p.out.sh);
+      const uint4* g = reinterpret_cast<const uint4*>((const __nv_bfloat16*)p.dout.p + b * p.dout.sb + t * p.dout.sr + h * p.dout.sh);
+      const int pieces = p.a.D / 8, mid = (pieces + 1) / 2;
+      for (int i = half * mid; i < (half == 0 ? mid : pieces); ++i) {
+        const uint4 x = o[i], y = g[i];
+        const uint32_t *xp = &x.x, *yp = &y.x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          dot = fmaf(__uint_as_float(xp[e] << 16), __uint_as_float(yp[e] << 16), dot);
+          dot = fmaf(__uint_as_float(xp[e] & 0xffff0000u), __uint_as_float(yp[e] & 0xffff0000u), dot);
+        }
+      }
+    }
+    if (half == 1) part[row] = dot;
+    named_barrier<256>(1);
+    if (half == 0) {
+      dot += part[row];
+      part[row] = dot;
+      p.delta[at] = dot;
+    }
+    named_barrier<256>(1);
+    const float delta = part[row];
+    const int lo = vis.low(t), hi = vis.high(t);
+    bool ok = true;
+    for (int u = 0; u < n; ++u) {
+      const int key = (range.x + u) * AT_M;
+      const bool masked = !vis.whole(q0, q0 + AT_M - 1, key);
+      const int c_lo = lo - key - half * 64, c_hi = hi - key - half * 64;
+      ok = mbar_wait(s_full, u & 1);
+      if (!ok) break;
+      tc_fence_after_sync();
+      uint32_t x[32], y[32];
+      load_half(tS, x, y);
+      tc_fence_before_sync();
+      mbar_arrive(s_read);
+      const uint64_t cc = pack_f2(p.scale2, p.scale2), mm = pack_f2(-lse, -lse);
+      auto weights = [&](uint32_t (&r)[32], int c0) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          float a, e;
+          unpack_f2(fma2(pack_f2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), cc, mm), a, e);
+          a = ex2(a);
+          e = ex2(e);
+          if (masked) {
+            a = c0 + i <= c_hi && c0 + i >= c_lo ? a : 0.f;
+            e = c0 + i + 1 <= c_hi && c0 + i + 1 >= c_lo ? e : 0.f;
+          }
+          r[i] = __float_as_uint(a);
+          r[i + 1] = __float_as_uint(e);
+        }
+      };
+      weights(x, 0);
+      weights(y, 32);
+      ok = mbar_wait(dp_full, u & 1);
+      if (!ok) break;
+      tc_fence_after_sync();
+      const uint64_t dd = pack_f2(-delta, -delta);
+      auto slopes = [&](uint32_t (&r)[32], int c0) {
+        uint32_t d[32], o[16];
+        tmem_ld_32x32b_x32(tP + c0, d);
+        tmem_ld_wait_regs(d);
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          float a, e;
+          unpack_f2(mul2(add2(pack_f2(__uint_as_float(d[i]), __uint_as_float(d[i + 1])), dd), pack_f2(__uint_as_float(r[i]), __uint_as_float(r[i + 1]))), a, e);
+          if (masked) {  // zero times what is no number
+            a = c0 + i <= c_hi && c0 + i >= c_lo ? a : 0.f;
+            e = c0 + i + 1 <= c_hi && c0 + i + 1 >= c_lo ? e : 0.f;
+          }
+          o[i / 2] = pack_bf16x2(a, e);
+        }
+        tmem_st_32x32b_x16(tP + c0 / 2, o);  // over columns that this thread has read
+      };
+      slopes(x, 0);
+      slopes(y, 32);
+      tmem_st_wait();
+      tc_fence_before_sync();
+      mbar_arrive(ds_ready);
+    }
+    if (ok && n > 0) ok = mbar_wait(done, 0);
+    tc_fence_after_sync();
+    __nv_bfloat16* o = p.dq + (((long long)b * p.a.T + t) * p.a.H + h) * p.a.D;
+    for (int c = half * 32 * DB; c < (half + 1) * 32 * DB; c += 16) {
+      uint32_t v[16] = {};
+      if (n > 0) {
+        tmem_ld_32x32b_x16(tmem + lane_base + 256 + c, v);
+        tmem_ld_wait();
+      }
+      if (t < p.a.T) store_row16(o, c, p.a.D, v, n > 0 ? p.a.scale : 0.f);
+    }
+    if (!ok && p.status) *p.status = ST_TIMEOUT_TMEM;
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  if (warp == 2) tmem_dealloc(tmem, 512);
+}
+
+// ---------------------------------------------------------------------------------------------------------------- keys, values
+template <int DB>
+__global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
+                                                                      const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                                                                      const BwdParams p) {
+  constexpr int TILE = DB * AT_BOX, STATS = 2 * AT_M * 4;  // lse and delta of a query tile
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  uint8_t *sK = smem, *sV = sK + TILE, *sQ = sV + TILE, *sG = sQ + 2 * TILE;
+  float* sStat = reinterpret_cast<float*>(sG + 2 * TILE);
+  __shared__ __align__(8) uint64_t bars[10];
+  uint64_t *kv_full = bars, *q_full = bars + 1, *q_empty = bars + 3, *s_full = bars + 5, *p_ready = bars + 6, *dp_full = bars + 7, *ds_ready = bars + 8,
+           *done = bars + 9;
+  __shared__ uint32_t tmem_slot;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kvh = blockIdx.x % p.a.G, b = blockIdx.x / p.a.G, rep = p.a.H / p.a.G;
+  const int k0 = blockIdx.y * AT_M;  // with a causal mask the first keys are seen by the most queries
+  const Visible vis(p.a, b);
+  const int first = vis.first(k0), last = vis.last(min(p.a.S, k0 + AT_M) - 1, p.a.T);
+  const int i0 = first / AT_M, per = k0 < vis.length && last >= first ? last / AT_M + 1 - i0 : 0, n = per * rep;
+  const int padded = (p.a.T + AT_M - 1) / AT_M * AT_M;
+
+  if (threadIdx.x == 0) {
+    mbar_init(kv_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(q_full + i, 1);
+      mbar_init(q_empty + i, 1);
+    }
+    mbar_init(s_full, 1);
+    mbar_init(p_ready, 256);
+    mbar_init(dp_full, 1);
+    mbar_init(ds_ready, 256);
+    mbar_init(done, 1);
+    mbar_fence_init();
+  }
+  if (warp == 2) {
+    tmem_alloc(&tmem_slot, 512);
+    tmem_relinquish();
+  }
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0 && n > 0) {
+      prefetch_tmap(&tmQ);
+      prefetch_tmap(&tmG);
+      prefetch_tmap(&tmK);
+      prefetch_tmap(&tmV);
+      mbar_expect_tx(kv_full, 2 * TILE);
+      for (int d = 0; d < DB; ++d) {
+        tma_load_4d(sK + d * AT_BOX, &tmK, kv_full, d * 64, k0, kvh, b);
+        tma_load_4d(sV + d * AT_BOX, &tmV, kv_full, d * 64, k0, kvh, b);
+      }
+      bool ok = true;
+      for (int u = 0; u < n && ok; ++u) {
+        const int s = u & 1, h = kvh * rep + u / per, t0 = (i0 + u % per) * AT_M;
+        if (u >= 2) ok = mbar_wait(q_empty + s, ((u >> 1) & 1) ^ 1);
+        if (!ok) break;
+        mbar_expect_tx(q_full + s, 2 * TILE + STATS);
+        for (int d = 0; d < DB; ++d) {
+          tma_load_4d(sQ + s * TILE + d * AT_BOX, &tmQ, q_full + s, d * 64, t0, h, b);
+          tma_load_4d(sG + s * TILE + d * AT_BOX, &tmG, q_full + s, d * 64, t0, h, b);
+        }
+        const long long at = ((long long)b * p.a.H + h) * padded + t0;
+        bulk_load(sStat + s * 2 * AT_M, p.lse + at, AT_M * 4, q_full + s);
+        bulk_load(sStat + s * 2 * AT_M + AT_M, p.delta + at, AT_M * 4, q_full + s);
+      }
+      if (!ok && p.status) *p.status = ST_TIMEOUT_EMPTY;
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && n > 0) {
+      const uint32_t id_s = make_idesc(128, 128, 1, 1, 0, 0), id_k = make_idesc(128, 64 * DB, 1, 1, 0, 1);
+      const int ks = (p.a.D + 15) / 16;
+      const uint32_t k = smem_u32(sK), v = smem_u32(sV), q = smem_u32(sQ), g = smem_u32(sG);
+      auto arrived = [&](int u) { return mbar_wait(q_full + (u & 1), (u >> 1) & 1); };
+      bool ok = mbar_wait(kv_full, 0) && arrived(0);
+      if (ok) {
+        tc_fence_after_sync();
+        scores_product(tmem, k, q, id_s, ks);
+        umma_commit(s_full);
+        scores_product(tmem + 128, v, g, id_s, ks);
+        umma_commit(dp_full);
+        for (int u = 0; u < n && ok; ++u) {
+          const int s = u & 1, t = s ^ 1;
+          const bool next = u + 1 < n;
+          ok = mbar_wait(p_ready, u & 1);
+          if (!ok) break;
+          tc_fence_after_sync();
+          rows_product<DB>(tmem + 256, tmem, g + s * TILE, id_k, u > 0);
+          if (next) {
+            ok = arrived(u + 1);
+            if (!ok) break;
+            tc_fence_after_sync();
+            scores_product(tmem, k, q + t * TILE, id_s, ks);  // behind the product that reads P
+            umma_commit(s_full);
+          }
+          ok = mbar_wait(ds_ready, u & 1);
+          if (!ok) break;
+          tc_fence_after_sync();
+          rows_product<DB>(tmem + 384, tmem + 128, q + s * TILE, id_k, u > 0);
+          umma_commit(q_empty + s);
+          if (next) {
+            scores_product(tmem + 128, v, g + t * TILE, id_s, ks);
+            umma_commit(dp_full);
+          }
+        }
+        if (ok) umma_commit(done);
+      }
+      if (!ok && p.status) *p.status = ST_TIMEOUT_FULL;
+    }
+  } else if (warp >= 4) {
+    const int half = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane, key = k0 + row;
+    const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+    const uint32_t tS = tmem + lane_base + half * 64, tP = tS + 128;
+    const bool inside = key < vis.length;
+    const int lo = inside ? vis.first(key) : p.a.T, hi = inside ? vis.last(key, p.a.T) : -1;  // queries that see this key
+    bool ok = true;
+    for (int u = 0; u < n; ++u) {
+      const int t0 = (i0 + u % per) * AT_M;
+      const bool masked = !vis.whole(t0, t0 + AT_M - 1, k0);
+      const int c_lo = lo - t0 - half * 64, c_hi = hi - t0 - half * 64;
+      const float4 *lse = reinterpret_cast<const float4*>(sStat + (u & 1) * 2 * AT_M + half * 64), *delta = lse + AT_M / 4;
+      ok = mbar_wait(q_full + (u & 1), (u >> 1) & 1) && mbar_wait(s_full, u & 1);
+      if (!ok) break;
+      tc_fence_after_sync();
+      uint32_t x[32], y[32];
+      load_half(tS, x, y);
+      const uint64_t cc = pack_f2(p.scale2, p.scale2);
+      auto weights = [&](uint32_t (&r)[32], int c0) {
+        uint32_t o[16];
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          const float4 z = lse[(c0 + i) / 4];
+          float a[4];
+          unpack_f2(fma2(pack_f2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), cc, pack_f2(-z.x, -z.y)), a[0], a[1]);
+          unpack_f2(fma2(pack_f2(__uint_as_float(r[i + 2]), __uint_as_float(r[i + 3])), cc, pack_f2(-z.z, -z.w)), a[2], a[3]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            a[e] = ex2(a[e]);
+            if (masked) a[e] = c0 + i + e <= c_hi && c0 + i + e >= c_lo ? a[e] : 0.f;
+            r[i + e] = __float_as_uint(a[e]);
+          }
+          o[i / 2] = pack_bf16x2(a[0], a[1]);
+          o[i / 2 + 1] = pack_bf16x2(a[2], a[3]);
+        }
+        tmem_st_32x32b_x16(tS + c0 / 2, o);
+      };
+      weights(x, 0);
+      weights(y, 32);
+      tmem_st_wait();
+      tc_fence_before_sync();
+      mbar_arrive(p_ready);
+      ok = mbar_wait(dp_full, u & 1);
+      if (!ok) break;
+      tc_fence_after_sync();
+      auto slopes = [&](uint32_t (&r)[32], int c0) {
+        uint32_t d[32], o[16];
+        tmem_ld_32x32b_x32(tP + c0, d);
+        tmem_ld_wait_regs(d);
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          const float4 z = delta[(c0 + i) / 4];
+          float a[4];
+          unpack_f2(mul2(add2(pack_f2(__uint_as_float(d[i]), __uint_as_float(d[i + 1])), pack_f2(-z.x, -z.y)),
+                         pack_f2(__uint_as_float(r[i]), __uint_as_float(r[i + 1]))), a[0], a[1]);
+          unpack_f2(mul2(add2(pack_f2(__uint_as_float(d[i + 2]), __uint_as_float(d[i + 3])), pack_f2(-z.z, -z.w)),
+                         pack_f2(__uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]))), a[2], a[3]);
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[e] = c0 + i + e <= c_hi && c0 + i + e >= c_lo ? a[e] : 0.f;
+          }
+          o[i / 2] = pack_bf16x2(a[0], a[1]);
+          o[i / 2 + 1] = pack_bf16x2(a[2], a[3]);
+        }
+        tmem_st_32x32b_x16(tP + c0 / 2, o);
+      };
+      slopes(x, 0);
+      slopes(y, 32);
+      tmem_st_wait();
+      tc_fence_before_sync();
+      mbar_arrive(ds_ready);
+    }
+    if (ok && n > 0) ok = mbar_wait(done, 0);
+    tc_fence_after_sync();
+    // the first half of the warps writes dV, the second dK
+    __nv_bfloat16* o = (half == 0 ? p.dv : p.dk) + (((long long)b * p.a.S + key) * p.a.G + kvh) * p.a.D;
+    const float f = half == 0 ? 1.f : p.a.scale;
+    for (int c = 0; c < 64 * DB; c += 16) {
+      uint32_t v[16] = {};
+      if (n > 0) {
+        tmem_ld_32x32b_x16(tmem + lane_base + 256 + half * 128 + c, v);
+        tmem_ld_wait();
+      }
+      if (!inside) {  // what keys past the length hold does not count
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = 0;
+      }
+      if (key < p.a.S) store_row16(o, c, p.a.D, v, n > 0 ? f : 0.f);
+    }
+    if (!ok && p.status) *p.status = ST_TIMEOUT_TMEM;
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  if (warp == 2) tmem_dealloc(tmem, 512);
+}
+
+template <int DB>
+void run_bwd(const AttentionBwd& f, cudaStream_t s) {
+  const AttentionShape& a = f.a;
+  constexpr int smem = 6 * DB * AT_BOX + 1024, smem_kv = smem + 2 * 2 * AT_M * 4;
+  const CUtensorMap tq = attention_map(f.q, a.D, a.T, a.H, a.B), tg = attention_map(f.dout, a.D, a.T, a.H, a.B),
+                    tk = attention_map(f.k, a.D, a.S, a.G, a.B), tv = attention_map(f.v, a.D, a.S, a.G, a.B);
+  const BwdParams p{a, f.out, f.dout, f.lse, f.delta, f.dq, f.dk, f.dv, a.scale * LOG2E, f.status};
+  static PerDeviceOnce once;
+  if (once.first_use()) {
+    cudaFuncSetAttribute(attention_dq_kernel<DB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaFuncSetAttribute(attention_dkv_kernel<DB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_kv);
+  }
+  attention_dq_kernel<DB><<<dim3(a.B * a.H, (a.T + AT_M - 1) / AT_M), BW_THREADS, smem, s>>>(tq, tg, tk, tv, p);
+  attention_check_launch("attention_dq");
+  attention_dkv_kernel<DB><<<dim3(a.B * a.G, (a.S + AT_M - 1) / AT_M), BW_THREADS, smem_kv, s>>>(tq, tg, tk, tv, p);
+  attention_check_launch("attention_dkv");
+}
+
+}  // namespace
+
+void launch_attention_bwd(const AttentionBwd& f, cudaStream_t s) {
+  if (f.a.D <= 64) run_bwd<1>(f, s);
+  else run_bwd<2>(f, s);
+}
+
+}  // namespace tb

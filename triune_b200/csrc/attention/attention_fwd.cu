@@ -1,0 +1,523 @@
+// Forward pass: o_i = sum_j p_ij v_j with p the softmax over the visible keys, on the tensor cores.
+//
+// A CTA has two groups of four softmax warps, each with a tile of 128 queries by 128 keys under way, so that one group's
+// exponentials run under the other group's products:
+//   * pairs (PAIR): the groups have two neighbouring query tiles and walk the same keys;
+//   * halves: both have the same query tile, one the even and one the odd key tiles, and are added up at the end. Taken where
+//     pairs would leave SMs idle; the keys may then also be split over CTAs (`splits`), whose parts a second kernel adds up.
+// Warp roles:
+//   warp 0      TMA producer: query tiles once, then two-stage rings of key and value tiles
+//   warp 1      tcgen05.mma: S_w = Q_w K^T into TMEM, O_w += P_w V with P_w read from TMEM
+//   warps 2-3   pass the value tiles on; in those where not all keys are visible to all queries, values that are no numbers, and
+//               those of keys past the sequence's length, are set to zero first, since zero weights would not take them out
+//   warps 4-7, 8-11   softmax, one query per thread (TMEM lane = query)
+// P (bf16: every weight is off by 2^-8 of itself at most, which averages out over the keys) takes the first half of its S columns. The
+// running maximum is lazy: sums are rescaled only when it has grown by more than 2^8. fp32 sums take the weights before rounding.
+// TMEM: columns 0-127 S_0, 128-255 S_1, 256-383 O_0, 384-511 O_1.
+#include <algorithm>
+
+#include "../common/per_device.h"
+#include "attention_tiles.cuh"
+
+namespace tb {
+namespace {
+
+constexpr int FW_THREADS = 384;
+constexpr float FW_LAZY = 8.f;
+
+struct FwdParams {
+  AttentionShape a;
+  __nv_bfloat16* out;
+  float* lse;
+  float* part;  // [splits, B, H, T, 64 * DB] sums, then [splits, B, H, T, 2] maxima and weights
+  const __nv_bfloat16* v;
+  long long vr, vh, vb;
+  int splits;
+  float scale2;  // scale * log2(e)
+  int* status;
+};
+
+template <int DB, bool PAIR>
+__global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                                                                      const __grid_constant__ CUtensorMap tmV, const FwdParams p) {
+  constexpr int QT = PAIR ? 2 : 1, TILE = DB * AT_BOX;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  uint8_t *sQ = smem, *sK = sQ + QT * TILE, *sV = sK + 2 * TILE;
+  __shared__ __align__(8) uint64_t bars[17];
+  uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 7, *s_full = bars + 9, *p_ready = bars + 11,
+           *o_full = bars + 13, *v_clean = bars + 15;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int special;  // a value that is no number was set to zero
+  __shared__ float2 other[AT_M];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int h = blockIdx.x % p.a.H, b = blockIdx.x / p.a.H, kvh = h / (p.a.H / p.a.G);
+  const int q0 = (gridDim.y - 1 - blockIdx.y) * QT * AT_M;  // the rows with the most keys start first
+  const Visible vis(p.a, b);
+  // key tiles of the two groups: group w takes tiles x, x + step, ... below y
+  constexpr int step = PAIR ? 1 : 2;
+  int2 range[2];
+  int j0, j1;
+  if constexpr (PAIR) {
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const int t0 = q0 + w * AT_M;
+      range[w] = t0 < p.a.T ? vis.tiles(t0, min(p.a.T, t0 + AT_M) - 1) : make_int2(0, 0);
+    }
+    const bool e0 = range[0].x == range[0].y, e1 = range[1].x == range[1].y;
+    j0 = e0 ? range[1].x : e1 ? range[0].x : min(range[0].x, range[1].x);
+    j1 = e0 ? range[1].y : e1 ? range[0].y : max(range[0].y, range[1].y);
+  } else {
+    const int2 all = vis.tiles(q0, min(p.a.T, q0 + AT_M) - 1);
+    const int n = all.y - all.x, per = (n + p.splits - 1) / p.splits;
+    j0 = min(all.y, all.x + (int)blockIdx.z * per);
+    j1 = min(all.y, j0 + per);
+    range[0] = make_int2(j0, j1);
+    range[1] = make_int2(min(j0 + 1, j1), j1);
+  }
+  auto count = [&](int w) { return (range[w].y - range[w].x + step - 1) / step; };
+  auto takes = [&](int w, int j) { return PAIR ? j >= range[w].x && j < range[w].y : ((j - j0) & 1) == w; };
+  // tiles whose values are looked through; the queries past T take part, so this holds for whole query tiles
+  auto partial = [&](int j) {
+    bool some = false;
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+      if (takes(w, j)) some = some || !vis.whole(q0 + (PAIR ? w : 0) * AT_M, q0 + (PAIR ? w : 0) * AT_M + AT_M - 1, j * AT_M);
+    return some;
+  };
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(k_full + i, 1);
+      mbar_init(k_empty + i, 1);
+      mbar_init(v_full + i, 1);
+      mbar_init(v_empty + i, 1);
+      mbar_init(s_full + i, 1);
+      mbar_init(p_ready + i, 128);
+      mbar_init(o_full + i, 1);
+      mbar_init(v_clean + i, 64);
+    }
+    mbar_fence_init();
+    special = 0;
+  }
+  if (warp == 2) {
+    tmem_alloc(&tmem_slot, 512);
+    tmem_relinquish();
+  }
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0 && j1 > j0) {
+      prefetch_tmap(&tmQ);
+      prefetch_tmap(&tmK);
+      prefetch_tmap(&tmV);
+      mbar_expect_tx(q_full, QT * TILE);
+      for (int w = 0; w < QT; ++w)
+        for (int d = 0; d < DB; ++d) tma_load_4d(sQ + w * TILE + d * AT_BOX, &tmQ, q_full, d * 64, q0 + w * AT_M, h, b);
+      bool ok = true;
+      // keys run one tile ahead of values: the scores of the next tile are issued before the use of these values ends
+      for (int u = 0; u <= j1 - j0 && ok; ++u) {
+        if (u < j1 - j0) {
+          const int s = u & 1;
+          if (u >= 2) ok = mbar_wait(k_empty + s, ((u >> 1) & 1) ^ 1);
+          if (!ok) break;
+          mbar_expect_tx(k_full + s, TILE);
+          for (int d = 0; d < DB; ++d) tma_load_4d(sK + s * TILE + d * AT_BOX, &tmK, k_full + s, d * 64, (j0 + u) * AT_M, kvh, b);
+        }
+        if (u > 0) {
+          const int i = u - 1, s = i & 1;
+          if (i >= 2) ok = mbar_wait(v_empty + s, ((i >> 1) & 1) ^ 1);
+          if (!ok) break;
+          mbar_expect_tx(v_full + s, TILE);
+          for (int d = 0; d < DB; ++d) tma_load_4d(sV + s * TILE + d * AT_BOX, &tmV, v_full + s, d * 64, (j0 + i) * AT_M, kvh, b);
+        }
+      }
+      if (!ok && p.status) *p.status = ST_TIMEOUT_EMPTY;
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && j1 > j0) {
+      const uint32_t id_s = make_idesc(128, 128, 1, 1, 0, 0), id_o = make_idesc(128, 64 * DB, 1, 1, 0, 1);
+      const int ks = (p.a.D + 15) / 16;
+      auto scores = [&](int w, int j) {
+        const uint32_t qa = smem_u32(sQ + (PAIR ? w : 0) * TILE), ka = smem_u32(sK + ((j - j0) & 1) * TILE);
+        for (int k = 0; k < ks; ++k) {
+          const uint32_t off = (k >> 2) * AT_BOX + (k & 3) * 32;
+          umma_bf16(tmem + w * 128, make_smem_desc(qa + off, 16, 1024), make_smem_desc(ka + off, 16, 1024), id_s, k > 0);
+        }
+        umma_commit(s_full + w);
+      };
+      auto values = [&](int w, int j) {
+        const uint32_t va = smem_u32(sV + ((j - j0) & 1) * TILE);
+#pragma unroll
+        for (int k = 0; k < AT_M / 16; ++k)
+          umma_bf16_ts(tmem + 256 + w * 128, tmem + w * 128 + k * 8, make_smem_desc(va + k * 2048, AT_BOX, 1024), id_o, j != range[w].x || k > 0);
+      };
+      int done[2] = {0, 0};
+      auto k_arrived = [&](int j) { return mbar_wait(k_full + ((j - j0) & 1), ((j - j0) >> 1) & 1); };
+      bool ok = mbar_wait(q_full, 0) && k_arrived(j0);
+      if (ok) {
+        tc_fence_after_sync();
+        if constexpr (PAIR) {
+          for (int w = 0; w < 2; ++w)
+            if (takes(w, j0)) scores(w, j0);
+          umma_commit(k_empty);
+        } else {
+          scores(0, j0);
+          umma_commit(k_empty);
+          if (j1 - j0 > 1) {
+            ok = k_arrived(j0 + 1);
+            if (ok) {
+              tc_fence_after_sync();
+              scores(1, j0 + 1);
+              umma_commit(k_empty + 1);
+            }
+          }
+        }
+        for (int j = j0; j < j1 && ok; ++j) {
+          const int s = (j - j0) & 1;
+          ok = mbar_wait(v_clean + s, ((j - j0) >> 1) & 1);
+          const int jn = j + step;  // the next tile whose scores are issued
+          if (ok && jn < j1) ok = k_arrived(jn);
+          for (int w = 0; w < 2 && ok; ++w) {
+            const bool now = takes(w, j), next = jn < j1 && (PAIR ? takes(w, jn) : now);
+            if (now) {
+              ok = mbar_wait(p_ready + w, done[w] & 1);
+              ++done[w];
+              if (!ok) break;
+              tc_fence_after_sync();
+              values(w, j);
+              if (done[w] == count(w)) umma_commit(o_full + w);
+            }
+            if (next) scores(w, jn);
+          }
+          if (!ok) break;
+          umma_commit(v_empty + s);
+          if (jn < j1) umma_commit(k_empty + ((jn - j0) & 1));
+        }
+      }
+      if (!ok && p.status) *p.status = ST_TIMEOUT_FULL;
+    }
+  } else if (warp < 4) {
+    const int tid = threadIdx.x - 64;
+    bool ok = true;
+    for (int j = j0; j < j1 && ok; ++j) {
+      const bool look = partial(j);
+      const int s = (j - j0) & 1, keep = vis.length - j * AT_M;
+      ok = mbar_wait(v_full + s, ((j - j0) >> 1) & 1);
+      if (!ok) break;
+      bool found = false;
+      for (int i = look ? tid : TILE; i < TILE / 16; i += 64) {
+        uint4* x = reinterpret_cast<uint4*>(sV + s * TILE) + i;
+        const int row = (i >> 3) & (AT_M - 1);  // 128-byte rows; the swizzle stays within them
+        if (row >= keep) {
+          *x = make_uint4(0, 0, 0, 0);
+          continue;
+        }
+        uint4 y = *x;
+        uint32_t* w = &y.x;
+        bool bad = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (bf16x2_special(w[e])) {
+            bad = true;
+            if ((w[e] & 0x7f80u) == 0x7f80u) w[e] &= 0xffff0000u;
+            if ((w[e] & 0x7f800000u) == 0x7f800000u) w[e] &= 0x0000ffffu;
+          }
+        if (bad) *x = y;
+        found = found || bad;
+      }
+      if (found) special = 1;
+      fence_proxy_async_smem();
+      mbar_arrive(v_clean + s);
+    }
+    if (!ok && p.status) *p.status = ST_TIMEOUT_FULL;
+  } else {
+    const int w = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    const int first = q0 + (PAIR ? w : 0) * AT_M, t = first + row;
+    const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+    const uint32_t tS = tmem + lane_base + w * 128, tO = tmem + lane_base + 256 + w * 128;
+    const float c2 = p.scale2;
+    const int n = count(w), lo = vis.low(t), hi = vis.high(t);
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int it = 0; it < n; ++it) {
+      const int j = range[w].x + it * step;
+      ok = mbar_wait(s_full + w, it & 1);
+      if (!ok) break;
+      tc_fence_after_sync();
+      const bool masked = !vis.whole(first, first + AT_M - 1, j * AT_M);
+      const int c_lo = lo - j * AT_M, c_hi = hi - j * AT_M;  // visible columns
+      uint32_t ra[32], rb[32];
+      float mx = -INFINITY;
+      auto row_max = [&](uint32_t (&r)[32], int c0) {
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (c0 + i <= c_hi && c0 + i >= c_lo) mx = fmaxf(mx, __uint_as_float(r[i]));
+        } else {
+          float x0 = __uint_as_float(r[0]), x1 = __uint_as_float(r[1]), x2 = __uint_as_float(r[2]), x3 = __uint_as_float(r[3]);
+#pragma unroll
+          for (int i = 4; i < 32; i += 4) {
+            x0 = fmaxf(x0, __uint_as_float(r[i]));
+            x1 = fmaxf(x1, __uint_as_float(r[i + 1]));
+            x2 = fmaxf(x2, __uint_as_float(r[i + 2]));
+            x3 = fmaxf(x3, __uint_as_float(r[i + 3]));
+          }
+          mx = fmaxf(mx, fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)));
+        }
+      };
+      tmem_ld_32x32b_x32(tS, ra);
+      tmem_ld_wait_regs(ra);
+      tmem_ld_32x32b_x32(tS + 32, rb);
+      row_max(ra, 0);
+      tmem_ld_wait_regs(rb);
+      tmem_ld_32x32b_x32(tS + 64, ra);
+      row_max(rb, 32);
+      tmem_ld_wait_regs(ra);
+      tmem_ld_32x32b_x32(tS + 96, rb);
+      row_max(ra, 64);
+      tmem_ld_wait_regs(rb);
+      tmem_ld_32x32b_x32(tS, ra);  // the first columns again, for the exponentials
+      row_max(rb, 96);
+      const float mn = fmaxf(m, mx * c2);
+      const bool grow = mn > m && (m == -INFINITY || mn - m > FW_LAZY);
+      float f = 1.f;
+      if (grow) {
+        f = m == -INFINITY ? 0.f : ex2(m - mn);  // sums over invisible keys so far are zero
+        m = mn;
+        l *= f;
+      }
+      tmem_ld_wait_regs(ra);
+      if (it > 0 && __any_sync(0xffffffffu, grow)) {
+        for (int c = 0; c < 64 * DB; c += 16) {
+          uint32_t o[16];
+          tmem_ld_32x32b_x16(tO + c, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+          tmem_st_32x32b_x16(tO + c, o);
+        }
+        tmem_st_wait();
+      }
+      const float ms = m == -INFINITY ? 0.f : m;  // no visible key yet: the weights are masked, or no numbers
+      const uint64_t cc = pack_f2(c2, c2), mm = pack_f2(-ms, -ms);
+      uint64_t sum2 = pack_f2(0.f, 0.f);
+      auto weights = [&](uint32_t (&r)[32], int c0) {
+        uint32_t q[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float x, e;
+          unpack_f2(fma2(pack_f2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), cc, mm), x, e);
+          x = ex2(x);
+          e = ex2(e);
+          if (masked) {
+            const int c = c0 + 2 * i;
+            x = c <= c_hi && c >= c_lo ? x : 0.f;
+            e = c + 1 <= c_hi && c + 1 >= c_lo ? e : 0.f;
+          }
+          sum2 = add2(sum2, pack_f2(x, e));
+          q[i] = pack_bf16x2(x, e);
+        }
+        tmem_st_32x32b_x16(tS + c0 / 2, q);  // lands in columns whose scores this thread has already read
+      };
+      tmem_ld_32x32b_x32(tS + 32, rb);
+      weights(ra, 0);
+      tmem_ld_wait_regs(rb);
+      tmem_ld_32x32b_x32(tS + 64, ra);
+      weights(rb, 32);
+      tmem_ld_wait_regs(ra);
+      tmem_ld_32x32b_x32(tS + 96, rb);
+      weights(ra, 64);
+      tmem_ld_wait_regs(rb);
+      weights(rb, 96);
+      float s0, s1;
+      unpack_f2(sum2, s0, s1);
+      l += s0 + s1;
+      tmem_st_wait();
+      tc_fence_before_sync();
+      mbar_arrive(p_ready + w);
+    }
+    if (ok && n > 0) ok = mbar_wait(o_full + w, 0);
+    tc_fence_after_sync();
+    float share = 1.f;  // of this group's sums in the row
+    float* half = reinterpret_cast<float*>(sK);
+    if constexpr (!PAIR) {
+      // the second group hands its sums over through the key tiles, which no product reads any more
+      const bool both = count(1) > 0;
+      if (w == 1 && both) {
+        other[row] = make_float2(m, l);
+        for (int c = 0; c < 64 * DB; c += 16) {
+          uint32_t o[16];
+          tmem_ld_32x32b_x16(tO + c, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) half[(c + i) * AT_M + row] = __uint_as_float(o[i]);
+        }
+      }
+      if (both) named_barrier<256>(1);
+    }
+    if (PAIR || w == 0) {
+      float r1 = 0.f;
+      const bool both = !PAIR && count(1) > 0;
+      if (both) {
+        const float2 o = other[row];
+        const float mn = fmaxf(m, o.x);
+        share = m == -INFINITY ? 0.f : ex2(m - mn);
+        r1 = o.x == -INFINITY ? 0.f : ex2(o.x - mn);
+        // a row whose scores were no numbers has a sum that is none, whatever its maximum
+        l = (m == -INFINITY && l == l ? 0.f : l * (m == -INFINITY ? 1.f : share)) + (o.x == -INFINITY && o.y == o.y ? 0.f : o.y * (o.x == -INFINITY ? 1.f : r1));
+        m = mn;
+      }
+      const bool split = !PAIR && p.splits > 1;
+      const float r = split ? 1.f : l == 0.f ? 0.f : 1.f / l;
+      const bool inside = t < p.a.T;
+      const long long row_at = ((long long)b * p.a.H + h) * p.a.T + t;
+      const int padded = (p.a.T + AT_M - 1) / AT_M * AT_M;
+      if (p.lse != nullptr && !split && t < padded) p.lse[((long long)b * p.a.H + h) * padded + t] = inside && l != 0.f ? m + log2f(l) : INFINITY;
+      if (split && inside) {
+        const long long rows = (long long)p.a.B * p.a.H * p.a.T;
+        float2* ml = reinterpret_cast<float2*>(p.part + p.splits * rows * 64 * DB);
+        ml[blockIdx.z * rows + row_at] = make_float2(m, l);
+      }
+      __nv_bfloat16* o = p.out + (((long long)b * p.a.T + t) * p.a.H + h) * p.a.D;
+      float* po = p.part + ((long long)blockIdx.z * p.a.B * p.a.H * p.a.T + row_at) * 64 * DB;
+      const bool any = n > 0;
+      for (int c = 0; c < 64 * DB; c += 16) {
+        uint32_t x[16];
+        if (any) {
+          tmem_ld_32x32b_x16(tO + c, x);
+          tmem_ld_wait();
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float y = any ? __uint_as_float(x[i]) : 0.f;
+          if (both) y = y * share + half[(c + i) * AT_M + row] * r1;
+          x[i] = __float_as_uint(y);
+        }
+        if (special != 0 && inside) {
+          // values that are no numbers were left out of the products of the tiles that are not whole: for the rows that see them
+          // they are added here, whatever their (positive) weight
+          for (int j = j0; j < j1; ++j) {
+            if (!partial(j)) continue;
+            const int k0 = max(lo, j * AT_M), k1 = min(hi, j * AT_M + AT_M - 1);
+            for (int k = k0; k <= k1; ++k)
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                if (c + i < p.a.D) {
+                  const float y = __bfloat162float(p.v[b * p.vb + k * p.vr + kvh * p.vh + c + i]);
+                  if (!isfinite(y)) x[i] = __float_as_uint(__uint_as_float(x[i]) + y);
+                }
+          }
+        }
+        if (!inside) continue;
+        if (split) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) reinterpret_cast<uint4*>(po + c)[g] = make_uint4(x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]);
+        } else {
+          store_row16(o, c, p.a.D, x, r);
+        }
+      }
+    }
+    if (!ok && p.status) *p.status = ST_TIMEOUT_TMEM;
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  if (warp == 2) tmem_dealloc(tmem, 512);
+}
+
+// Parts of rows whose keys were split over CTAs: a warp per row.
+template <int DB>
+__global__ void __launch_bounds__(256) attention_join_kernel(const FwdParams p) {
+  const long long rows = (long long)p.a.B * p.a.H * p.a.T, row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= rows) return;
+  const float2* ml = reinterpret_cast<const float2*>(p.part + p.splits * rows * 64 * DB);
+  float m = -INFINITY;
+  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, ml[s * rows + row].x);
+  float l = 0.f, acc[2 * DB] = {};
+  for (int s = 0; s < p.splits; ++s) {
+    const float2 x = ml[s * rows + row];
+    const float f = x.x == -INFINITY ? (x.y == x.y ? 0.f : 1.f) : ex2(x.x - m);
+    if (f == 0.f && x.y == x.y) continue;  // nothing visible there (its sums may not have been formed), or nothing that counts
+    l += x.y * f;
+#pragma unroll
+    for (int i = 0; i < 2 * DB; ++i) acc[i] += p.part[(s * rows + row) * 64 * DB + lane + 32 * i] * f;
+  }
+  const int t = row % p.a.T, h = row / p.a.T % p.a.H;
+  const long long b = row / ((long long)p.a.T * p.a.H);
+  const float r = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int i = 0; i < 2 * DB; ++i)
+    if (lane + 32 * i < p.a.D) p.out[((b * p.a.T + t) * p.a.H + h) * p.a.D + lane + 32 * i] = __float2bfloat16(acc[i] * r);
+  if (p.lse != nullptr && lane == 0) {
+    const int padded = (p.a.T + AT_M - 1) / AT_M * AT_M;
+    float* at = p.lse + row / p.a.T * padded;
+    at[t] = l != 0.f ? m + log2f(l) : INFINITY;
+    if (t == p.a.T - 1)
+      for (int i = p.a.T; i < padded; ++i) at[i] = INFINITY;
+  }
+}
+
+int multiprocessors() {
+  static int count[PerDeviceOnce::kMaxDevices] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= PerDeviceOnce::kMaxDevices) return 148;
+  if (count[dev] == 0) cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev);
+  return count[dev];
+}
+
+// Pairs where they give every SM a CTA; else halves, with the keys split so far that the CTAs fill the SMs once, each with two key
+// tiles at least.
+int fwd_splits(const AttentionShape& a, bool& pair) {
+  const int sms = multiprocessors();
+  const long long heads = (long long)a.B * a.H, tiles = (a.T + AT_M - 1) / AT_M;
+  pair = heads * ((tiles + 1) / 2) >= sms;
+  if (pair) return 1;
+  const long long most = std::max(1, (a.S + AT_M - 1) / AT_M / 2);
+  return (int)std::max<long long>(1, std::min({sms / (heads * tiles), most, 32ll}));
+}
+
+template <int DB, bool PAIR>
+void run(const FwdParams& p, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t s) {
+  constexpr int QT = PAIR ? 2 : 1, smem = (QT + 4) * DB * AT_BOX + 1024;
+  static PerDeviceOnce once;
+  auto kern = attention_fwd_kernel<DB, PAIR>;
+  if (once.first_use()) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  kern<<<dim3(p.a.B * p.a.H, (p.a.T + QT * AT_M - 1) / (QT * AT_M), p.splits), FW_THREADS, smem, s>>>(tq, tk, tv, p);
+  attention_check_launch("attention_fwd");
+}
+
+template <int DB>
+void run_width(const AttentionFwd& f, cudaStream_t s) {
+  const AttentionShape& a = f.a;
+  const CUtensorMap tq = attention_map(f.q, a.D, a.T, a.H, a.B), tk = attention_map(f.k, a.D, a.S, a.G, a.B), tv = attention_map(f.v, a.D, a.S, a.G, a.B);
+  bool pair;
+  FwdParams p{a, f.out, f.lse, f.part, (const __nv_bfloat16*)f.v.p, f.v.sr, f.v.sh, f.v.sb, fwd_splits(a, pair), a.scale * LOG2E, f.status};
+  if (pair) return run<DB, true>(p, tq, tk, tv, s);
+  run<DB, false>(p, tq, tk, tv, s);
+  if (p.splits > 1) {
+    const long long rows = (long long)a.B * a.H * a.T;
+    attention_join_kernel<DB><<<(unsigned)((rows + 7) / 8), 256, 0, s>>>(p);
+    attention_check_launch("attention_join");
+  }
+}
+
+}  // namespace
+
+long long attention_fwd_scratch(const AttentionShape& a) {
+  bool pair;
+  const int splits = fwd_splits(a, pair);
+  return splits > 1 ? (long long)splits * a.B * a.H * a.T * ((a.D <= 64 ? 64 : 128) + 2) * 4 : 0;
+}
+
+void launch_attention_fwd(const AttentionFwd& f, cudaStream_t s) {
+  if (f.a.D <= 64) run_width<1>(f, s);
+  else run_width<2>(f, s);
+}
+
+}  // namespace tb

@@ -1,0 +1,160 @@
+// Tokens into and out of the 8-bit cache. Both kernels pass over the data once, a CTA per block of 64 tokens of one head, of keys or
+// of values; rows are read and written in 16-byte pieces (codes in 8-byte pieces).
+#include <cuda_fp8.h>
+
+#include "kv8.cuh"
+
+namespace tb {
+namespace {
+
+struct AppendParams {
+  Kv8Cache c;
+  AttentionView k, v;
+  int T, D, blocks;
+  Kv8Pos pos;
+};
+
+__device__ __forceinline__ long long pos_at(const Kv8Pos& p, int b) { return p.dev != nullptr ? p.dev[(long long)b * p.step] : p.host; }
+
+template <bool E4M3>
+__device__ __forceinline__ uint32_t code_of(float x, float s) {
+  const float y = s > 0.f ? __fdiv_rn(x, s) : 0.f;  // the whole block is zero, or reads as NaN whatever its codes
+  if constexpr (E4M3) return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+  return (uint32_t)__float2int_rn(y) & 0xffu;
+}
+
+// A thread has PIECES pieces of 8 columns of a block.
+template <int P, bool E4M3>
+__global__ void __launch_bounds__(256) kv8_append_kernel(const AppendParams p) {
+  constexpr int ACROSS = P / 8, PIECES = KV8_BLOCK * ACROSS / 256;
+  __shared__ uint32_t most[8];
+  long long at = blockIdx.x;
+  const int i = at % p.blocks;
+  at /= p.blocks;
+  const int side = at & 1;
+  at >>= 1;
+  const int g = at % p.c.G, b = at / p.c.G;
+  const long long start = pos_at(p.pos, b);
+  if (start < 0 || start >= p.c.C) return;
+  const int begin = (int)start, end = (int)min((long long)p.c.C, start + p.T);
+  const int m = begin / KV8_BLOCK + i, base = m * KV8_BLOCK;
+  if (base >= end) return;
+  const long long head = (long long)b * p.c.G + g;
+  const AttentionView& x = side ? p.v : p.k;
+  const __nv_bfloat16* rows = (const __nv_bfloat16*)x.p + b * x.sb + g * x.sh;
+  uint4* ring = reinterpret_cast<uint4*>((side ? p.c.vt : p.c.kt) + head * KV8_RING * P);
+  auto token = [&](int pos, int piece) {  // of the new ones
+    return piece * 8 < p.D ? *reinterpret_cast<const uint4*>(rows + (long long)(pos - begin) * x.sr + piece * 8) : make_uint4(0, 0, 0, 0);
+  };
+  if (base + KV8_BLOCK <= end) {
+    uint4 z[PIECES];
+    uint32_t top = 0;  // magnitudes of bf16 numbers order like their bits, infinities and NaN above all
+#pragma unroll
+    for (int e = 0; e < PIECES; ++e) {
+      const int at = threadIdx.x + 256 * e, row = at / ACROSS, piece = at % ACROSS;
+      z[e] = base + row < begin ? ring[(m & 1) * KV8_BLOCK * ACROSS + at] : token(base + row, piece);
+      const uint32_t* w = &z[e].x;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) top = max(top, most[w]);
+    const float s = top >= 0x7f80u ? __int_as_float(0x7fc00000) : __fdiv_rn(__uint_as_float(top << 16), E4M3 ? 448.f : 127.f);
+    if (threadIdx.x == 0) (side ? p.c.vs : p.c.ks)[head * (p.c.C / KV8_BLOCK) + m] = s;
+    uint2* codes = reinterpret_cast<uint2*>((side ? p.c.v8 : p.c.k8) + (head * p.c.C + base) * P);
+#pragma unroll
+    for (int e = 0; e < PIECES; ++e) {
+      const uint32_t* w = &z[e].x;
+      uint32_t o[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        o[k] = code_of<E4M3>(__uint_as_float(w[2 * k] << 16), s) | code_of<E4M3>(__uint_as_float(w[2 * k] & 0xffff0000u), s) << 8 |
+               code_of<E4M3>(__uint_as_float(w[2 * k + 1] << 16), s) << 16 | code_of<E4M3>(__uint_as_float(w[2 * k + 1] & 0xffff0000u), s) << 24;
+      codes[threadIdx.x + 256 * e] = make_uint2(o[0], o[1]);
+    }
+  }
+  // The first two blocks write the ring, each its half: the newest token of every row. The first block's threads have read the old
+  // rows of their own places above.
+  if (i < 2) {
+#pragma unroll
+    for (int e = 0; e < PIECES; ++e) {
+      const int at = threadIdx.x + 256 * e, row = at / ACROSS, slot = (m & 1) * KV8_BLOCK + row;
+      const int pos = end - 1 - ((end - 1 - slot) & (KV8_RING - 1));
+      if (pos >= begin) ring[(m & 1) * KV8_BLOCK * ACROSS + at] = token(pos, at % ACROSS);
+    }
+  }
+}
+
+struct ExpandParams {
+  Kv8Cache c;
+  __nv_bfloat16 *k, *v;
+  int rows, D, blocks;
+  Kv8Pos length;
+};
+
+template <int P, bool E4M3>
+__global__ void __launch_bounds__(256) kv8_expand_kernel(const ExpandParams p) {
+  constexpr int ACROSS = P / 8, PIECES = KV8_BLOCK * ACROSS / 256;
+  long long at = blockIdx.x;
+  const int m = at % p.blocks;
+  at /= p.blocks;
+  const int side = at & 1;
+  at >>= 1;  // head
+  const long long given = pos_at(p.length, at / p.c.G);
+  const int n = (int)max(0ll, min(given, (long long)p.c.C)), base = m * KV8_BLOCK;
+  const bool full = base + KV8_BLOCK <= n;
+  __nv_bfloat16* out = (side ? p.v : p.k) + (at * p.rows + base) * p.D;
+  const uint2* codes = reinterpret_cast<const uint2*>((side ? p.c.v8 : p.c.k8) + (at * p.c.C + base) * P);
+  const uint4* ring = reinterpret_cast<const uint4*>((side ? p.c.vt : p.c.kt) + (at * KV8_RING + (m & 1) * KV8_BLOCK) * P);
+  const float s = full ? (side ? p.c.vs : p.c.ks)[at * (p.c.C / KV8_BLOCK) + m] : 0.f;
+#pragma unroll
+  for (int e = 0; e < PIECES; ++e) {
+    const int i = threadIdx.x + 256 * e, row = i / ACROSS, piece = i % ACROSS;
+    if (base + row >= p.rows || piece * 8 >= p.D) continue;
+    uint4 z = make_uint4(0, 0, 0, 0);
+    if (full) {
+      const uint2 c = codes[i];
+      float x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t byte = ((k < 4 ? c.x : c.y) >> (8 * (k & 3))) & 0xffu;
+        if constexpr (E4M3) x[k] = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));
+        else x[k] = (float)(int8_t)byte;
+      }
+      uint32_t* w = &z.x;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const __nv_bfloat162 y = __floats2bfloat162_rn(x[2 * k] * s, x[2 * k + 1] * s);
+        w[k] = *reinterpret_cast<const uint32_t*>(&y);
+      }
+    } else if (base + row < n) {
+      z = ring[i];
+    }
+    *reinterpret_cast<uint4*>(out + (long long)row * p.D + piece * 8) = z;
+  }
+}
+
+}  // namespace
+
+void launch_kv8_append(const Kv8Cache& c, const AttentionView& k, const AttentionView& v, int T, int D, const Kv8Pos& pos, cudaStream_t s) {
+  const int blocks = (T + KV8_BLOCK - 2) / KV8_BLOCK + 1;  // that T tokens can touch
+  const AppendParams p{c, k, v, T, D, blocks, pos};
+  const unsigned grid = (unsigned)((long long)blocks * 2 * c.B * c.G);
+  if (c.P == 64) (c.e4m3 ? kv8_append_kernel<64, true> : kv8_append_kernel<64, false>)<<<grid, 256, 0, s>>>(p);
+  else (c.e4m3 ? kv8_append_kernel<128, true> : kv8_append_kernel<128, false>)<<<grid, 256, 0, s>>>(p);
+  attention_check_launch("kv8_append");
+}
+
+void launch_kv8_expand(const Kv8Cache& c, __nv_bfloat16* k, __nv_bfloat16* v, int rows, int D, const Kv8Pos& length, cudaStream_t s) {
+  const int blocks = (rows + KV8_BLOCK - 1) / KV8_BLOCK;
+  const ExpandParams p{c, k, v, rows, D, blocks, length};
+  const unsigned grid = (unsigned)((long long)blocks * 2 * c.B * c.G);
+  if (c.P == 64) (c.e4m3 ? kv8_expand_kernel<64, true> : kv8_expand_kernel<64, false>)<<<grid, 256, 0, s>>>(p);
+  else (c.e4m3 ? kv8_expand_kernel<128, true> : kv8_expand_kernel<128, false>)<<<grid, 256, 0, s>>>(p);
+  attention_check_launch("kv8_expand");
+}
+
+}  // namespace tb

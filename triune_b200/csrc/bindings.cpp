@@ -498,6 +498,7 @@ void register_decode(pybind11::module& m);
 void register_block(pybind11::module& m);
 void register_hybrid(pybind11::module& m);
 void register_gla(pybind11::module& m);
+void register_attention(pybind11::module& m);
 void register_quant(pybind11::module& m);
 void register_comm(pybind11::module& m);
 
@@ -541,6 +542,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("neuron_heatmap", &neuron_heatmap);
   m.def("tier_render", &tier_render);
   register_gla(m);
+  register_attention(m);
   register_quant(m);
   register_comm(m);
   register_hybrid(m);

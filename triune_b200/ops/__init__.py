@@ -1170,3 +1170,7 @@ def lora_linear(x, w, bias, A, B, scaling: float):
             and r % 8 == 0 and w.shape[0] % 8 == 0 and w.shape[1] % 8 == 0 and not w.requires_grad):
         return _LoRALinearFn.apply(x, w, bias, A, B, scaling)
     return F.linear(x, w, bias) + F.linear(F.linear(x, A), B) * scaling
+
+
+# at the end: it builds on the names above
+from .softmax_attention import attention, attention_supported, kv8_append, kv8_attention, kv8_cache, kv8_expand, kv8_kind  # noqa: E402,F401

@@ -21,7 +21,7 @@ Semantics follow the reference project (paths relative to its root):
 from __future__ import annotations
 
 import math
-from typing import Optional, Tuple
+from typing import List, Optional, Tuple
 
 import torch
 import torch.nn.functional as F
@@ -723,3 +723,110 @@ def moe_capacity_mask(idx: torch.Tensor, w: torch.Tensor, num_experts: int, capa
         tok = order[order2]
         keep[tok, j] = rank < capacity
     return keep
+
+
+# ----------------------------------------------------------------------------
+# Softmax attention, and its cache in 8 bits
+# ----------------------------------------------------------------------------
+KV8_BLOCK, KV8_RING = 64, 128  # tokens that share a scale; tokens that are kept as they came
+
+
+def _per_sequence(pos, batch: int) -> List[int]:
+    x = pos.reshape(-1).tolist() if torch.is_tensor(pos) else [int(pos)]
+    return [int(y) for y in x] * batch if len(x) == 1 else [int(y) for y in x]
+
+
+def attention(q, k, v, causal: bool = True, window: Optional[int] = None, key_lengths=None, query_start=None, scale: Optional[float] = None):
+    """Softmax attention with shared key/value heads over the keys that each query sees (:func:`triune_b200.ops.attention`); fp32 inside, fp64 for
+    fp64 inputs."""
+    B, T, H, D = q.shape
+    S, G = k.shape[1], k.shape[2]
+    wide = torch.float64 if q.dtype == torch.float64 else torch.float32
+    start = S - T if query_start is None else query_start
+    start = start.reshape(-1, 1, 1).to(q.device) if torch.is_tensor(start) else torch.full((1, 1, 1), int(start), device=q.device)
+    at, key = start + torch.arange(T, device=q.device)[:, None], torch.arange(S, device=q.device)
+    ends = torch.full((1, 1, 1), S, device=q.device) if key_lengths is None else key_lengths.reshape(-1, 1, 1)
+    seen = (key < ends).expand(B, T, S)
+    if causal:
+        seen = seen & (key <= at)
+    if window:
+        seen = seen & (key > at - window)
+    inside = (key < ends.expand(B, 1, 1)).reshape(B, S, 1, 1)
+    kk = torch.where(inside, k.to(wide), torch.zeros((), dtype=wide, device=k.device)).repeat_interleave(H // G, 2)
+    vv = torch.where(inside, v.to(wide), torch.zeros((), dtype=wide, device=v.device)).repeat_interleave(H // G, 2)
+    seen = seen[:, None]
+    s = torch.einsum("bthd,bshd->bhts", q.to(wide), kk) * (D ** -0.5 if scale is None else scale)
+    s = s.masked_fill(~seen, float("-inf"))
+    top = s.detach().amax(-1, keepdim=True) if S else s.new_zeros(B, H, T, 1)
+    p = torch.exp(s - torch.where(top == float("-inf"), torch.zeros_like(top), top))
+    p = p / p.sum(-1, keepdim=True).masked_fill(~seen.any(-1, keepdim=True), 1.0)
+    bad = ~torch.isfinite(vv)
+    out = torch.einsum("bhts,bshd->bthd", p, vv.masked_fill(bad, 0.0))
+    if bool(bad.any()):  # what is no number reaches the queries that see it, and no others
+        hit = torch.einsum("bhts,bshd->bthd", seen.expand(B, H, T, S).to(wide), bad.to(wide)) > 0
+        out = out.masked_fill(hit, float("nan"))
+    return out.to(q.dtype)
+
+
+def kv8_codes(x: torch.Tensor, dtype: torch.dtype):
+    """[..., 64, D] -> (codes, scales [...]): one scale per block, its largest magnitude over the largest code."""
+    x = x.float()
+    scale = x.abs().amax((-1, -2)) / torch.full((), 127.0 if dtype == torch.int8 else 448.0, device=x.device)
+    scale = torch.where(torch.isfinite(scale), scale, torch.full_like(scale, float("nan")))
+    y = torch.where(scale[..., None, None] > 0, x / torch.where(scale > 0, scale, torch.ones_like(scale))[..., None, None], torch.zeros_like(x))
+    return (y.round().to(torch.int8) if dtype == torch.int8 else y.to(dtype)), scale
+
+
+def kv8_append(cache, k, v, pos) -> None:
+    for b, p in enumerate(_per_sequence(pos, k.shape[0])):
+        room = cache["k8"].shape[2]
+        end = min(p + k.shape[1], room)
+        if p < 0 or p >= end:
+            continue
+        for name, new in (("k", k), ("v", v)):
+            ring, rows = cache[name + "t"], new[b, : end - p].transpose(0, 1)  # [G, T, D]
+            D = rows.shape[2]
+            first = p // KV8_BLOCK * KV8_BLOCK
+            old = ring[b][:, torch.arange(first, p, device=ring.device) % KV8_RING]
+            since = torch.zeros(old.shape[0], end - first, ring.shape[3], dtype=ring.dtype, device=ring.device)
+            since[:, : p - first] = old
+            since[:, p - first :, :D] = rows
+            full = (end - first) // KV8_BLOCK
+            if full:
+                codes, scale = kv8_codes(since[:, : full * KV8_BLOCK].unflatten(1, (full, KV8_BLOCK)), cache[name + "8"].dtype)
+                cache[name + "8"][b, :, first : first + full * KV8_BLOCK] = codes.flatten(1, 2)
+                cache[name + "s"][b, :, first // KV8_BLOCK : first // KV8_BLOCK + full] = scale
+            last = torch.arange(max(p, end - KV8_RING), end, device=ring.device)
+            ring[b, :, last % KV8_RING] = since[:, last - first]
+
+
+def _kv8_values(cache, name: str, b: int, n: int) -> torch.Tensor:
+    """[G, n, pitch] in fp32."""
+    codes, scale, ring = (cache[name + x][b] for x in ("8", "s", "t"))
+    full = n // KV8_BLOCK
+    held = codes[:, : full * KV8_BLOCK].float().unflatten(1, (full, KV8_BLOCK)) * scale[:, :full, None, None] if full else codes[:, :0].float()[:, None]
+    return torch.cat((held.flatten(1, 2), ring[:, torch.arange(full * KV8_BLOCK, n, device=ring.device) % KV8_RING].float()), 1)
+
+
+def kv8_expand(cache, length, head_dim: int, rows: int):
+    B, G, room, _ = cache["k8"].shape
+    out = [torch.zeros(B, rows, G, head_dim, dtype=cache["kt"].dtype, device=cache["kt"].device) for _ in "kv"]
+    for b, n in enumerate(_per_sequence(length, B)):
+        n = max(0, min(n, room))
+        for x, name in zip(out, ("k", "v")):
+            x[b, : min(n, rows)] = _kv8_values(cache, name, b, n)[:, :rows, :head_dim].transpose(0, 1).to(x.dtype)
+    return tuple(out)
+
+
+def kv8_attention(q, cache, pos, scale: float):
+    out = torch.zeros_like(q)
+    T, D, room = q.shape[1], q.shape[3], cache["k8"].shape[2]
+    for b, p in enumerate(_per_sequence(pos, q.shape[0])):
+        if p < 0:
+            continue
+        n = min(p + T, room)
+        if p < n:
+            k, v = (_kv8_values(cache, name, b, n)[None, :, :, :D].transpose(1, 2) for name in ("k", "v"))
+            out[b] = attention(q[b : b + 1].float(), k, v, query_start=p, scale=scale)[0].to(q.dtype)
+        out[b, max(0, room - p) :] = float("nan")
+    return out

@@ -35,6 +35,7 @@ inline int attention_rows(int T) { return (T + 127) / 128 * 128; }
 
 // out [B, T, H, D] contiguous; lse (or null): base-2 logarithm of the softmax's sum, scores times log2(e), +inf for empty rows.
 // part (attention_fwd_scratch(a) bytes or null): where the keys of few queries are split over blocks.
+// k_scales, v_scales (or null): [B, G, blocks], what blocks of 64 keys and values are multiplied by.
 struct AttentionFwd {
   AttentionShape a;
   AttentionView q, k, v;
@@ -42,6 +43,8 @@ struct AttentionFwd {
   float* lse;
   float* part;
   int* status;
+  const float *k_scales, *v_scales;
+  int blocks;
 };
 long long attention_fwd_scratch(const AttentionShape& a);
 void launch_attention_fwd(const AttentionFwd& f, cudaStream_t s);

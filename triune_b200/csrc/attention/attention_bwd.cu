@@ -29,33 +29,8 @@ struct BwdParams {
   int* status;
 };
 
-// 64 columns of a row from TMEM columns `at` on
-__device__ __forceinline__ void load_half(uint32_t at, uint32_t (&x)[32], uint32_t (&y)[32]) {
-  tmem_ld_32x32b_x32(at, x);
-  tmem_ld_32x32b_x32(at + 32, y);
-  tmem_ld_wait_regs(x);
-  asm volatile("" : "+r"(y[0]), "+r"(y[1]), "+r"(y[2]), "+r"(y[3]), "+r"(y[4]), "+r"(y[5]), "+r"(y[6]), "+r"(y[7]), "+r"(y[8]), "+r"(y[9]), "+r"(y[10]),
-               "+r"(y[11]), "+r"(y[12]), "+r"(y[13]), "+r"(y[14]), "+r"(y[15])::"memory");
-  asm volatile("" : "+r"(y[16]), "+r"(y[17]), "+r"(y[18]), "+r"(y[19]), "+r"(y[20]), "+r"(y[21]), "+r"(y[22]), "+r"(y[23]), "+r"(y[24]), "+r"(y[25]),
-               "+r"(y[26]), "+r"(y[27]), "+r"(y[28]), "+r"(y[29]), "+r"(y[30]), "+r"(y[31])::"memory");
-}
-
-// D += A B, A: 128 x 128 bf16 in TMEM as two halves of 64 columns, each in the first 32 TMEM columns of its half of `a`; B: rows
-// `b` of a [128][64 DB] tile
-template <int DB>
-__device__ __forceinline__ void rows_product(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
-#pragma unroll
-  for (int k = 0; k < AT_M / 16; ++k)
-    umma_bf16_ts(d, a + (k >> 2) * 64 + (k & 3) * 8, make_smem_desc(b + k * 2048, AT_BOX, 1024), idesc, add || k > 0);
-}
-
-// D = A B^T over the head dimension
-__device__ __forceinline__ void scores_product(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int steps) {
-  for (int k = 0; k < steps; ++k) {
-    const uint32_t off = (k >> 2) * AT_BOX + (k & 3) * 32;
-    umma_bf16(d, make_smem_desc(a + off, 16, 1024), make_smem_desc(b + off, 16, 1024), idesc, k > 0);
-  }
-}
+// TMEM column of step k of a 128 x 128 bf16 operand: two halves of 64 values, each in the first 32 columns of its 64
+__device__ __forceinline__ int half_column(int k) { return (k >> 2) * 64 + (k & 3) * 8; }
 
 // ---------------------------------------------------------------------------------------------------------------- queries
 template <int DB>
@@ -127,42 +102,44 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
           tma_load_4d(sV + s * TILE + d * AT_BOX, &tmV, full, d * 64, (range.x + u) * AT_M, kvh, b);
         }
       }
+      for (int u = max(0, n - 2); u < n && ok; ++u) ok = mbar_wait(kv_empty + (u & 1), (u >> 1) & 1);  // nothing may arrive once the block is gone
       if (!ok && p.status) *p.status = ST_TIMEOUT_EMPTY;
     }
+    __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0 && n > 0) {
-      const uint32_t id_s = make_idesc(128, 128, 1, 1, 0, 0), id_q = make_idesc(128, 64 * DB, 1, 1, 0, 1);
+    if (n > 0) {
+      const bool leader = elect_one();
       const int ks = (p.a.D + 15) / 16;
       const uint32_t q = smem_u32(sQ), g = smem_u32(sG), k = smem_u32(sK), v = smem_u32(sV);
-      auto arrived = [&](int u) { return u == ragged ? mbar_wait(end_full, 0) && mbar_wait(k_clean, 0) : mbar_wait(kv_full + (u & 1), (u >> 1) & 1); };
-      bool ok = mbar_wait(q_full, 0) && arrived(0);
+      auto arrived = [&](int u) { return u == ragged ? warp_wait(end_full, 0) && warp_wait(k_clean, 0) : warp_wait(kv_full + (u & 1), (u >> 1) & 1); };
+      bool ok = warp_wait(q_full, 0) && arrived(0);
       if (ok) {
         tc_fence_after_sync();
-        scores_product(tmem, q, k, id_s, ks);
-        umma_commit(s_full);
-        scores_product(tmem + 128, g, v, id_s, ks);
-        umma_commit(dp_full);
+        issue(leader, [&] { scores_product<DB>(tmem, q, k, ks); });
+        issue(leader, [&] { umma_commit(s_full); });
+        issue(leader, [&] { scores_product<DB>(tmem + 128, g, v, ks); });
+        issue(leader, [&] { umma_commit(dp_full); });
         for (int u = 0; u < n && ok; ++u) {
           const int s = u & 1, t = s ^ 1;
           const bool next = u + 1 < n;
           if (next) {
-            ok = mbar_wait(s_read, u & 1) && arrived(u + 1);
+            ok = warp_wait(s_read, u & 1) && arrived(u + 1);
             if (!ok) break;
             tc_fence_after_sync();
-            scores_product(tmem, q, k + t * TILE, id_s, ks);
-            umma_commit(s_full);
+            issue(leader, [&] { scores_product<DB>(tmem, q, k + t * TILE, ks); });
+            issue(leader, [&] { umma_commit(s_full); });
           }
-          ok = mbar_wait(ds_ready, u & 1);
+          ok = warp_wait(ds_ready, u & 1);
           if (!ok) break;
           tc_fence_after_sync();
-          rows_product<DB>(tmem + 256, tmem + 128, k + s * TILE, id_q, u > 0);
-          umma_commit(kv_empty + s);
+          issue(leader, [&] { rows_product<DB, 0, 8>(tmem + 256, tmem + 128, k + s * TILE, u > 0, half_column); });
+          issue(leader, [&] { umma_commit(kv_empty + s); });
           if (next) {
-            scores_product(tmem + 128, g, v + t * TILE, id_s, ks);
-            umma_commit(dp_full);
+            issue(leader, [&] { scores_product<DB>(tmem + 128, g, v + t * TILE, ks); });
+            issue(leader, [&] { umma_commit(dp_full); });
           }
         }
-        if (ok) umma_commit(done);
+        if (ok) issue(leader, [&] { umma_commit(done); });
       }
       if (!ok && p.status) *p.status = ST_TIMEOUT_FULL;
     }
@@ -215,11 +192,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
       const int key = (range.x + u) * AT_M;
       const bool masked = !vis.whole(q0, q0 + AT_M - 1, key);
       const int c_lo = lo - key - half * 64, c_hi = hi - key - half * 64;
-      ok = mbar_wait(s_full, u & 1);
+      ok = warp_wait(s_full, u & 1);
       if (!ok) break;
       tc_fence_after_sync();
       uint32_t x[32], y[32];
-      load_half(tS, x, y);
+      tmem_load(tS, x, y);
       tc_fence_before_sync();
       mbar_arrive(s_read);
       const uint64_t cc = pack_f2(p.scale2, p.scale2), mm = pack_f2(-lse, -lse);
@@ -240,14 +217,13 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
       };
       weights(x, 0);
       weights(y, 32);
-      ok = mbar_wait(dp_full, u & 1);
+      ok = warp_wait(dp_full, u & 1);
       if (!ok) break;
       tc_fence_after_sync();
       const uint64_t dd = pack_f2(-delta, -delta);
       auto slopes = [&](uint32_t (&r)[32], int c0) {
         uint32_t d[32], o[16];
-        tmem_ld_32x32b_x32(tP + c0, d);
-        tmem_ld_wait_regs(d);
+        tmem_load(tP + c0, d);
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
           float a, e;
@@ -266,19 +242,20 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
       tc_fence_before_sync();
       mbar_arrive(ds_ready);
     }
-    if (ok && n > 0) ok = mbar_wait(done, 0);
+    if (ok && n > 0) ok = warp_wait(done, 0);
     tc_fence_after_sync();
     __nv_bfloat16* o = p.dq + (((long long)b * p.a.T + t) * p.a.H + h) * p.a.D;
     for (int c = half * 32 * DB; c < (half + 1) * 32 * DB; c += 16) {
       uint32_t v[16] = {};
       if (n > 0) {
-        tmem_ld_32x32b_x16(tmem + lane_base + 256 + c, v);
-        tmem_ld_wait();
+        __syncwarp();
+        tmem_load(tmem + lane_base + 256 + c, v);
       }
       if (t < p.a.T) store_row16(o, c, p.a.D, v, n > 0 ? p.a.scale : 0.f);
     }
     if (!ok && p.status) *p.status = ST_TIMEOUT_TMEM;
   }
+  __syncwarp();  // the block's barrier counts warps, not threads
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
@@ -353,46 +330,48 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
         bulk_load(sStat + s * 2 * AT_M, p.lse + at, AT_M * 4, q_full + s);
         bulk_load(sStat + s * 2 * AT_M + AT_M, p.delta + at, AT_M * 4, q_full + s);
       }
+      for (int u = max(0, n - 2); u < n && ok; ++u) ok = mbar_wait(q_empty + (u & 1), (u >> 1) & 1);
       if (!ok && p.status) *p.status = ST_TIMEOUT_EMPTY;
     }
+    __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0 && n > 0) {
-      const uint32_t id_s = make_idesc(128, 128, 1, 1, 0, 0), id_k = make_idesc(128, 64 * DB, 1, 1, 0, 1);
+    if (n > 0) {
+      const bool leader = elect_one();
       const int ks = (p.a.D + 15) / 16;
       const uint32_t k = smem_u32(sK), v = smem_u32(sV), q = smem_u32(sQ), g = smem_u32(sG);
-      auto arrived = [&](int u) { return mbar_wait(q_full + (u & 1), (u >> 1) & 1); };
-      bool ok = mbar_wait(kv_full, 0) && arrived(0);
+      auto arrived = [&](int u) { return warp_wait(q_full + (u & 1), (u >> 1) & 1); };
+      bool ok = warp_wait(kv_full, 0) && arrived(0);
       if (ok) {
         tc_fence_after_sync();
-        scores_product(tmem, k, q, id_s, ks);
-        umma_commit(s_full);
-        scores_product(tmem + 128, v, g, id_s, ks);
-        umma_commit(dp_full);
+        issue(leader, [&] { scores_product<DB>(tmem, k, q, ks); });
+        issue(leader, [&] { umma_commit(s_full); });
+        issue(leader, [&] { scores_product<DB>(tmem + 128, v, g, ks); });
+        issue(leader, [&] { umma_commit(dp_full); });
         for (int u = 0; u < n && ok; ++u) {
           const int s = u & 1, t = s ^ 1;
           const bool next = u + 1 < n;
-          ok = mbar_wait(p_ready, u & 1);
+          ok = warp_wait(p_ready, u & 1);
           if (!ok) break;
           tc_fence_after_sync();
-          rows_product<DB>(tmem + 256, tmem, g + s * TILE, id_k, u > 0);
+          issue(leader, [&] { rows_product<DB, 0, 8>(tmem + 256, tmem, g + s * TILE, u > 0, half_column); });
           if (next) {
             ok = arrived(u + 1);
             if (!ok) break;
             tc_fence_after_sync();
-            scores_product(tmem, k, q + t * TILE, id_s, ks);  // behind the product that reads P
-            umma_commit(s_full);
+            issue(leader, [&] { scores_product<DB>(tmem, k, q + t * TILE, ks); });  // behind the product that reads P
+            issue(leader, [&] { umma_commit(s_full); });
           }
-          ok = mbar_wait(ds_ready, u & 1);
+          ok = warp_wait(ds_ready, u & 1);
           if (!ok) break;
           tc_fence_after_sync();
-          rows_product<DB>(tmem + 384, tmem + 128, q + s * TILE, id_k, u > 0);
-          umma_commit(q_empty + s);
+          issue(leader, [&] { rows_product<DB, 0, 8>(tmem + 384, tmem + 128, q + s * TILE, u > 0, half_column); });
+          issue(leader, [&] { umma_commit(q_empty + s); });
           if (next) {
-            scores_product(tmem + 128, v, g + t * TILE, id_s, ks);
-            umma_commit(dp_full);
+            issue(leader, [&] { scores_product<DB>(tmem + 128, v, g + t * TILE, ks); });
+            issue(leader, [&] { umma_commit(dp_full); });
           }
         }
-        if (ok) umma_commit(done);
+        if (ok) issue(leader, [&] { umma_commit(done); });
       }
       if (!ok && p.status) *p.status = ST_TIMEOUT_FULL;
     }
@@ -408,11 +387,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
       const bool masked = !vis.whole(t0, t0 + AT_M - 1, k0);
       const int c_lo = lo - t0 - half * 64, c_hi = hi - t0 - half * 64;
       const float4 *lse = reinterpret_cast<const float4*>(sStat + (u & 1) * 2 * AT_M + half * 64), *delta = lse + AT_M / 4;
-      ok = mbar_wait(q_full + (u & 1), (u >> 1) & 1) && mbar_wait(s_full, u & 1);
+      ok = warp_wait(q_full + (u & 1), (u >> 1) & 1) && warp_wait(s_full, u & 1);
       if (!ok) break;
       tc_fence_after_sync();
       uint32_t x[32], y[32];
-      load_half(tS, x, y);
+      tmem_load(tS, x, y);
       const uint64_t cc = pack_f2(p.scale2, p.scale2);
       auto weights = [&](uint32_t (&r)[32], int c0) {
         uint32_t o[16];
@@ -438,13 +417,12 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
       tmem_st_wait();
       tc_fence_before_sync();
       mbar_arrive(p_ready);
-      ok = mbar_wait(dp_full, u & 1);
+      ok = warp_wait(dp_full, u & 1);
       if (!ok) break;
       tc_fence_after_sync();
       auto slopes = [&](uint32_t (&r)[32], int c0) {
         uint32_t d[32], o[16];
-        tmem_ld_32x32b_x32(tP + c0, d);
-        tmem_ld_wait_regs(d);
+        tmem_load(tP + c0, d);
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
           const float4 z = delta[(c0 + i) / 4];
@@ -468,7 +446,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
       tc_fence_before_sync();
       mbar_arrive(ds_ready);
     }
-    if (ok && n > 0) ok = mbar_wait(done, 0);
+    if (ok && n > 0) ok = warp_wait(done, 0);
     tc_fence_after_sync();
     // the first half of the warps writes dV, the second dK
     __nv_bfloat16* o = (half == 0 ? p.dv : p.dk) + (((long long)b * p.a.S + key) * p.a.G + kvh) * p.a.D;
@@ -476,8 +454,8 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
     for (int c = 0; c < 64 * DB; c += 16) {
       uint32_t v[16] = {};
       if (n > 0) {
-        tmem_ld_32x32b_x16(tmem + lane_base + 256 + half * 128 + c, v);
-        tmem_ld_wait();
+        __syncwarp();
+        tmem_load(tmem + lane_base + 256 + half * 128 + c, v);
       }
       if (!inside) {  // what keys past the length hold does not count
 #pragma unroll
@@ -487,6 +465,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
     }
     if (!ok && p.status) *p.status = ST_TIMEOUT_TMEM;
   }
+  __syncwarp();  // the block's barrier counts warps, not threads
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();

@@ -15,6 +15,7 @@
 // running maximum is lazy: sums are rescaled only when it has grown by more than 2^8. fp32 sums take the weights before rounding.
 // TMEM: columns 0-127 S_0, 128-255 S_1, 256-383 O_0, 384-511 O_1.
 #include <algorithm>
+#include <type_traits>
 
 #include "../common/per_device.h"
 #include "attention_tiles.cuh"
@@ -24,6 +25,7 @@ namespace {
 
 constexpr int FW_THREADS = 384;
 constexpr float FW_LAZY = 8.f;
+constexpr int FW_POLY = 4;  // of so many pairs of exponentials one is a polynomial
 
 struct FwdParams {
   AttentionShape a;
@@ -32,26 +34,54 @@ struct FwdParams {
   float* part;  // [splits, B, H, T, 64 * DB] sums, then [splits, B, H, T, 2] maxima and weights
   const __nv_bfloat16* v;
   long long vr, vh, vb;
-  int splits;
+  const float *k_scales, *v_scales;  // [B, G, blocks]
+  int blocks, splits;
   float scale2;  // scale * log2(e)
   int* status;
 };
 
-template <int DB, bool PAIR>
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 2^x of two values up to 2^7 (below 2^-126: 2^-126): x = n + r with |r| <= 1/2, a polynomial of degree 4 in r (minimax of the relative
+// error, 2.6e-6, by the exchange algorithm of Remez), times 2^n. What is no number stays so. The units that multiply and add have room where
+// the exponential unit, at 16 results per clock, is what a tile waits for.
+__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
+  float a, b;
+  unpack_f2(x, a, b);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-126.f));
+  x = pack_f2(a, b);
+  const float big = 12582912.f;  // 1.5 * 2^23: the sum's last bits are the rounded x
+  const uint64_t t = add2(x, pack_f2(big, big));
+  const uint64_t r = add2(x, mul2(add2(t, pack_f2(-big, -big)), pack_f2(-1.f, -1.f)));
+  uint64_t y = pack_f2(9.570102207362652e-3f, 9.570102207362652e-3f);
+  y = fma2(y, r, pack_f2(5.591785907745361e-2f, 5.591785907745361e-2f));
+  y = fma2(y, r, pack_f2(0.240247443318367f, 0.240247443318367f));
+  y = fma2(y, r, pack_f2(0.6931217908859253f, 0.6931217908859253f));
+  y = fma2(y, r, pack_f2(0.9999992847442627f, 0.9999992847442627f));
+  unpack_f2(t, a, b);
+  return mul2(y, pack_f2(__uint_as_float(__float_as_uint(a) * 0x800000u + 0x3f800000u), __uint_as_float(__float_as_uint(b) * 0x800000u + 0x3f800000u)));
+}
+
+template <int DB, bool PAIR, bool SCALED>
 __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                                                                       const __grid_constant__ CUtensorMap tmV, const FwdParams p) {
   constexpr int QT = PAIR ? 2 : 1, TILE = DB * AT_BOX;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   uint8_t *sQ = smem, *sK = sQ + QT * TILE, *sV = sK + 2 * TILE;
-  __shared__ __align__(8) uint64_t bars[17];
+  __shared__ __align__(8) uint64_t bars[19];
   uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 7, *s_full = bars + 9, *p_ready = bars + 11,
-           *o_full = bars + 13, *v_clean = bars + 15;
+           *o_full = bars + 13, *v_clean = bars + 15, *p_half = bars + 17;
   __shared__ uint32_t tmem_slot;
   __shared__ int special;  // a value that is no number was set to zero
   __shared__ float2 other[AT_M];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = blockIdx.x % p.a.H, b = blockIdx.x / p.a.H, kvh = h / (p.a.H / p.a.G);
+  const int h = blockIdx.x % p.a.H, b = blockIdx.x / p.a.H, kvh = h / (p.a.H / p.a.G), kv_head = b * p.a.G + kvh;
   const int q0 = (gridDim.y - 1 - blockIdx.y) * QT * AT_M;  // the rows with the most keys start first
   const Visible vis(p.a, b);
   // key tiles of the two groups: group w takes tiles x, x + step, ... below y
@@ -95,6 +125,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __gr
       mbar_init(v_empty + i, 1);
       mbar_init(s_full + i, 1);
       mbar_init(p_ready + i, 128);
+      mbar_init(p_half + i, 128);
       mbar_init(o_full + i, 1);
       mbar_init(v_clean + i, 64);
     }
@@ -135,67 +166,74 @@ __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __gr
           for (int d = 0; d < DB; ++d) tma_load_4d(sV + s * TILE + d * AT_BOX, &tmV, v_full + s, d * 64, (j0 + i) * AT_M, kvh, b);
         }
       }
+      // nothing may arrive at the barriers once the block is gone
+      for (int u = max(0, j1 - j0 - 2); u < j1 - j0 && ok; ++u) ok = mbar_wait(k_empty + (u & 1), (u >> 1) & 1) && mbar_wait(v_empty + (u & 1), (u >> 1) & 1);
       if (!ok && p.status) *p.status = ST_TIMEOUT_EMPTY;
     }
+    __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0 && j1 > j0) {
-      const uint32_t id_s = make_idesc(128, 128, 1, 1, 0, 0), id_o = make_idesc(128, 64 * DB, 1, 1, 0, 1);
+    if (j1 > j0) {
+      const bool leader = elect_one();
       const int ks = (p.a.D + 15) / 16;
+      const uint32_t qa = smem_u32(sQ), ka = smem_u32(sK), va = smem_u32(sV);
       auto scores = [&](int w, int j) {
-        const uint32_t qa = smem_u32(sQ + (PAIR ? w : 0) * TILE), ka = smem_u32(sK + ((j - j0) & 1) * TILE);
-        for (int k = 0; k < ks; ++k) {
-          const uint32_t off = (k >> 2) * AT_BOX + (k & 3) * 32;
-          umma_bf16(tmem + w * 128, make_smem_desc(qa + off, 16, 1024), make_smem_desc(ka + off, 16, 1024), id_s, k > 0);
-        }
-        umma_commit(s_full + w);
+        issue(leader, [&] {
+          scores_product<DB>(tmem + w * 128, qa + (PAIR ? w : 0) * TILE, ka + ((j - j0) & 1) * TILE, ks);
+          umma_commit(s_full + w);
+        });
       };
-      auto values = [&](int w, int j) {
-        const uint32_t va = smem_u32(sV + ((j - j0) & 1) * TILE);
-#pragma unroll
-        for (int k = 0; k < AT_M / 16; ++k)
-          umma_bf16_ts(tmem + 256 + w * 128, tmem + w * 128 + k * 8, make_smem_desc(va + k * 2048, AT_BOX, 1024), id_o, j != range[w].x || k > 0);
+      auto values = [&](int w, int j, auto half) {
+        constexpr int K0 = decltype(half)::value * 4;
+        issue(leader, [&] {
+          rows_product<DB, K0, 4>(tmem + 256 + w * 128, tmem + w * 128, va + ((j - j0) & 1) * TILE, j != range[w].x, [](int k) { return k * 8; });
+        });
       };
+      auto commit = [&](uint64_t* bar) { issue(leader, [&] { umma_commit(bar); }); };
       int done[2] = {0, 0};
-      auto k_arrived = [&](int j) { return mbar_wait(k_full + ((j - j0) & 1), ((j - j0) >> 1) & 1); };
-      bool ok = mbar_wait(q_full, 0) && k_arrived(j0);
+      auto k_arrived = [&](int j) { return warp_wait(k_full + ((j - j0) & 1), ((j - j0) >> 1) & 1); };
+      bool ok = warp_wait(q_full, 0) && k_arrived(j0);
       if (ok) {
         tc_fence_after_sync();
         if constexpr (PAIR) {
           for (int w = 0; w < 2; ++w)
             if (takes(w, j0)) scores(w, j0);
-          umma_commit(k_empty);
+          commit(k_empty);
         } else {
           scores(0, j0);
-          umma_commit(k_empty);
+          commit(k_empty);
           if (j1 - j0 > 1) {
             ok = k_arrived(j0 + 1);
             if (ok) {
               tc_fence_after_sync();
               scores(1, j0 + 1);
-              umma_commit(k_empty + 1);
+              commit(k_empty + 1);
             }
           }
         }
         for (int j = j0; j < j1 && ok; ++j) {
           const int s = (j - j0) & 1;
-          ok = mbar_wait(v_clean + s, ((j - j0) >> 1) & 1);
+          ok = warp_wait(v_clean + s, ((j - j0) >> 1) & 1);
           const int jn = j + step;  // the next tile whose scores are issued
           if (ok && jn < j1) ok = k_arrived(jn);
           for (int w = 0; w < 2 && ok; ++w) {
             const bool now = takes(w, j), next = jn < j1 && (PAIR ? takes(w, jn) : now);
             if (now) {
-              ok = mbar_wait(p_ready + w, done[w] & 1);
+              ok = warp_wait(p_half + w, done[w] & 1);
+              if (!ok) break;
+              tc_fence_after_sync();
+              values(w, j, std::integral_constant<int, 0>{});
+              ok = warp_wait(p_ready + w, done[w] & 1);
               ++done[w];
               if (!ok) break;
               tc_fence_after_sync();
-              values(w, j);
-              if (done[w] == count(w)) umma_commit(o_full + w);
+              values(w, j, std::integral_constant<int, 1>{});
+              if (done[w] == count(w)) commit(o_full + w);
             }
             if (next) scores(w, jn);
           }
           if (!ok) break;
-          umma_commit(v_empty + s);
-          if (jn < j1) umma_commit(k_empty + ((jn - j0) & 1));
+          commit(v_empty + s);
+          if (jn < j1) commit(k_empty + ((jn - j0) & 1));
         }
       }
       if (!ok && p.status) *p.status = ST_TIMEOUT_FULL;
@@ -243,46 +281,45 @@ __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __gr
     const int n = count(w), lo = vis.low(t), hi = vis.high(t);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
-    for (int it = 0; it < n; ++it) {
-      const int j = range[w].x + it * step;
-      ok = mbar_wait(s_full + w, it & 1);
-      if (!ok) break;
-      tc_fence_after_sync();
-      const bool masked = !vis.whole(first, first + AT_M - 1, j * AT_M);
-      const int c_lo = lo - j * AT_M, c_hi = hi - j * AT_M;  // visible columns
-      uint32_t ra[32], rb[32];
-      float mx = -INFINITY;
-      auto row_max = [&](uint32_t (&r)[32], int c0) {
-        if (masked) {
+    // One tile: maximum, then weights, their sums and their bf16 form. MASKED: not all of the tile's keys are visible to all queries.
+    auto softmax = [&](auto some, int it, int key) {
+      constexpr bool MASKED = decltype(some)::value;
+      const int c_lo = lo - key, c_hi = hi - key;  // visible columns
+      // Half of the 128 scores fits beside the rest: the second half is read for its maximum, and again behind the first half's weights
+      uint32_t x[32], y[32];
+      float top[4];
+      auto chunk_max = [&](uint32_t (&r)[32], int c) {
+        if constexpr (MASKED) {
 #pragma unroll
           for (int i = 0; i < 32; ++i)
-            if (c0 + i <= c_hi && c0 + i >= c_lo) mx = fmaxf(mx, __uint_as_float(r[i]));
-        } else {
-          float x0 = __uint_as_float(r[0]), x1 = __uint_as_float(r[1]), x2 = __uint_as_float(r[2]), x3 = __uint_as_float(r[3]);
-#pragma unroll
-          for (int i = 4; i < 32; i += 4) {
-            x0 = fmaxf(x0, __uint_as_float(r[i]));
-            x1 = fmaxf(x1, __uint_as_float(r[i + 1]));
-            x2 = fmaxf(x2, __uint_as_float(r[i + 2]));
-            x3 = fmaxf(x3, __uint_as_float(r[i + 3]));
-          }
-          mx = fmaxf(mx, fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)));
+            if (32 * c + i > c_hi || 32 * c + i < c_lo) r[i] = 0xff800000u;  // -inf
         }
+        float a = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])), e = fmaxf(__uint_as_float(r[2]), __uint_as_float(r[3]));
+#pragma unroll
+        for (int i = 4; i < 32; i += 4) {
+          a = max3(a, __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+          e = max3(e, __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]));
+        }
+        top[c] = fmaxf(a, e);
       };
-      tmem_ld_32x32b_x32(tS, ra);
-      tmem_ld_wait_regs(ra);
-      tmem_ld_32x32b_x32(tS + 32, rb);
-      row_max(ra, 0);
-      tmem_ld_wait_regs(rb);
-      tmem_ld_32x32b_x32(tS + 64, ra);
-      row_max(rb, 32);
-      tmem_ld_wait_regs(ra);
-      tmem_ld_32x32b_x32(tS + 96, rb);
-      row_max(ra, 64);
-      tmem_ld_wait_regs(rb);
-      tmem_ld_32x32b_x32(tS, ra);  // the first columns again, for the exponentials
-      row_max(rb, 96);
-      const float mn = fmaxf(m, mx * c2);
+      tmem_load(tS + 64, x, y);
+      chunk_max(x, 2);
+      chunk_max(y, 3);
+      tmem_load(tS, x, y);
+      chunk_max(x, 0);
+      chunk_max(y, 1);
+      float f0 = c2, f1 = c2;  // what the scores of the two blocks of 64 keys are multiplied by
+      [[maybe_unused]] uint64_t v0 = 0, v1 = 0;
+      if constexpr (SCALED) {
+        f0 *= p.k_scales[(long long)kv_head * p.blocks + key / 64];
+        f1 *= key / 64 + 1 < p.blocks ? p.k_scales[(long long)kv_head * p.blocks + key / 64 + 1] : 0.f;
+        const float a = p.v_scales[(long long)kv_head * p.blocks + key / 64];
+        const float e = key / 64 + 1 < p.blocks ? p.v_scales[(long long)kv_head * p.blocks + key / 64 + 1] : 0.f;
+        v0 = pack_f2(a, a), v1 = pack_f2(e, e);
+      }
+      const float t0 = fmaxf(top[0], top[1]), t1 = fmaxf(top[2], top[3]);
+      // a scale of zero takes no score (minus infinity, of a block without visible keys) to NaN: fmaxf passes over those
+      const float mn = SCALED ? max3(m, t0 * f0, t1 * f1) : fmaxf(m, fmaxf(t0, t1) * c2);
       const bool grow = mn > m && (m == -INFINITY || mn - m > FW_LAZY);
       float f = 1.f;
       if (grow) {
@@ -290,57 +327,70 @@ __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __gr
         m = mn;
         l *= f;
       }
-      tmem_ld_wait_regs(ra);
-      if (it > 0 && __any_sync(0xffffffffu, grow)) {
+      const bool any = __any_sync(0xffffffffu, grow);  // also brings the warp together again
+      if (it > 0 && any) {
         for (int c = 0; c < 64 * DB; c += 16) {
           uint32_t o[16];
-          tmem_ld_32x32b_x16(tO + c, o);
-          tmem_ld_wait();
+          tmem_load(tO + c, o);
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
           tmem_st_32x32b_x16(tO + c, o);
         }
-        tmem_st_wait();
       }
-      const float ms = m == -INFINITY ? 0.f : m;  // no visible key yet: the weights are masked, or no numbers
-      const uint64_t cc = pack_f2(c2, c2), mm = pack_f2(-ms, -ms);
+      const float ms = m == -INFINITY ? 0.f : m;  // no visible key yet
+      const uint64_t mm = pack_f2(-ms, -ms);
       uint64_t sum2 = pack_f2(0.f, 0.f);
-      auto weights = [&](uint32_t (&r)[32], int c0) {
+      auto weights = [&](uint32_t (&r)[32], int c) {
+        const float fc = c < 2 ? f0 : f1;
+        const uint64_t cc = pack_f2(fc, fc);
         uint32_t q[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          float x, e;
-          unpack_f2(fma2(pack_f2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), cc, mm), x, e);
-          x = ex2(x);
-          e = ex2(e);
-          if (masked) {
-            const int c = c0 + 2 * i;
-            x = c <= c_hi && c >= c_lo ? x : 0.f;
-            e = c + 1 <= c_hi && c + 1 >= c_lo ? e : 0.f;
+          const uint64_t y = fma2(pack_f2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), cc, mm);
+          uint64_t e;
+          if (i % FW_POLY == FW_POLY - 1 && !MASKED) {
+            e = exp2_pair(y);
+          } else {
+            float a, z;
+            unpack_f2(y, a, z);
+            a = ex2(a);
+            z = ex2(z);
+            if constexpr (MASKED) {  // also where a block's scale, zero or no number, was multiplied by minus infinity
+              const int k = 32 * c + 2 * i;
+              a = k <= c_hi && k >= c_lo ? a : 0.f;
+              z = k + 1 <= c_hi && k + 1 >= c_lo ? z : 0.f;
+            }
+            e = pack_f2(a, z);
           }
-          sum2 = add2(sum2, pack_f2(x, e));
-          q[i] = pack_bf16x2(x, e);
+          sum2 = add2(sum2, e);
+          if constexpr (SCALED) e = mul2(e, c < 2 ? v0 : v1);
+          q[i] = f2_to_bf16x2(e);
         }
-        tmem_st_32x32b_x16(tS + c0 / 2, q);  // lands in columns whose scores this thread has already read
+        tmem_st_32x32b_x16(tS + 16 * c, q);  // over columns that this thread has read
+        if (c & 1) {  // the product starts on the first half of the keys
+          tmem_st_wait();
+          tc_fence_before_sync();
+          mbar_arrive(c == 1 ? p_half + w : p_ready + w);
+        }
       };
-      tmem_ld_32x32b_x32(tS + 32, rb);
-      weights(ra, 0);
-      tmem_ld_wait_regs(rb);
-      tmem_ld_32x32b_x32(tS + 64, ra);
-      weights(rb, 32);
-      tmem_ld_wait_regs(ra);
-      tmem_ld_32x32b_x32(tS + 96, rb);
-      weights(ra, 64);
-      tmem_ld_wait_regs(rb);
-      weights(rb, 96);
+      weights(x, 0);
+      weights(y, 1);
+      tmem_load(tS + 64, x, y);
+      weights(x, 2);
+      weights(y, 3);
       float s0, s1;
       unpack_f2(sum2, s0, s1);
       l += s0 + s1;
-      tmem_st_wait();
-      tc_fence_before_sync();
-      mbar_arrive(p_ready + w);
+    };
+    for (int it = 0; it < n; ++it) {
+      const int key = (range[w].x + it * step) * AT_M;
+      ok = warp_wait(s_full + w, it & 1);
+      if (!ok) break;
+      tc_fence_after_sync();
+      if (vis.whole(first, first + AT_M - 1, key)) softmax(std::false_type{}, it, key);
+      else softmax(std::true_type{}, it, key);
     }
-    if (ok && n > 0) ok = mbar_wait(o_full + w, 0);
+    if (ok && n > 0) ok = warp_wait(o_full + w, 0);
     tc_fence_after_sync();
     float share = 1.f;  // of this group's sums in the row
     float* half = reinterpret_cast<float*>(sK);
@@ -351,8 +401,8 @@ __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __gr
         other[row] = make_float2(m, l);
         for (int c = 0; c < 64 * DB; c += 16) {
           uint32_t o[16];
-          tmem_ld_32x32b_x16(tO + c, o);
-          tmem_ld_wait();
+          __syncwarp();
+          tmem_load(tO + c, o);
 #pragma unroll
           for (int i = 0; i < 16; ++i) half[(c + i) * AT_M + row] = __uint_as_float(o[i]);
         }
@@ -387,9 +437,9 @@ __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __gr
       const bool any = n > 0;
       for (int c = 0; c < 64 * DB; c += 16) {
         uint32_t x[16];
+        __syncwarp();
         if (any) {
-          tmem_ld_32x32b_x16(tO + c, x);
-          tmem_ld_wait();
+          tmem_load(tO + c, x);
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -423,6 +473,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __gr
     }
     if (!ok && p.status) *p.status = ST_TIMEOUT_TMEM;
   }
+  __syncwarp();  // the block's barrier counts warps: one whose threads came one by one would count more than once
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
@@ -482,24 +533,24 @@ int fwd_splits(const AttentionShape& a, bool& pair) {
   return (int)std::max<long long>(1, std::min({sms / (heads * tiles), most, 32ll}));
 }
 
-template <int DB, bool PAIR>
+template <int DB, bool PAIR, bool SCALED>
 void run(const FwdParams& p, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t s) {
   constexpr int QT = PAIR ? 2 : 1, smem = (QT + 4) * DB * AT_BOX + 1024;
   static PerDeviceOnce once;
-  auto kern = attention_fwd_kernel<DB, PAIR>;
+  auto kern = attention_fwd_kernel<DB, PAIR, SCALED>;
   if (once.first_use()) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   kern<<<dim3(p.a.B * p.a.H, (p.a.T + QT * AT_M - 1) / (QT * AT_M), p.splits), FW_THREADS, smem, s>>>(tq, tk, tv, p);
   attention_check_launch("attention_fwd");
 }
 
-template <int DB>
+template <int DB, bool SCALED>
 void run_width(const AttentionFwd& f, cudaStream_t s) {
   const AttentionShape& a = f.a;
   const CUtensorMap tq = attention_map(f.q, a.D, a.T, a.H, a.B), tk = attention_map(f.k, a.D, a.S, a.G, a.B), tv = attention_map(f.v, a.D, a.S, a.G, a.B);
   bool pair;
-  FwdParams p{a, f.out, f.lse, f.part, (const __nv_bfloat16*)f.v.p, f.v.sr, f.v.sh, f.v.sb, fwd_splits(a, pair), a.scale * LOG2E, f.status};
-  if (pair) return run<DB, true>(p, tq, tk, tv, s);
-  run<DB, false>(p, tq, tk, tv, s);
+  FwdParams p{a, f.out, f.lse, f.part, (const __nv_bfloat16*)f.v.p, f.v.sr, f.v.sh, f.v.sb, f.k_scales, f.v_scales, f.blocks, fwd_splits(a, pair), a.scale * LOG2E, f.status};
+  if (pair) return run<DB, true, SCALED>(p, tq, tk, tv, s);
+  run<DB, false, SCALED>(p, tq, tk, tv, s);
   if (p.splits > 1) {
     const long long rows = (long long)a.B * a.H * a.T;
     attention_join_kernel<DB><<<(unsigned)((rows + 7) / 8), 256, 0, s>>>(p);
@@ -516,8 +567,8 @@ long long attention_fwd_scratch(const AttentionShape& a) {
 }
 
 void launch_attention_fwd(const AttentionFwd& f, cudaStream_t s) {
-  if (f.a.D <= 64) run_width<1>(f, s);
-  else run_width<2>(f, s);
+  if (f.k_scales != nullptr) f.a.D <= 64 ? run_width<1, true>(f, s) : run_width<2, true>(f, s);
+  else f.a.D <= 64 ? run_width<1, false>(f, s) : run_width<2, false>(f, s);
 }
 
 }  // namespace tb

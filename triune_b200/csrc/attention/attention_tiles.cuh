@@ -48,8 +48,77 @@ __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint3
                : "memory");
 }
 
+// Products of tiles, issued by one elected thread of a warp that stays together: every thread comes to the waits and to the end of each
+// issue (`issue`), since the operands are in registers that all threads of a warp share. Descriptors are formed once per tile and moved
+// on by constants: formed for each product, the issuing thread took 125 clocks a product, twice what the tensor core needs for it.
+template <typename F>
+__device__ __forceinline__ void issue(bool leader, F f) {
+  if (leader) f();
+  __syncwarp();
+}
+// D = A B^T over the head dimension, `steps` times 16 columns; tiles of DB boxes of 64 columns.
+template <int DB>
+__device__ __forceinline__ void scores_product(uint32_t d, uint32_t a, uint32_t b, int steps) {
+  constexpr uint32_t idesc = make_idesc(AT_M, AT_M, 1, 1, 0, 0);
+  const uint64_t da = make_smem_desc(a, 16, 1024), db = make_smem_desc(b, 16, 1024);
+#pragma unroll
+  for (int k = 0; k < 4 * DB; ++k)
+    if (k < steps) {
+      const uint32_t off = ((k >> 2) * AT_BOX + (k & 3) * 32) >> 4;
+      umma_bf16(d, da + off, db + off, idesc, k > 0);
+    }
+}
+// D (+)= A B, A: 16-column steps K0 .. K0 + N - 1 of 128 x 128 bf16 in TMEM (step k at `a` + columns at(k)), B: rows of a [128][64 DB] tile
+template <int DB, int K0, int N, typename At>
+__device__ __forceinline__ void rows_product(uint32_t d, uint32_t a, uint32_t b, bool add, At at) {
+  constexpr uint32_t idesc = make_idesc(AT_M, 64 * DB, 1, 1, 0, 1);
+  const uint64_t db = make_smem_desc(b, AT_BOX, 1024);
+#pragma unroll
+  for (int k = K0; k < K0 + N; ++k) umma_bf16_ts(d, a + at(k), db + ((k * 2048) >> 4), idesc, k > 0 || add);
+}
+
+// Loads of 32, 64 or 16 columns of this warp's lanes that are complete when they return. Load and wait are one statement: a load lands
+// in its registers whenever it does, and nothing else would keep the compiler from moving or spilling registers that it has still to
+// write (which turns into wrong values and wrong addresses as soon as registers are short).
+__device__ __forceinline__ void tmem_load(uint32_t at, uint32_t (&x)[32]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+               "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]), "=r"(x[8]), "=r"(x[9]), "=r"(x[10]),
+                 "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15]), "=r"(x[16]), "=r"(x[17]), "=r"(x[18]), "=r"(x[19]), "=r"(x[20]),
+                 "=r"(x[21]), "=r"(x[22]), "=r"(x[23]), "=r"(x[24]), "=r"(x[25]), "=r"(x[26]), "=r"(x[27]), "=r"(x[28]), "=r"(x[29]), "=r"(x[30]),
+                 "=r"(x[31])
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_load(uint32_t at, uint32_t (&x)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]), "=r"(x[8]), "=r"(x[9]), "=r"(x[10]),
+                 "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15])
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_load(uint32_t at, uint32_t (&x)[32], uint32_t (&y)[32]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+               "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, "
+               "%46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]), "=r"(x[8]), "=r"(x[9]), "=r"(x[10]),
+                 "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15]), "=r"(x[16]), "=r"(x[17]), "=r"(x[18]), "=r"(x[19]), "=r"(x[20]),
+                 "=r"(x[21]), "=r"(x[22]), "=r"(x[23]), "=r"(x[24]), "=r"(x[25]), "=r"(x[26]), "=r"(x[27]), "=r"(x[28]), "=r"(x[29]), "=r"(x[30]),
+                 "=r"(x[31]), "=r"(y[0]), "=r"(y[1]), "=r"(y[2]), "=r"(y[3]), "=r"(y[4]), "=r"(y[5]), "=r"(y[6]), "=r"(y[7]), "=r"(y[8]), "=r"(y[9]),
+                 "=r"(y[10]), "=r"(y[11]), "=r"(y[12]), "=r"(y[13]), "=r"(y[14]), "=r"(y[15]), "=r"(y[16]), "=r"(y[17]), "=r"(y[18]), "=r"(y[19]),
+                 "=r"(y[20]), "=r"(y[21]), "=r"(y[22]), "=r"(y[23]), "=r"(y[24]), "=r"(y[25]), "=r"(y[26]), "=r"(y[27]), "=r"(y[28]), "=r"(y[29]),
+                 "=r"(y[30]), "=r"(y[31])
+               : "r"(at)
+               : "memory");
+}
+
+// A wait of a whole warp. Its threads may see the barrier's phase end at different times; the tcgen05 loads and stores that follow
+// are instructions of whole warps, so the warp is brought together here.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
+
 template <int N>
 __device__ __forceinline__ void named_barrier(int id) {
+  __syncwarp();  // warps are counted, not threads
   asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory");
 }
 

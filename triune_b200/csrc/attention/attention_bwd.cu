@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
            *done = bars + 9, *k_clean = bars + 10, *end_full = bars + 11;
   __shared__ uint32_t tmem_slot;
   __shared__ float part[AT_M];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int h = blockIdx.x % p.a.H, b = blockIdx.x / p.a.H, kvh = h / (p.a.H / p.a.G);
   const int q0 = (gridDim.y - 1 - blockIdx.y) * AT_M;
   const Visible vis(p.a, b);
@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
   }
   __syncthreads();
   tc_fence_after_sync();
-  const uint32_t tmem = tmem_slot;
+  const uint32_t tmem = uniform(tmem_slot);
 
   if (warp == 0) {
     if (lane == 0 && n > 0) {
@@ -108,17 +108,16 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
     __syncwarp();
   } else if (warp == 1) {
     if (n > 0) {
-      const bool leader = elect_one();
       const int ks = (p.a.D + 15) / 16;
       const uint32_t q = smem_u32(sQ), g = smem_u32(sG), k = smem_u32(sK), v = smem_u32(sV);
       auto arrived = [&](int u) { return u == ragged ? warp_wait(end_full, 0) && warp_wait(k_clean, 0) : warp_wait(kv_full + (u & 1), (u >> 1) & 1); };
       bool ok = warp_wait(q_full, 0) && arrived(0);
       if (ok) {
         tc_fence_after_sync();
-        issue(leader, [&] { scores_product<DB>(tmem, q, k, ks); });
-        issue(leader, [&] { umma_commit(s_full); });
-        issue(leader, [&] { scores_product<DB>(tmem + 128, g, v, ks); });
-        issue(leader, [&] { umma_commit(dp_full); });
+        issue([&] { scores_product<DB>(tmem, q, k, ks); });
+        issue([&] { umma_commit(s_full); });
+        issue([&] { scores_product<DB>(tmem + 128, g, v, ks); });
+        issue([&] { umma_commit(dp_full); });
         for (int u = 0; u < n && ok; ++u) {
           const int s = u & 1, t = s ^ 1;
           const bool next = u + 1 < n;
@@ -126,20 +125,20 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
             ok = warp_wait(s_read, u & 1) && arrived(u + 1);
             if (!ok) break;
             tc_fence_after_sync();
-            issue(leader, [&] { scores_product<DB>(tmem, q, k + t * TILE, ks); });
-            issue(leader, [&] { umma_commit(s_full); });
+            issue([&] { scores_product<DB>(tmem, q, k + t * TILE, ks); });
+            issue([&] { umma_commit(s_full); });
           }
           ok = warp_wait(ds_ready, u & 1);
           if (!ok) break;
           tc_fence_after_sync();
-          issue(leader, [&] { rows_product<DB, 0, 8>(tmem + 256, tmem + 128, k + s * TILE, u > 0, half_column); });
-          issue(leader, [&] { umma_commit(kv_empty + s); });
+          issue([&] { rows_product<DB, 0, 8>(tmem + 256, tmem + 128, k + s * TILE, u > 0, half_column); });
+          issue([&] { umma_commit(kv_empty + s); });
           if (next) {
-            issue(leader, [&] { scores_product<DB>(tmem + 128, g, v + t * TILE, ks); });
-            issue(leader, [&] { umma_commit(dp_full); });
+            issue([&] { scores_product<DB>(tmem + 128, g, v + t * TILE, ks); });
+            issue([&] { umma_commit(dp_full); });
           }
         }
-        if (ok) issue(leader, [&] { umma_commit(done); });
+        if (ok) issue([&] { umma_commit(done); });
       }
       if (!ok && p.status) *p.status = ST_TIMEOUT_FULL;
     }
@@ -276,7 +275,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
   uint64_t *kv_full = bars, *q_full = bars + 1, *q_empty = bars + 3, *s_full = bars + 5, *p_ready = bars + 6, *dp_full = bars + 7, *ds_ready = bars + 8,
            *done = bars + 9;
   __shared__ uint32_t tmem_slot;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int kvh = blockIdx.x % p.a.G, b = blockIdx.x / p.a.G, rep = p.a.H / p.a.G;
   const int k0 = blockIdx.y * AT_M;  // with a causal mask the first keys are seen by the most queries
   const Visible vis(p.a, b);
@@ -303,7 +302,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
   }
   __syncthreads();
   tc_fence_after_sync();
-  const uint32_t tmem = tmem_slot;
+  const uint32_t tmem = uniform(tmem_slot);
 
   if (warp == 0) {
     if (lane == 0 && n > 0) {
@@ -336,42 +335,41 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
     __syncwarp();
   } else if (warp == 1) {
     if (n > 0) {
-      const bool leader = elect_one();
       const int ks = (p.a.D + 15) / 16;
       const uint32_t k = smem_u32(sK), v = smem_u32(sV), q = smem_u32(sQ), g = smem_u32(sG);
       auto arrived = [&](int u) { return warp_wait(q_full + (u & 1), (u >> 1) & 1); };
       bool ok = warp_wait(kv_full, 0) && arrived(0);
       if (ok) {
         tc_fence_after_sync();
-        issue(leader, [&] { scores_product<DB>(tmem, k, q, ks); });
-        issue(leader, [&] { umma_commit(s_full); });
-        issue(leader, [&] { scores_product<DB>(tmem + 128, v, g, ks); });
-        issue(leader, [&] { umma_commit(dp_full); });
+        issue([&] { scores_product<DB>(tmem, k, q, ks); });
+        issue([&] { umma_commit(s_full); });
+        issue([&] { scores_product<DB>(tmem + 128, v, g, ks); });
+        issue([&] { umma_commit(dp_full); });
         for (int u = 0; u < n && ok; ++u) {
           const int s = u & 1, t = s ^ 1;
           const bool next = u + 1 < n;
           ok = warp_wait(p_ready, u & 1);
           if (!ok) break;
           tc_fence_after_sync();
-          issue(leader, [&] { rows_product<DB, 0, 8>(tmem + 256, tmem, g + s * TILE, u > 0, half_column); });
+          issue([&] { rows_product<DB, 0, 8>(tmem + 256, tmem, g + s * TILE, u > 0, half_column); });
           if (next) {
             ok = arrived(u + 1);
             if (!ok) break;
             tc_fence_after_sync();
-            issue(leader, [&] { scores_product<DB>(tmem, k, q + t * TILE, ks); });  // behind the product that reads P
-            issue(leader, [&] { umma_commit(s_full); });
+            issue([&] { scores_product<DB>(tmem, k, q + t * TILE, ks); });  // behind the product that reads P
+            issue([&] { umma_commit(s_full); });
           }
           ok = warp_wait(ds_ready, u & 1);
           if (!ok) break;
           tc_fence_after_sync();
-          issue(leader, [&] { rows_product<DB, 0, 8>(tmem + 384, tmem + 128, q + s * TILE, u > 0, half_column); });
-          issue(leader, [&] { umma_commit(q_empty + s); });
+          issue([&] { rows_product<DB, 0, 8>(tmem + 384, tmem + 128, q + s * TILE, u > 0, half_column); });
+          issue([&] { umma_commit(q_empty + s); });
           if (next) {
-            issue(leader, [&] { scores_product<DB>(tmem + 128, v, g + t * TILE, ks); });
-            issue(leader, [&] { umma_commit(dp_full); });
+            issue([&] { scores_product<DB>(tmem + 128, v, g + t * TILE, ks); });
+            issue([&] { umma_commit(dp_full); });
           }
         }
-        if (ok) issue(leader, [&] { umma_commit(done); });
+        if (ok) issue([&] { umma_commit(done); });
       }
       if (!ok && p.status) *p.status = ST_TIMEOUT_FULL;
     }

@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __gr
   __shared__ uint32_t tmem_slot;
   __shared__ int special;  // a value that is no number was set to zero
   __shared__ float2 other[AT_M];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int h = blockIdx.x % p.a.H, b = blockIdx.x / p.a.H, kvh = h / (p.a.H / p.a.G), kv_head = b * p.a.G + kvh;
   const int q0 = (gridDim.y - 1 - blockIdx.y) * QT * AT_M;  // the rows with the most keys start first
   const Visible vis(p.a, b);
@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __gr
   }
   __syncthreads();
   tc_fence_after_sync();
-  const uint32_t tmem = tmem_slot;
+  const uint32_t tmem = uniform(tmem_slot);
 
   if (warp == 0) {
     if (lane == 0 && j1 > j0) {
@@ -173,22 +173,21 @@ __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __gr
     __syncwarp();
   } else if (warp == 1) {
     if (j1 > j0) {
-      const bool leader = elect_one();
       const int ks = (p.a.D + 15) / 16;
       const uint32_t qa = smem_u32(sQ), ka = smem_u32(sK), va = smem_u32(sV);
       auto scores = [&](int w, int j) {
-        issue(leader, [&] {
+        issue([&] {
           scores_product<DB>(tmem + w * 128, qa + (PAIR ? w : 0) * TILE, ka + ((j - j0) & 1) * TILE, ks);
           umma_commit(s_full + w);
         });
       };
       auto values = [&](int w, int j, auto half) {
         constexpr int K0 = decltype(half)::value * 4;
-        issue(leader, [&] {
+        issue([&] {
           rows_product<DB, K0, 4>(tmem + 256 + w * 128, tmem + w * 128, va + ((j - j0) & 1) * TILE, j != range[w].x, [](int k) { return k * 8; });
         });
       };
-      auto commit = [&](uint64_t* bar) { issue(leader, [&] { umma_commit(bar); }); };
+      auto commit = [&](uint64_t* bar) { issue([&] { umma_commit(bar); }); };
       int done[2] = {0, 0};
       auto k_arrived = [&](int j) { return warp_wait(k_full + ((j - j0) & 1), ((j - j0) >> 1) & 1); };
       bool ok = warp_wait(q_full, 0) && k_arrived(j0);

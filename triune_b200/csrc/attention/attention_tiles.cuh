@@ -11,15 +11,22 @@ constexpr int AT_M = 128;             // queries of a tile, keys of a tile
 constexpr int AT_BOX = AT_M * 64 * 2;  // bytes of a box of 128 rows and 64 columns
 constexpr float LOG2E = 1.4426950408889634f;
 
+// A value that all threads of the warp have, made known as such: what is formed from it stays in the warp's uniform registers, from
+// which tensor-core instructions take their operands
+template <typename T>
+__device__ __forceinline__ T uniform(T x) {
+  return __shfl_sync(0xffffffffu, x, 0);
+}
+
 struct Visible {  // of one sequence
   int start, length, window;
   bool causal;
   __device__ __forceinline__ Visible(const AttentionShape& a, int b) : window(a.window), causal(a.causal) {
     // positions past these limits see what those at the limits see
     const long long s0 = a.starts != nullptr ? a.starts[b] : a.start, lim = 1ll << 30;
-    start = (int)(s0 < -lim ? -lim : s0 > lim ? lim : s0);
+    start = uniform((int)(s0 < -lim ? -lim : s0 > lim ? lim : s0));
     const long long n = a.lengths != nullptr ? a.lengths[b] : a.S;
-    length = (int)(n < 0 ? 0 : n > a.S ? a.S : n);
+    length = uniform((int)(n < 0 ? 0 : n > a.S ? a.S : n));
   }
   // keys low(t) .. high(t) are visible to query t; both grow with t
   __device__ __forceinline__ int low(int t) const { return window > 0 ? max(0, start + t - window + 1) : 0; }
@@ -52,8 +59,8 @@ __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint3
 // issue (`issue`), since the operands are in registers that all threads of a warp share. Descriptors are formed once per tile and moved
 // on by constants: formed for each product, the issuing thread took 125 clocks a product, twice what the tensor core needs for it.
 template <typename F>
-__device__ __forceinline__ void issue(bool leader, F f) {
-  if (leader) f();
+__device__ __forceinline__ void issue(F f) {
+  if (elect_one()) f();
   __syncwarp();
 }
 // D = A B^T over the head dimension, `steps` times 16 columns; tiles of DB boxes of 64 columns.

@@ -4,13 +4,13 @@
 //
 // Two kernels, each of which keeps its sums in TMEM and writes every gradient once: one per 128 queries (dQ; it also forms delta),
 // one per 128 keys (dK, dV). S and dP are formed in both, so there are seven tile products instead of the five of a kernel that
-// adds dQ up in global memory: no atomics, the same bits every time, no fp32 copy of dQ, and every product that reads P or dS
-// takes it from TMEM as its first operand (rows = lanes), so neither passes through shared memory.
+// adds dQ up in global memory: no atomics, the same bits every time, no fp32 copy of dQ.
 // Both: warp 0 TMA producer, warp 1 tcgen05.mma, warps 4-11 softmax; a thread has one row and half of its 128 columns, and keeps
 // the fp32 probabilities in registers between S and dP. P and dS are rounded to bf16 for the products (2^-8 of each term at
 // most, which averages out over the sums); dS is formed from the unrounded P.
-// The tensor cores work on the next tile's scores while the softmax warps form dS, and on dP while they form P.
-// TMEM: columns 0-127 S (P or its transpose over it), 128-255 dP (dS over it), 256-383 and 384-511 the sums.
+// The next tile's scores are formed as soon as these are in registers. dQ has two sets of columns for dP (dS over it), so that a
+// tile's dP need not wait for the product with the last one's dS. For dK and dV, P has columns of its own with heads of up to 64, and
+// goes through shared memory with wider ones.
 #include "../common/per_device.h"
 #include "attention_tiles.cuh"
 
@@ -29,6 +29,15 @@ struct BwdParams {
   int* status;
 };
 
+// D (+)= A B, A: 128 x 128 bf16 in two boxes of 64 columns, B: rows of a [128][64 DB] tile
+template <int DB>
+__device__ __forceinline__ void square_product(uint32_t d, uint32_t a, uint32_t b, bool add) {
+  constexpr uint32_t idesc = make_idesc(AT_M, 64 * DB, 1, 1, 0, 1);
+  const uint64_t da = make_smem_desc(a, 16, 1024), db = make_smem_desc(b, AT_BOX, 1024);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) umma_bf16(d, da + (((k >> 2) * AT_BOX + (k & 3) * 32) >> 4), db + ((k * 2048) >> 4), idesc, k > 0 || add);
+}
+
 // TMEM column of step k of a 128 x 128 bf16 operand: two halves of 64 values, each in the first 32 columns of its 64
 __device__ __forceinline__ int half_column(int k) { return (k >> 2) * 64 + (k & 3) * 8; }
 
@@ -41,9 +50,10 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   uint8_t *sQ = smem, *sG = sQ + TILE, *sK = sG + TILE, *sV = sK + 2 * TILE;  // G: dO
-  __shared__ __align__(8) uint64_t bars[12];
+  __shared__ __align__(8) uint64_t bars[13];
   uint64_t *q_full = bars, *kv_full = bars + 1, *kv_empty = bars + 3, *s_full = bars + 5, *s_read = bars + 6, *dp_full = bars + 7, *ds_ready = bars + 8,
-           *done = bars + 9, *k_clean = bars + 10, *end_full = bars + 11;
+           *done = bars + 9, *k_clean = bars + 10, *end_full = bars + 11,
+           *dp_next = bars + 12;
   __shared__ uint32_t tmem_slot;
   __shared__ float part[AT_M];
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -69,6 +79,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
     mbar_init(done, 1);
     mbar_init(k_clean, 64);
     mbar_init(end_full, 1);
+    mbar_init(dp_next, 1);
     mbar_fence_init();
   }
   if (warp == 2) {
@@ -114,29 +125,30 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
       bool ok = warp_wait(q_full, 0) && arrived(0);
       if (ok) {
         tc_fence_after_sync();
-        issue([&] { scores_product<DB>(tmem, q, k, ks); });
-        issue([&] { umma_commit(s_full); });
-        issue([&] { scores_product<DB>(tmem + 128, g, v, ks); });
-        issue([&] { umma_commit(dp_full); });
+        auto scores = [&](int u) {
+          issue([&] {
+            scores_product<DB>(tmem, q, k + (u & 1) * TILE, ks);
+            umma_commit(s_full);
+            scores_product<DB>(tmem + 128 + (u & 1) * 128, g, v + (u & 1) * TILE, ks);
+            umma_commit(u & 1 ? dp_next : dp_full);  // one for each set of columns
+          });
+        };
+        scores(0);
         for (int u = 0; u < n && ok; ++u) {
-          const int s = u & 1, t = s ^ 1;
-          const bool next = u + 1 < n;
-          if (next) {
+          const int s = u & 1;
+          if (u + 1 < n) {  // the other dP columns were read by the product before
             ok = warp_wait(s_read, u & 1) && arrived(u + 1);
             if (!ok) break;
             tc_fence_after_sync();
-            issue([&] { scores_product<DB>(tmem, q, k + t * TILE, ks); });
-            issue([&] { umma_commit(s_full); });
+            scores(u + 1);
           }
           ok = warp_wait(ds_ready, u & 1);
           if (!ok) break;
           tc_fence_after_sync();
-          issue([&] { rows_product<DB, 0, 8>(tmem + 256, tmem + 128, k + s * TILE, u > 0, half_column); });
-          issue([&] { umma_commit(kv_empty + s); });
-          if (next) {
-            issue([&] { scores_product<DB>(tmem + 128, g, v + t * TILE, ks); });
-            issue([&] { umma_commit(dp_full); });
-          }
+          issue([&] {
+            rows_product<DB, 0, 8>(tmem + 384, tmem + 128 + s * 128, k + s * TILE, u > 0, half_column);
+            umma_commit(kv_empty + s);
+          });
         }
         if (ok) issue([&] { umma_commit(done); });
       }
@@ -156,7 +168,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
   } else {
     const int half = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane, t = q0 + row;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-    const uint32_t tS = tmem + lane_base + half * 64, tP = tS + 128;
+    const uint32_t tS = tmem + lane_base + half * 64;
     const int padded = (p.a.T + AT_M - 1) / AT_M * AT_M;
     const long long at = ((long long)b * p.a.H + h) * padded + t;
     const float lse = p.lse[at];
@@ -216,10 +228,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
       };
       weights(x, 0);
       weights(y, 32);
-      ok = warp_wait(dp_full, u & 1);
+      ok = warp_wait(u & 1 ? dp_next : dp_full, (u >> 1) & 1);
       if (!ok) break;
       tc_fence_after_sync();
       const uint64_t dd = pack_f2(-delta, -delta);
+      const uint32_t tP = tS + 128 + (u & 1) * 128;
       auto slopes = [&](uint32_t (&r)[32], int c0) {
         uint32_t d[32], o[16];
         tmem_load(tP + c0, d);
@@ -248,7 +261,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
       uint32_t v[16] = {};
       if (n > 0) {
         __syncwarp();
-        tmem_load(tmem + lane_base + 256 + c, v);
+        tmem_load(tmem + lane_base + 384 + c, v);
       }
       if (t < p.a.T) store_row16(o, c, p.a.D, v, n > 0 ? p.a.scale : 0.f);
     }
@@ -267,14 +280,19 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
                                                                       const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                                                                       const BwdParams p) {
   constexpr int TILE = DB * AT_BOX, STATS = 2 * AT_M * 4;  // lse and delta of a query tile
-  extern __shared__ uint8_t raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  uint8_t *sK = smem, *sV = sK + TILE, *sQ = sV + TILE, *sG = sQ + 2 * TILE;
-  float* sStat = reinterpret_cast<float*>(sG + 2 * TILE);
-  __shared__ __align__(8) uint64_t bars[10];
+  // TMEM columns: S 0-127, dP (dS over it) 128-255, P where it fits (else it is in shared memory), and the sums
+  constexpr uint32_t P_AT = 256, V_AT = DB == 1 ? 384 : 256, K_AT = DB == 1 ? 448 : 384;
+  extern __shared__ __align__(1024) uint8_t smem[];  // no other shared memory: it starts on a tile's boundary, which is looked at below
+  uint8_t *sK = smem, *sV = sK + TILE, *sQ = sV + TILE, *sG = sQ + 2 * TILE, *sP = sG + 2 * TILE;
+  float* sStat = reinterpret_cast<float*>(sP + (DB == 1 ? 0 : 2 * AT_BOX));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sStat + 4 * AT_M);
   uint64_t *kv_full = bars, *q_full = bars + 1, *q_empty = bars + 3, *s_full = bars + 5, *p_ready = bars + 6, *dp_full = bars + 7, *ds_ready = bars + 8,
-           *done = bars + 9;
-  __shared__ uint32_t tmem_slot;
+           *done = bars + 9, *s_read = bars + 10, *p_free = bars + 11;
+  uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 12);
+  if ((smem_u32(smem) & 1023) != 0) {
+    if (threadIdx.x == 0 && p.status) *p.status = ST_BAD_ARGUMENT;
+    return;
+  }
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int kvh = blockIdx.x % p.a.G, b = blockIdx.x / p.a.G, rep = p.a.H / p.a.G;
   const int k0 = blockIdx.y * AT_M;  // with a causal mask the first keys are seen by the most queries
@@ -294,6 +312,8 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
     mbar_init(dp_full, 1);
     mbar_init(ds_ready, 256);
     mbar_init(done, 1);
+    mbar_init(s_read, 256);
+    mbar_init(p_free, 1);
     mbar_fence_init();
   }
   if (warp == 2) {
@@ -341,33 +361,45 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
       bool ok = warp_wait(kv_full, 0) && arrived(0);
       if (ok) {
         tc_fence_after_sync();
-        issue([&] { scores_product<DB>(tmem, k, q, ks); });
-        issue([&] { umma_commit(s_full); });
-        issue([&] { scores_product<DB>(tmem + 128, v, g, ks); });
-        issue([&] { umma_commit(dp_full); });
+        auto scores = [&](int u) {
+          issue([&] {
+            scores_product<DB>(tmem, k, q + (u & 1) * TILE, ks);
+            umma_commit(s_full);
+          });
+        };
+        auto slopes = [&](int u) {
+          issue([&] {
+            scores_product<DB>(tmem + 128, v, g + (u & 1) * TILE, ks);
+            umma_commit(dp_full);
+          });
+        };
+        scores(0);
+        slopes(0);
         for (int u = 0; u < n && ok; ++u) {
-          const int s = u & 1, t = s ^ 1;
+          const int s = u & 1;
           const bool next = u + 1 < n;
+          if (next) {  // the softmax warps have the scores in registers
+            ok = warp_wait(s_read, u & 1) && arrived(u + 1);
+            if (!ok) break;
+            tc_fence_after_sync();
+            scores(u + 1);
+          }
           ok = warp_wait(p_ready, u & 1);
           if (!ok) break;
           tc_fence_after_sync();
-          issue([&] { rows_product<DB, 0, 8>(tmem + 256, tmem, g + s * TILE, u > 0, half_column); });
-          if (next) {
-            ok = arrived(u + 1);
-            if (!ok) break;
-            tc_fence_after_sync();
-            issue([&] { scores_product<DB>(tmem, k, q + t * TILE, ks); });  // behind the product that reads P
-            issue([&] { umma_commit(s_full); });
-          }
+          issue([&] {
+            if constexpr (DB == 1) rows_product<DB, 0, 8>(tmem + V_AT, tmem + P_AT, g + s * TILE, u > 0, [](int k) { return k * 8; });
+            else square_product<DB>(tmem + V_AT, smem_u32(sP), g + s * TILE, u > 0);
+            umma_commit(p_free);
+          });
           ok = warp_wait(ds_ready, u & 1);
           if (!ok) break;
           tc_fence_after_sync();
-          issue([&] { rows_product<DB, 0, 8>(tmem + 384, tmem + 128, q + s * TILE, u > 0, half_column); });
-          issue([&] { umma_commit(q_empty + s); });
-          if (next) {
-            issue([&] { scores_product<DB>(tmem + 128, v, g + t * TILE, ks); });
-            issue([&] { umma_commit(dp_full); });
-          }
+          issue([&] {
+            rows_product<DB, 0, 8>(tmem + K_AT, tmem + 128, q + s * TILE, u > 0, half_column);
+            umma_commit(q_empty + s);
+          });
+          if (next) slopes(u + 1);  // behind the product that reads dS from the same columns
         }
         if (ok) issue([&] { umma_commit(done); });
       }
@@ -390,6 +422,13 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
       tc_fence_after_sync();
       uint32_t x[32], y[32];
       tmem_load(tS, x, y);
+      tc_fence_before_sync();
+      mbar_arrive(s_read);
+      if (u > 0) {  // the product that read the last weights is done
+        ok = warp_wait(p_free, (u - 1) & 1);
+        if (!ok) break;
+        tc_fence_after_sync();
+      }
       const uint64_t cc = pack_f2(p.scale2, p.scale2);
       auto weights = [&](uint32_t (&r)[32], int c0) {
         uint32_t o[16];
@@ -408,11 +447,18 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
           o[i / 2] = pack_bf16x2(a[0], a[1]);
           o[i / 2 + 1] = pack_bf16x2(a[2], a[3]);
         }
-        tmem_st_32x32b_x16(tS + c0 / 2, o);
+        if constexpr (DB == 1) {
+          tmem_st_32x32b_x16(tmem + lane_base + P_AT + half * 32 + c0 / 2, o);
+        } else {  // 16-byte pieces of the row, as TMA would have swizzled them
+          uint4* at = reinterpret_cast<uint4*>(sP + half * AT_BOX + row * 128);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) at[(c0 / 8 + i) ^ (row & 7)] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        }
       };
       weights(x, 0);
       weights(y, 32);
-      tmem_st_wait();
+      if constexpr (DB == 1) tmem_st_wait();
+      else fence_proxy_async_smem();
       tc_fence_before_sync();
       mbar_arrive(p_ready);
       ok = warp_wait(dp_full, u & 1);
@@ -453,7 +499,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
       uint32_t v[16] = {};
       if (n > 0) {
         __syncwarp();
-        tmem_load(tmem + lane_base + 256 + half * 128 + c, v);
+        tmem_load(tmem + lane_base + (half == 0 ? V_AT : K_AT) + c, v);
       }
       if (!inside) {  // what keys past the length hold does not count
 #pragma unroll
@@ -473,7 +519,8 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
 template <int DB>
 void run_bwd(const AttentionBwd& f, cudaStream_t s) {
   const AttentionShape& a = f.a;
-  constexpr int smem = 6 * DB * AT_BOX + 1024, smem_kv = smem + 2 * 2 * AT_M * 4;
+  constexpr int smem = 6 * DB * AT_BOX + 1024, smem_kv = 6 * DB * AT_BOX + (DB == 1 ? 0 : 2 * AT_BOX) + 4 * AT_M * 4 + 14 * 8;
+  static_assert(smem <= 227 * 1024 && smem_kv <= 227 * 1024, "shared memory of a block");
   const CUtensorMap tq = attention_map(f.q, a.D, a.T, a.H, a.B), tg = attention_map(f.dout, a.D, a.T, a.H, a.B),
                     tk = attention_map(f.k, a.D, a.S, a.G, a.B), tv = attention_map(f.v, a.D, a.S, a.G, a.B);
   const BwdParams p{a, f.out, f.dout, f.lse, f.delta, f.dq, f.dk, f.dv, a.scale * LOG2E, f.status};

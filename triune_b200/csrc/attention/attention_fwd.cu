@@ -11,9 +11,11 @@
 //   warps 2-3   pass the value tiles on; in those where not all keys are visible to all queries, values that are no numbers, and
 //               those of keys past the sequence's length, are set to zero first, since zero weights would not take them out
 //   warps 4-7, 8-11   softmax, one query per thread (TMEM lane = query)
-// P (bf16: every weight is off by 2^-8 of itself at most, which averages out over the keys) takes the first half of its S columns. The
-// running maximum is lazy: sums are rescaled only when it has grown by more than 2^8. fp32 sums take the weights before rounding.
-// TMEM: columns 0-127 S_0, 128-255 S_1, 256-383 O_0, 384-511 O_1.
+// Heads of up to 64 have columns for scores and weights apart, so that the scores of a group's next tile are ready when it is done
+// with one; with wider heads, whose sums take the room, weights lie over the scores, and the next scores wait for the product.
+// P is bf16 (every weight is off by 2^-8 of itself at most, which averages out over the keys); fp32 sums take the weights before
+// rounding. The running maximum is lazy: sums are rescaled only when it has grown by more than 2^8.
+// TMEM: S_0 0-127, S_1 128-255, O_0 and O_1 from 256 on, P_0 384-447, P_1 448-511 or over the scores.
 #include <algorithm>
 #include <type_traits>
 
@@ -71,12 +73,15 @@ template <int DB, bool PAIR, bool SCALED>
 __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                                                                       const __grid_constant__ CUtensorMap tmV, const FwdParams p) {
   constexpr int QT = PAIR ? 2 : 1, TILE = DB * AT_BOX;
+  // TMEM columns of the groups' scores, weights and sums. APART: weights do not lie over the scores
+  constexpr bool APART = DB == 1;
+  constexpr int S_AT[2] = {0, 128}, P_AT[2] = {APART ? 384 : 0, APART ? 448 : 128}, O_AT[2] = {256, 256 + 64 * DB};
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   uint8_t *sQ = smem, *sK = sQ + QT * TILE, *sV = sK + 2 * TILE;
-  __shared__ __align__(8) uint64_t bars[19];
-  uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 7, *s_full = bars + 9, *p_ready = bars + 11,
-           *o_full = bars + 13, *v_clean = bars + 15, *p_half = bars + 17;
+  __shared__ __align__(8) uint64_t bars[21];
+  uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 7, *v_clean = bars + 9, *s_full = bars + 11,
+           *s_read = bars + 13, *p_half = bars + 15, *p_ready = bars + 17, *o_done = bars + 19;
   __shared__ uint32_t tmem_slot;
   __shared__ int special;  // a value that is no number was set to zero
   __shared__ float2 other[AT_M];
@@ -126,7 +131,8 @@ __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __gr
       mbar_init(s_full + i, 1);
       mbar_init(p_ready + i, 128);
       mbar_init(p_half + i, 128);
-      mbar_init(o_full + i, 1);
+      mbar_init(s_read + i, 128);
+      mbar_init(o_done + i, 1);
       mbar_init(v_clean + i, 64);
     }
     mbar_fence_init();
@@ -139,7 +145,9 @@ __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __gr
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = uniform(tmem_slot);
-
+  // 128 threads of 88 registers and 256 of 208 are 64512, the 384 * 168 that the block is launched with
+  if (warp < 4) {
+  registers_down<88>();
   if (warp == 0) {
     if (lane == 0 && j1 > j0) {
       prefetch_tmap(&tmQ);
@@ -175,69 +183,72 @@ __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __gr
     if (j1 > j0) {
       const int ks = (p.a.D + 15) / 16;
       const uint32_t qa = smem_u32(sQ), ka = smem_u32(sK), va = smem_u32(sV);
-      auto scores = [&](int w, int j) {
+      int issued[2] = {0, 0}, done[2] = {0, 0};
+      // Scores of tile j for group w, behind its read of the last ones (APART), or behind the product that read the weights over them
+      auto scores = [&](auto group, int j) {
+        constexpr int w = decltype(group)::value;
+        if (APART && issued[w] > 0 && !warp_wait(s_read + w, (issued[w] - 1) & 1)) return false;
+        tc_fence_after_sync();
         issue([&] {
-          scores_product<DB>(tmem + w * 128, qa + (PAIR ? w : 0) * TILE, ka + ((j - j0) & 1) * TILE, ks);
+          scores_product<DB>(tmem + S_AT[w], qa + (PAIR ? w : 0) * TILE, ka + ((j - j0) & 1) * TILE, ks);
           umma_commit(s_full + w);
         });
+        ++issued[w];
+        return true;
       };
-      auto values = [&](int w, int j, auto half) {
-        constexpr int K0 = decltype(half)::value * 4;
+      auto values = [&](auto group, int j) {
+        constexpr int w = decltype(group)::value;
+        const uint32_t v = va + ((j - j0) & 1) * TILE;
+        const bool add = done[w] > 0;
+        if (!warp_wait(p_half + w, done[w] & 1)) return false;
+        tc_fence_after_sync();
+        issue([&] { rows_product<DB, 0, 4>(tmem + O_AT[w], tmem + P_AT[w], v, add, [](int k) { return k * 8; }); });
+        if (!warp_wait(p_ready + w, done[w] & 1)) return false;
+        tc_fence_after_sync();
         issue([&] {
-          rows_product<DB, K0, 4>(tmem + 256 + w * 128, tmem + w * 128, va + ((j - j0) & 1) * TILE, j != range[w].x, [](int k) { return k * 8; });
+          rows_product<DB, 4, 4>(tmem + O_AT[w], tmem + P_AT[w], v, true, [](int k) { return k * 8; });
+          umma_commit(o_done + w);
         });
+        ++done[w];
+        return true;
       };
       auto commit = [&](uint64_t* bar) { issue([&] { umma_commit(bar); }); };
-      int done[2] = {0, 0};
       auto k_arrived = [&](int j) { return warp_wait(k_full + ((j - j0) & 1), ((j - j0) >> 1) & 1); };
+      constexpr std::integral_constant<int, 0> g0{};
+      constexpr std::integral_constant<int, 1> g1{};
       bool ok = warp_wait(q_full, 0) && k_arrived(j0);
-      if (ok) {
-        tc_fence_after_sync();
-        if constexpr (PAIR) {
-          for (int w = 0; w < 2; ++w)
-            if (takes(w, j0)) scores(w, j0);
-          commit(k_empty);
-        } else {
-          scores(0, j0);
-          commit(k_empty);
-          if (j1 - j0 > 1) {
-            ok = k_arrived(j0 + 1);
-            if (ok) {
-              tc_fence_after_sync();
-              scores(1, j0 + 1);
-              commit(k_empty + 1);
-            }
-          }
+      if constexpr (PAIR) {
+        if (takes(0, j0)) ok = ok && scores(g0, j0);
+        if (takes(1, j0)) ok = ok && scores(g1, j0);
+        commit(k_empty);
+      } else {
+        ok = ok && scores(g0, j0);
+        commit(k_empty);
+        if (j1 - j0 > 1) {
+          ok = ok && k_arrived(j0 + 1) && scores(g1, j0 + 1);
+          commit(k_empty + 1);
         }
-        for (int j = j0; j < j1 && ok; ++j) {
-          const int s = (j - j0) & 1;
-          ok = warp_wait(v_clean + s, ((j - j0) >> 1) & 1);
-          const int jn = j + step;  // the next tile whose scores are issued
-          if (ok && jn < j1) ok = k_arrived(jn);
-          for (int w = 0; w < 2 && ok; ++w) {
-            const bool now = takes(w, j), next = jn < j1 && (PAIR ? takes(w, jn) : now);
-            if (now) {
-              ok = warp_wait(p_half + w, done[w] & 1);
-              if (!ok) break;
-              tc_fence_after_sync();
-              values(w, j, std::integral_constant<int, 0>{});
-              ok = warp_wait(p_ready + w, done[w] & 1);
-              ++done[w];
-              if (!ok) break;
-              tc_fence_after_sync();
-              values(w, j, std::integral_constant<int, 1>{});
-              if (done[w] == count(w)) commit(o_full + w);
-            }
-            if (next) scores(w, jn);
-          }
-          if (!ok) break;
-          commit(v_empty + s);
-          if (jn < j1) commit(k_empty + ((jn - j0) & 1));
-        }
+      }
+      auto turn = [&](auto group, int j, int jn) {
+        constexpr int w = decltype(group)::value;
+        const int s = (j - j0) & 1;
+        const bool next = jn < j1 && takes(w, jn);
+        if (APART && next && !scores(group, jn)) return false;
+        if (takes(w, j) && !(warp_wait(v_clean + s, ((j - j0) >> 1) & 1) && values(group, j))) return false;
+        return APART || !next || scores(group, jn);
+      };
+      for (int j = j0; j < j1 && ok; ++j) {
+        const int s = (j - j0) & 1, jn = j + step;
+        const bool next = jn < j1;
+        if (next) ok = k_arrived(jn);
+        if (PAIR || s == 0) ok = ok && turn(g0, j, jn);
+        if (PAIR || s == 1) ok = ok && turn(g1, j, jn);
+        if (next) commit(k_empty + ((jn - j0) & 1));
+        commit(v_empty + s);
       }
       if (!ok && p.status) *p.status = ST_TIMEOUT_FULL;
     }
-  } else if (warp < 4) {
+  } else {
     const int tid = threadIdx.x - 64;
     bool ok = true;
     for (int j = j0; j < j1 && ok; ++j) {
@@ -271,11 +282,14 @@ __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __gr
       mbar_arrive(v_clean + s);
     }
     if (!ok && p.status) *p.status = ST_TIMEOUT_FULL;
+  }
   } else {
+    registers_up<208>();
     const int w = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const int first = q0 + (PAIR ? w : 0) * AT_M, t = first + row;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-    const uint32_t tS = tmem + lane_base + w * 128, tO = tmem + lane_base + 256 + w * 128;
+    const uint32_t tS = tmem + lane_base + (w == 0 ? S_AT[0] : S_AT[1]), tP = tmem + lane_base + (w == 0 ? P_AT[0] : P_AT[1]),
+                   tO = tmem + lane_base + (w == 0 ? O_AT[0] : O_AT[1]);
     const float c2 = p.scale2;
     const int n = count(w), lo = vis.low(t), hi = vis.high(t);
     float m = -INFINITY, l = 0.f;
@@ -284,14 +298,14 @@ __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __gr
     auto softmax = [&](auto some, int it, int key) {
       constexpr bool MASKED = decltype(some)::value;
       const int c_lo = lo - key, c_hi = hi - key;  // visible columns
-      // Half of the 128 scores fits beside the rest: the second half is read for its maximum, and again behind the first half's weights
-      uint32_t x[32], y[32];
+      uint32_t x[4][32];
       float top[4];
       auto chunk_max = [&](uint32_t (&r)[32], int c) {
         if constexpr (MASKED) {
+          const uint32_t see = visible_bits(c_lo - 32 * c, c_hi - 32 * c);
 #pragma unroll
           for (int i = 0; i < 32; ++i)
-            if (32 * c + i > c_hi || 32 * c + i < c_lo) r[i] = 0xff800000u;  // -inf
+            if (!(see >> i & 1)) r[i] = 0xff800000u;  // -inf
         }
         float a = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])), e = fmaxf(__uint_as_float(r[2]), __uint_as_float(r[3]));
 #pragma unroll
@@ -301,12 +315,12 @@ __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __gr
         }
         top[c] = fmaxf(a, e);
       };
-      tmem_load(tS + 64, x, y);
-      chunk_max(x, 2);
-      chunk_max(y, 3);
-      tmem_load(tS, x, y);
-      chunk_max(x, 0);
-      chunk_max(y, 1);
+      tmem_load(tS, x[0], x[1]);
+      tmem_load(tS + 64, x[2], x[3]);
+      tc_fence_before_sync();
+      if (APART) mbar_arrive(s_read + w);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) chunk_max(x[c], c);
       float f0 = c2, f1 = c2;  // what the scores of the two blocks of 64 keys are multiplied by
       [[maybe_unused]] uint64_t v0 = 0, v1 = 0;
       if constexpr (SCALED) {
@@ -327,6 +341,10 @@ __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __gr
         l *= f;
       }
       const bool any = __any_sync(0xffffffffu, grow);  // also brings the warp together again
+      if (APART && it > 0) {  // the weights' columns and the sums are free again
+        if (!warp_wait(o_done + w, (it - 1) & 1)) return false;
+        tc_fence_after_sync();
+      }
       if (it > 0 && any) {
         for (int c = 0; c < 64 * DB; c += 16) {
           uint32_t o[16];
@@ -341,6 +359,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __gr
       uint64_t sum2 = pack_f2(0.f, 0.f);
       auto weights = [&](uint32_t (&r)[32], int c) {
         const float fc = c < 2 ? f0 : f1;
+        [[maybe_unused]] const uint32_t see = MASKED && SCALED ? visible_bits(c_lo - 32 * c, c_hi - 32 * c) : 0u;
         const uint64_t cc = pack_f2(fc, fc);
         uint32_t q[16];
 #pragma unroll
@@ -354,10 +373,9 @@ __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __gr
             unpack_f2(y, a, z);
             a = ex2(a);
             z = ex2(z);
-            if constexpr (MASKED) {  // also where a block's scale, zero or no number, was multiplied by minus infinity
-              const int k = 32 * c + 2 * i;
-              a = k <= c_hi && k >= c_lo ? a : 0.f;
-              z = k + 1 <= c_hi && k + 1 >= c_lo ? z : 0.f;
+            if constexpr (MASKED && SCALED) {  // where a block's scale, zero or no number, was multiplied by minus infinity
+              a = see >> (2 * i) & 1 ? a : 0.f;
+              z = see >> (2 * i + 1) & 1 ? z : 0.f;
             }
             e = pack_f2(a, z);
           }
@@ -365,31 +383,30 @@ __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __gr
           if constexpr (SCALED) e = mul2(e, c < 2 ? v0 : v1);
           q[i] = f2_to_bf16x2(e);
         }
-        tmem_st_32x32b_x16(tS + 16 * c, q);  // over columns that this thread has read
+        tmem_st_32x32b_x16(tP + 16 * c, q);
         if (c & 1) {  // the product starts on the first half of the keys
           tmem_st_wait();
           tc_fence_before_sync();
           mbar_arrive(c == 1 ? p_half + w : p_ready + w);
         }
       };
-      weights(x, 0);
-      weights(y, 1);
-      tmem_load(tS + 64, x, y);
-      weights(x, 2);
-      weights(y, 3);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) weights(x[c], c);
       float s0, s1;
       unpack_f2(sum2, s0, s1);
       l += s0 + s1;
+      return true;
     };
     for (int it = 0; it < n; ++it) {
       const int key = (range[w].x + it * step) * AT_M;
       ok = warp_wait(s_full + w, it & 1);
       if (!ok) break;
       tc_fence_after_sync();
-      if (vis.whole(first, first + AT_M - 1, key)) softmax(std::false_type{}, it, key);
-      else softmax(std::true_type{}, it, key);
+      if (vis.whole(first, first + AT_M - 1, key)) ok = softmax(std::false_type{}, it, key);
+      else ok = softmax(std::true_type{}, it, key);
+      if (!ok) break;
     }
-    if (ok && n > 0) ok = warp_wait(o_full + w, 0);
+    if (ok && n > 0) ok = warp_wait(o_done + w, (n - 1) & 1);
     tc_fence_after_sync();
     float share = 1.f;  // of this group's sums in the row
     float* half = reinterpret_cast<float*>(sK);

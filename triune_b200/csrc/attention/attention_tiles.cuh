@@ -43,6 +43,12 @@ struct Visible {  // of one sequence
   __device__ __forceinline__ bool whole(int t0, int t1, int key) const { return low(t1) <= key && high(t0) >= key + AT_M - 1; }
 };
 
+// Bits lo .. hi of 32, whichever of them there are
+__device__ __forceinline__ uint32_t visible_bits(int lo, int hi) {
+  const uint32_t below = hi >= 31 ? 0xffffffffu : hi < 0 ? 0u : (2u << hi) - 1u, before = lo <= 0 ? 0u : lo > 31 ? 0xffffffffu : (1u << lo) - 1u;
+  return below & ~before;
+}
+
 // 64-wide boxes of 128 rows of one head: coordinates (column, row, head, batch); what is outside reads as zero
 inline CUtensorMap attention_map(const AttentionView& v, int d, int rows, int heads, int batch, uint32_t box_rows = AT_M) {
   return make_tmap_4d_bf16(v.p, {(uint64_t)d, (uint64_t)rows, (uint64_t)heads, (uint64_t)batch},
@@ -53,6 +59,16 @@ __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint3
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(smem_dst)),
                "l"(src), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
+}
+
+// A warpgroup's registers per thread from here on; the shares of a block's warpgroups have to fit what it was launched with.
+template <int N>
+__device__ __forceinline__ void registers_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void registers_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 // Products of tiles, issued by one elected thread of a warp that stays together: every thread comes to the waits and to the end of each

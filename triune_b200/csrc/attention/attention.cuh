@@ -30,10 +30,11 @@ struct AttentionShape {
   long long start;
 };
 
-// Rows of the statistics [B, H, attention_rows(T)]: whole tiles, so that they are fetched in whole tiles. Rows past T: +inf and zero.
+// Rows of the statistics [B, H, attention_rows(T)]: whole tiles, so that they are fetched in whole tiles.
 inline int attention_rows(int T) { return (T + 127) / 128 * 128; }
 
-// out [B, T, H, D] contiguous; lse (or null): base-2 logarithm of the softmax's sum, scores times log2(e), +inf for empty rows.
+// out [B, T, H, D] contiguous; lse (or null): minus the base-2 logarithm of the sum of the rows' exponentials; -inf for rows that see
+// no key and rows past T, whose weights are zero that way.
 // part (attention_fwd_scratch(a) bytes or null): where the keys of few queries are split over blocks.
 // k_scales, v_scales (or null): [B, G, blocks], what blocks of 64 keys and values are multiplied by.
 struct AttentionFwd {
@@ -49,7 +50,8 @@ struct AttentionFwd {
 long long attention_fwd_scratch(const AttentionShape& a);
 void launch_attention_fwd(const AttentionFwd& f, cudaStream_t s);
 
-// dq [B, T, H, D], dk, dv [B, S, G, D] contiguous; delta [B, H, attention_rows(T)] is written and read.
+// dq [B, T, H, D], dk, dv [B, S, G, D] contiguous; delta [B, H, attention_rows(T)] is written and read
+// (minus the rows' sums of dout times out).
 struct AttentionBwd {
   AttentionShape a;
   AttentionView q, k, v, out, dout;

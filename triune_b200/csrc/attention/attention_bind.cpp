@@ -112,7 +112,7 @@ std::vector<Tensor> attention_fwd(const Tensor& q, const Tensor& k, const Tensor
   if (out.numel() == 0) return {out, lse};
   if (f.a.S == 0) {
     out.zero_();
-    if (want_lse) lse.fill_(INFINITY);
+    if (want_lse) lse.fill_(-INFINITY);
     return {out, lse};
   }
   const long long bytes = tb::attention_fwd_scratch(f.a);

@@ -11,6 +11,8 @@
 // The next tile's scores are formed as soon as these are in registers. dQ has two sets of columns for dP (dS over it), so that a
 // tile's dP need not wait for the product with the last one's dS. For dK and dV, P has columns of its own with heads of up to 64, and
 // goes through shared memory with wider ones.
+#include <type_traits>
+
 #include "../common/per_device.h"
 #include "attention_tiles.cuh"
 
@@ -46,14 +48,14 @@ template <int DB>
 __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
                                                                      const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                                                                      const BwdParams p) {
-  constexpr int TILE = DB * AT_BOX;
+  // K is held until the product with dS, V only until dP is there: longer and shorter rings
+  constexpr int TILE = DB * AT_BOX, NK = DB == 1 ? 4 : 3, NV = DB == 1 ? 3 : 2;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  uint8_t *sQ = smem, *sG = sQ + TILE, *sK = sG + TILE, *sV = sK + 2 * TILE;  // G: dO
-  __shared__ __align__(8) uint64_t bars[13];
-  uint64_t *q_full = bars, *kv_full = bars + 1, *kv_empty = bars + 3, *s_full = bars + 5, *s_read = bars + 6, *dp_full = bars + 7, *ds_ready = bars + 8,
-           *done = bars + 9, *k_clean = bars + 10, *end_full = bars + 11,
-           *dp_next = bars + 12;
+  uint8_t *sQ = smem, *sG = sQ + TILE, *sK = sG + TILE, *sV = sK + NK * TILE;  // G: dO
+  __shared__ __align__(8) uint64_t bars[10 + 2 * NK + 2 * NV];
+  uint64_t *q_full = bars, *s_full = bars + 1, *s_read = bars + 2, *dp_full = bars + 3, *dp_next = bars + 4, *ds_ready = bars + 5, *done = bars + 6,
+           *k_clean = bars + 7, *end_full = bars + 8, *k_full = bars + 10, *k_empty = k_full + NK, *v_full = k_empty + NK, *v_empty = v_full + NV;
   __shared__ uint32_t tmem_slot;
   __shared__ float part[AT_M];
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -68,9 +70,13 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(kv_full + i, 1);
-      mbar_init(kv_empty + i, 1);
+    for (int i = 0; i < NK; ++i) {
+      mbar_init(k_full + i, 1);
+      mbar_init(k_empty + i, 1);
+    }
+    for (int i = 0; i < NV; ++i) {
+      mbar_init(v_full + i, 1);
+      mbar_init(v_empty + i, 1);
     }
     mbar_init(s_full, 1);
     mbar_init(s_read, 256);
@@ -103,17 +109,19 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
       }
       bool ok = true;
       for (int u = 0; u < n && ok; ++u) {
-        const int s = u & 1;
-        if (u >= 2) ok = mbar_wait(kv_empty + s, ((u >> 1) & 1) ^ 1);
+        const int ks = u % NK, vs = u % NV;
+        uint64_t *kf = u == ragged ? end_full : k_full + ks, *vf = u == ragged ? end_full : v_full + vs;
+        if (u >= NK) ok = mbar_wait(k_empty + ks, ((u / NK) & 1) ^ 1);
+        if (u >= NV) ok = ok && mbar_wait(v_empty + vs, ((u / NV) & 1) ^ 1);
         if (!ok) break;
-        uint64_t* full = u == ragged ? end_full : kv_full + s;
-        mbar_expect_tx(full, 2 * TILE);
-        for (int d = 0; d < DB; ++d) {
-          tma_load_4d(sK + s * TILE + d * AT_BOX, &tmK, full, d * 64, (range.x + u) * AT_M, kvh, b);
-          tma_load_4d(sV + s * TILE + d * AT_BOX, &tmV, full, d * 64, (range.x + u) * AT_M, kvh, b);
-        }
+        mbar_expect_tx(kf, u == ragged ? 2 * TILE : TILE);
+        if (u != ragged) mbar_expect_tx(vf, TILE);
+        for (int d = 0; d < DB; ++d) tma_load_4d(sK + ks * TILE + d * AT_BOX, &tmK, kf, d * 64, (range.x + u) * AT_M, kvh, b);
+        for (int d = 0; d < DB; ++d) tma_load_4d(sV + vs * TILE + d * AT_BOX, &tmV, vf, d * 64, (range.x + u) * AT_M, kvh, b);
       }
-      for (int u = max(0, n - 2); u < n && ok; ++u) ok = mbar_wait(kv_empty + (u & 1), (u >> 1) & 1);  // nothing may arrive once the block is gone
+      // nothing may arrive once the block is gone
+      for (int u = max(0, n - NK); u < n && ok; ++u) ok = mbar_wait(k_empty + u % NK, (u / NK) & 1);
+      for (int u = max(0, n - NV); u < n && ok; ++u) ok = mbar_wait(v_empty + u % NV, (u / NV) & 1);
       if (!ok && p.status) *p.status = ST_TIMEOUT_EMPTY;
     }
     __syncwarp();
@@ -121,33 +129,33 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
     if (n > 0) {
       const int ks = (p.a.D + 15) / 16;
       const uint32_t q = smem_u32(sQ), g = smem_u32(sG), k = smem_u32(sK), v = smem_u32(sV);
-      auto arrived = [&](int u) { return u == ragged ? warp_wait(end_full, 0) && warp_wait(k_clean, 0) : warp_wait(kv_full + (u & 1), (u >> 1) & 1); };
-      bool ok = warp_wait(q_full, 0) && arrived(0);
-      if (ok) {
+      // scores and dP of a tile, as its keys and values arrive
+      auto scores = [&](int u) {
+        const int ks_at = u % NK, vs_at = u % NV;
+        if (!(u == ragged ? warp_wait(end_full, 0) && warp_wait(k_clean, 0) : warp_wait(k_full + ks_at, (u / NK) & 1))) return false;
         tc_fence_after_sync();
-        auto scores = [&](int u) {
-          issue([&] {
-            scores_product<DB>(tmem, q, k + (u & 1) * TILE, ks);
-            umma_commit(s_full);
-            scores_product<DB>(tmem + 128 + (u & 1) * 128, g, v + (u & 1) * TILE, ks);
-            umma_commit(u & 1 ? dp_next : dp_full);  // one for each set of columns
-          });
-        };
-        scores(0);
+        issue([&] {
+          scores_product<DB>(tmem, q, k + ks_at * TILE, ks);
+          umma_commit(s_full);
+        });
+        if (u != ragged && !warp_wait(v_full + vs_at, (u / NV) & 1)) return false;
+        issue([&] {
+          scores_product<DB>(tmem + 128 + (u & 1) * 128, g, v + vs_at * TILE, ks);
+          umma_commit(u & 1 ? dp_next : dp_full);  // one for each set of columns
+          umma_commit(v_empty + vs_at);
+        });
+        return true;
+      };
+      bool ok = warp_wait(q_full, 0) && scores(0);
+      if (ok) {
         for (int u = 0; u < n && ok; ++u) {
-          const int s = u & 1;
-          if (u + 1 < n) {  // the other dP columns were read by the product before
-            ok = warp_wait(s_read, u & 1) && arrived(u + 1);
-            if (!ok) break;
-            tc_fence_after_sync();
-            scores(u + 1);
-          }
-          ok = warp_wait(ds_ready, u & 1);
+          if (u + 1 < n) ok = warp_wait(s_read, u & 1) && scores(u + 1);  // the other dP columns were read by the product before
+          ok = ok && warp_wait(ds_ready, u & 1);
           if (!ok) break;
           tc_fence_after_sync();
           issue([&] {
-            rows_product<DB, 0, 8>(tmem + 384, tmem + 128 + s * 128, k + s * TILE, u > 0, half_column);
-            umma_commit(kv_empty + s);
+            rows_product<DB, 0, 8>(tmem + 384, tmem + 128 + (u & 1) * 128, k + u % NK * TILE, u > 0, half_column);
+            umma_commit(k_empty + u % NK);
           });
         }
         if (ok) issue([&] { umma_commit(done); });
@@ -156,7 +164,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
     }
   } else if (warp < 4) {
     if (ragged >= 0 && ragged < n) {
-      const int s = ragged & 1, keep = vis.length % AT_M;
+      const int s = ragged % NK, keep = vis.length % AT_M;
       const bool ok = mbar_wait(end_full, 0);
       if (ok)
         for (int i = threadIdx.x - 64; i < TILE / 16; i += 64)
@@ -193,66 +201,74 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
     if (half == 0) {
       dot += part[row];
       part[row] = dot;
-      p.delta[at] = dot;
+      p.delta[at] = -dot;
     }
     named_barrier<256>(1);
-    const float delta = part[row];
+    const float delta = -part[row];
     const int lo = vis.low(t), hi = vis.high(t);
     bool ok = true;
-    for (int u = 0; u < n; ++u) {
-      const int key = (range.x + u) * AT_M;
-      const bool masked = !vis.whole(q0, q0 + AT_M - 1, key);
-      const int c_lo = lo - key - half * 64, c_hi = hi - key - half * 64;
-      ok = warp_wait(s_full, u & 1);
-      if (!ok) break;
-      tc_fence_after_sync();
+    const uint64_t cc = pack_f2(p.scale2, p.scale2), mm = pack_f2(lse, lse), dd = pack_f2(delta, delta);
+    // MASKED: not all keys of the tile are visible to all queries. Invisible ones have weight and slope zero, whatever they hold.
+    auto tile = [&](auto some, int u, int c_lo, int c_hi) {
+      constexpr bool MASKED = decltype(some)::value;
+      const uint32_t tP = tS + 128 + (u & 1) * 128;
       uint32_t x[32], y[32];
       tmem_load(tS, x, y);
       tc_fence_before_sync();
       mbar_arrive(s_read);
-      const uint64_t cc = pack_f2(p.scale2, p.scale2), mm = pack_f2(-lse, -lse);
       auto weights = [&](uint32_t (&r)[32], int c0) {
+        const uint32_t see = MASKED ? visible_bits(c_lo - c0, c_hi - c0) : 0u;
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
+          const uint64_t z = fma2(pack_f2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), cc, mm);
           float a, e;
-          unpack_f2(fma2(pack_f2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), cc, mm), a, e);
+          unpack_f2(z, a, e);
           a = ex2(a);
           e = ex2(e);
-          if (masked) {
-            a = c0 + i <= c_hi && c0 + i >= c_lo ? a : 0.f;
-            e = c0 + i + 1 <= c_hi && c0 + i + 1 >= c_lo ? e : 0.f;
+          if constexpr (MASKED) {
+            a = see >> i & 1 ? a : 0.f;
+            e = see >> (i + 1) & 1 ? e : 0.f;
           }
           r[i] = __float_as_uint(a);
           r[i + 1] = __float_as_uint(e);
         }
       };
-      weights(x, 0);
-      weights(y, 32);
-      ok = warp_wait(u & 1 ? dp_next : dp_full, (u >> 1) & 1);
-      if (!ok) break;
-      tc_fence_after_sync();
-      const uint64_t dd = pack_f2(-delta, -delta);
-      const uint32_t tP = tS + 128 + (u & 1) * 128;
       auto slopes = [&](uint32_t (&r)[32], int c0) {
+        const uint32_t see = MASKED ? visible_bits(c_lo - c0, c_hi - c0) : 0u;
         uint32_t d[32], o[16];
         tmem_load(tP + c0, d);
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
-          float a, e;
-          unpack_f2(mul2(add2(pack_f2(__uint_as_float(d[i]), __uint_as_float(d[i + 1])), dd), pack_f2(__uint_as_float(r[i]), __uint_as_float(r[i + 1]))), a, e);
-          if (masked) {  // zero times what is no number
-            a = c0 + i <= c_hi && c0 + i >= c_lo ? a : 0.f;
-            e = c0 + i + 1 <= c_hi && c0 + i + 1 >= c_lo ? e : 0.f;
+          const uint64_t z = mul2(add2(pack_f2(__uint_as_float(d[i]), __uint_as_float(d[i + 1])), dd), pack_f2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])));
+          if constexpr (MASKED) {
+            float a, e;
+            unpack_f2(z, a, e);
+            o[i / 2] = pack_bf16x2(see >> i & 1 ? a : 0.f, see >> (i + 1) & 1 ? e : 0.f);
+          } else {
+            o[i / 2] = f2_to_bf16x2(z);
           }
-          o[i / 2] = pack_bf16x2(a, e);
         }
         tmem_st_32x32b_x16(tP + c0 / 2, o);  // over columns that this thread has read
       };
+      weights(x, 0);
+      if (!warp_wait(u & 1 ? dp_next : dp_full, (u >> 1) & 1)) return false;
+      tc_fence_after_sync();
       slopes(x, 0);
+      weights(y, 32);
       slopes(y, 32);
       tmem_st_wait();
       tc_fence_before_sync();
       mbar_arrive(ds_ready);
+      return true;
+    };
+    for (int u = 0; u < n; ++u) {
+      const int key = (range.x + u) * AT_M;
+      ok = warp_wait(s_full, u & 1);
+      if (!ok) break;
+      tc_fence_after_sync();
+      if (vis.whole(q0, q0 + AT_M - 1, key)) ok = tile(std::false_type{}, u, 0, 0);
+      else ok = tile(std::true_type{}, u, lo - key - half * 64, hi - key - half * 64);
+      if (!ok) break;
     }
     if (ok && n > 0) ok = warp_wait(done, 0);
     tc_fence_after_sync();
@@ -275,20 +291,23 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
 }
 
 // ---------------------------------------------------------------------------------------------------------------- keys, values
+// Stages of query tiles: what shared memory holds
+__host__ __device__ constexpr int key_stages(int db) { return db == 1 ? 3 : 2; }
+
 template <int DB>
 __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
                                                                       const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                                                                       const BwdParams p) {
-  constexpr int TILE = DB * AT_BOX, STATS = 2 * AT_M * 4;  // lse and delta of a query tile
+  constexpr int TILE = DB * AT_BOX, STATS = 2 * AT_M * 4, NQ = key_stages(DB);  // lse and delta of a query tile
   // TMEM columns: S 0-127, dP (dS over it) 128-255, P where it fits (else it is in shared memory), and the sums
   constexpr uint32_t P_AT = 256, V_AT = DB == 1 ? 384 : 256, K_AT = DB == 1 ? 448 : 384;
   extern __shared__ __align__(1024) uint8_t smem[];  // no other shared memory: it starts on a tile's boundary, which is looked at below
-  uint8_t *sK = smem, *sV = sK + TILE, *sQ = sV + TILE, *sG = sQ + 2 * TILE, *sP = sG + 2 * TILE;
+  uint8_t *sK = smem, *sV = sK + TILE, *sQ = sV + TILE, *sG = sQ + NQ * TILE, *sP = sG + NQ * TILE;
   float* sStat = reinterpret_cast<float*>(sP + (DB == 1 ? 0 : 2 * AT_BOX));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sStat + 4 * AT_M);
-  uint64_t *kv_full = bars, *q_full = bars + 1, *q_empty = bars + 3, *s_full = bars + 5, *p_ready = bars + 6, *dp_full = bars + 7, *ds_ready = bars + 8,
-           *done = bars + 9, *s_read = bars + 10, *p_free = bars + 11;
-  uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 12);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sStat + NQ * 2 * AT_M);
+  uint64_t *kv_full = bars, *s_full = bars + 1, *p_ready = bars + 2, *dp_full = bars + 3, *ds_ready = bars + 4, *done = bars + 5, *s_read = bars + 6,
+           *p_free = bars + 7, *q_full = bars + 8, *q_empty = q_full + NQ;
+  uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(q_empty + NQ);
   if ((smem_u32(smem) & 1023) != 0) {
     if (threadIdx.x == 0 && p.status) *p.status = ST_BAD_ARGUMENT;
     return;
@@ -303,7 +322,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
 
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < NQ; ++i) {
       mbar_init(q_full + i, 1);
       mbar_init(q_empty + i, 1);
     }
@@ -336,9 +355,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
         tma_load_4d(sV + d * AT_BOX, &tmV, kv_full, d * 64, k0, kvh, b);
       }
       bool ok = true;
+      int i = 0, head = 0;
       for (int u = 0; u < n && ok; ++u) {
-        const int s = u & 1, h = kvh * rep + u / per, t0 = (i0 + u % per) * AT_M;
-        if (u >= 2) ok = mbar_wait(q_empty + s, ((u >> 1) & 1) ^ 1);
+        const int s = u % NQ, h = kvh * rep + head, t0 = (i0 + i) * AT_M;
+        if (++i == per) i = 0, ++head;
+        if (u >= NQ) ok = mbar_wait(q_empty + s, ((u / NQ) & 1) ^ 1);
         if (!ok) break;
         mbar_expect_tx(q_full + s, 2 * TILE + STATS);
         for (int d = 0; d < DB; ++d) {
@@ -349,7 +370,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
         bulk_load(sStat + s * 2 * AT_M, p.lse + at, AT_M * 4, q_full + s);
         bulk_load(sStat + s * 2 * AT_M + AT_M, p.delta + at, AT_M * 4, q_full + s);
       }
-      for (int u = max(0, n - 2); u < n && ok; ++u) ok = mbar_wait(q_empty + (u & 1), (u >> 1) & 1);
+      for (int u = max(0, n - NQ); u < n && ok; ++u) ok = mbar_wait(q_empty + u % NQ, (u / NQ) & 1);
       if (!ok && p.status) *p.status = ST_TIMEOUT_EMPTY;
     }
     __syncwarp();
@@ -357,26 +378,26 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
     if (n > 0) {
       const int ks = (p.a.D + 15) / 16;
       const uint32_t k = smem_u32(sK), v = smem_u32(sV), q = smem_u32(sQ), g = smem_u32(sG);
-      auto arrived = [&](int u) { return warp_wait(q_full + (u & 1), (u >> 1) & 1); };
+      auto arrived = [&](int u) { return warp_wait(q_full + u % NQ, (u / NQ) & 1); };
       bool ok = warp_wait(kv_full, 0) && arrived(0);
       if (ok) {
         tc_fence_after_sync();
         auto scores = [&](int u) {
           issue([&] {
-            scores_product<DB>(tmem, k, q + (u & 1) * TILE, ks);
+            scores_product<DB>(tmem, k, q + u % NQ * TILE, ks);
             umma_commit(s_full);
           });
         };
         auto slopes = [&](int u) {
           issue([&] {
-            scores_product<DB>(tmem + 128, v, g + (u & 1) * TILE, ks);
+            scores_product<DB>(tmem + 128, v, g + u % NQ * TILE, ks);
             umma_commit(dp_full);
           });
         };
         scores(0);
         slopes(0);
         for (int u = 0; u < n && ok; ++u) {
-          const int s = u & 1;
+          const int s = u % NQ;
           const bool next = u + 1 < n;
           if (next) {  // the softmax warps have the scores in registers
             ok = warp_wait(s_read, u & 1) && arrived(u + 1);
@@ -412,37 +433,35 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
     const bool inside = key < vis.length;
     const int lo = inside ? vis.first(key) : p.a.T, hi = inside ? vis.last(key, p.a.T) : -1;  // queries that see this key
     bool ok = true;
-    for (int u = 0; u < n; ++u) {
-      const int t0 = (i0 + u % per) * AT_M;
-      const bool masked = !vis.whole(t0, t0 + AT_M - 1, k0);
-      const int c_lo = lo - t0 - half * 64, c_hi = hi - t0 - half * 64;
-      const float4 *lse = reinterpret_cast<const float4*>(sStat + (u & 1) * 2 * AT_M + half * 64), *delta = lse + AT_M / 4;
-      ok = warp_wait(q_full + (u & 1), (u >> 1) & 1) && warp_wait(s_full, u & 1);
-      if (!ok) break;
-      tc_fence_after_sync();
+    const uint64_t cc = pack_f2(p.scale2, p.scale2);
+    auto tile = [&](auto some, int u, int c_lo, int c_hi) {  // as for the queries
+      constexpr bool MASKED = decltype(some)::value;
+      const float4 *lse = reinterpret_cast<const float4*>(sStat + u % NQ * 2 * AT_M + half * 64), *delta = lse + AT_M / 4;
       uint32_t x[32], y[32];
       tmem_load(tS, x, y);
       tc_fence_before_sync();
       mbar_arrive(s_read);
       if (u > 0) {  // the product that read the last weights is done
-        ok = warp_wait(p_free, (u - 1) & 1);
-        if (!ok) break;
+        if (!warp_wait(p_free, (u - 1) & 1)) return false;
         tc_fence_after_sync();
       }
-      const uint64_t cc = pack_f2(p.scale2, p.scale2);
       auto weights = [&](uint32_t (&r)[32], int c0) {
+        const uint32_t see = MASKED ? visible_bits(c_lo - c0, c_hi - c0) : 0u;
         uint32_t o[16];
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
           const float4 z = lse[(c0 + i) / 4];
           float a[4];
-          unpack_f2(fma2(pack_f2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), cc, pack_f2(-z.x, -z.y)), a[0], a[1]);
-          unpack_f2(fma2(pack_f2(__uint_as_float(r[i + 2]), __uint_as_float(r[i + 3])), cc, pack_f2(-z.z, -z.w)), a[2], a[3]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            a[e] = ex2(a[e]);
-            if (masked) a[e] = c0 + i + e <= c_hi && c0 + i + e >= c_lo ? a[e] : 0.f;
-            r[i + e] = __float_as_uint(a[e]);
+          for (int k = 0; k < 4; k += 2) {
+            unpack_f2(fma2(pack_f2(__uint_as_float(r[i + k]), __uint_as_float(r[i + k + 1])), cc, k == 0 ? pack_f2(z.x, z.y) : pack_f2(z.z, z.w)), a[k], a[k + 1]);
+            a[k] = ex2(a[k]);
+            a[k + 1] = ex2(a[k + 1]);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if constexpr (MASKED) a[k] = see >> (i + k) & 1 ? a[k] : 0.f;
+            r[i + k] = __float_as_uint(a[k]);
           }
           o[i / 2] = pack_bf16x2(a[0], a[1]);
           o[i / 2 + 1] = pack_bf16x2(a[2], a[3]);
@@ -461,26 +480,27 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
       else fence_proxy_async_smem();
       tc_fence_before_sync();
       mbar_arrive(p_ready);
-      ok = warp_wait(dp_full, u & 1);
-      if (!ok) break;
+      if (!warp_wait(dp_full, u & 1)) return false;
       tc_fence_after_sync();
       auto slopes = [&](uint32_t (&r)[32], int c0) {
+        const uint32_t see = MASKED ? visible_bits(c_lo - c0, c_hi - c0) : 0u;
         uint32_t d[32], o[16];
         tmem_load(tP + c0, d);
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
           const float4 z = delta[(c0 + i) / 4];
-          float a[4];
-          unpack_f2(mul2(add2(pack_f2(__uint_as_float(d[i]), __uint_as_float(d[i + 1])), pack_f2(-z.x, -z.y)),
-                         pack_f2(__uint_as_float(r[i]), __uint_as_float(r[i + 1]))), a[0], a[1]);
-          unpack_f2(mul2(add2(pack_f2(__uint_as_float(d[i + 2]), __uint_as_float(d[i + 3])), pack_f2(-z.z, -z.w)),
-                         pack_f2(__uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]))), a[2], a[3]);
-          if (masked) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) a[e] = c0 + i + e <= c_hi && c0 + i + e >= c_lo ? a[e] : 0.f;
+          for (int k = 0; k < 4; k += 2) {
+            const uint64_t w = mul2(add2(pack_f2(__uint_as_float(d[i + k]), __uint_as_float(d[i + k + 1])), k == 0 ? pack_f2(z.x, z.y) : pack_f2(z.z, z.w)),
+                                    pack_f2(__uint_as_float(r[i + k]), __uint_as_float(r[i + k + 1])));
+            if constexpr (MASKED) {
+              float a, e;
+              unpack_f2(w, a, e);
+              o[(i + k) / 2] = pack_bf16x2(see >> (i + k) & 1 ? a : 0.f, see >> (i + k + 1) & 1 ? e : 0.f);
+            } else {
+              o[(i + k) / 2] = f2_to_bf16x2(w);
+            }
           }
-          o[i / 2] = pack_bf16x2(a[0], a[1]);
-          o[i / 2 + 1] = pack_bf16x2(a[2], a[3]);
         }
         tmem_st_32x32b_x16(tP + c0 / 2, o);
       };
@@ -489,6 +509,17 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
       tmem_st_wait();
       tc_fence_before_sync();
       mbar_arrive(ds_ready);
+      return true;
+    };
+    for (int u = 0, i = 0; u < n; ++u) {
+      const int t0 = (i0 + i) * AT_M;
+      if (++i == per) i = 0;
+      ok = warp_wait(q_full + u % NQ, (u / NQ) & 1) && warp_wait(s_full, u & 1);
+      if (!ok) break;
+      tc_fence_after_sync();
+      if (vis.whole(t0, t0 + AT_M - 1, k0)) ok = tile(std::false_type{}, u, 0, 0);
+      else ok = tile(std::true_type{}, u, lo - t0 - half * 64, hi - t0 - half * 64);
+      if (!ok) break;
     }
     if (ok && n > 0) ok = warp_wait(done, 0);
     tc_fence_after_sync();
@@ -519,8 +550,10 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
 template <int DB>
 void run_bwd(const AttentionBwd& f, cudaStream_t s) {
   const AttentionShape& a = f.a;
-  constexpr int smem = 6 * DB * AT_BOX + 1024, smem_kv = 6 * DB * AT_BOX + (DB == 1 ? 0 : 2 * AT_BOX) + 4 * AT_M * 4 + 14 * 8;
-  static_assert(smem <= 227 * 1024 && smem_kv <= 227 * 1024, "shared memory of a block");
+  constexpr int NQ = key_stages(DB), NK = DB == 1 ? 4 : 3, NV = DB == 1 ? 3 : 2;
+  constexpr int smem = (2 + NK + NV) * DB * AT_BOX + 1024;
+  constexpr int smem_kv = (2 + 2 * NQ) * DB * AT_BOX + (DB == 1 ? 0 : 2 * AT_BOX) + NQ * 2 * AT_M * 4 + (9 + 2 * NQ) * 8;
+  static_assert(smem + 1280 <= 227 * 1024 && smem_kv <= 227 * 1024, "shared memory of a block");
   const CUtensorMap tq = attention_map(f.q, a.D, a.T, a.H, a.B), tg = attention_map(f.dout, a.D, a.T, a.H, a.B),
                     tk = attention_map(f.k, a.D, a.S, a.G, a.B), tv = attention_map(f.v, a.D, a.S, a.G, a.B);
   const BwdParams p{a, f.out, f.dout, f.lse, f.delta, f.dq, f.dk, f.dv, a.scale * LOG2E, f.status};

@@ -48,27 +48,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-// 2^x of two values up to 2^7 (below 2^-126: 2^-126): x = n + r with |r| <= 1/2, a polynomial of degree 4 in r (minimax of the relative
-// error, 2.6e-6, by the exchange algorithm of Remez), times 2^n. What is no number stays so. The units that multiply and add have room where
-// the exponential unit, at 16 results per clock, is what a tile waits for.
-__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
-  float a, b;
-  unpack_f2(x, a, b);
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-126.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-126.f));
-  x = pack_f2(a, b);
-  const float big = 12582912.f;  // 1.5 * 2^23: the sum's last bits are the rounded x
-  const uint64_t t = add2(x, pack_f2(big, big));
-  const uint64_t r = add2(x, mul2(add2(t, pack_f2(-big, -big)), pack_f2(-1.f, -1.f)));
-  uint64_t y = pack_f2(9.570102207362652e-3f, 9.570102207362652e-3f);
-  y = fma2(y, r, pack_f2(5.591785907745361e-2f, 5.591785907745361e-2f));
-  y = fma2(y, r, pack_f2(0.240247443318367f, 0.240247443318367f));
-  y = fma2(y, r, pack_f2(0.6931217908859253f, 0.6931217908859253f));
-  y = fma2(y, r, pack_f2(0.9999992847442627f, 0.9999992847442627f));
-  unpack_f2(t, a, b);
-  return mul2(y, pack_f2(__uint_as_float(__float_as_uint(a) * 0x800000u + 0x3f800000u), __uint_as_float(__float_as_uint(b) * 0x800000u + 0x3f800000u)));
-}
-
 template <int DB, bool PAIR, bool SCALED>
 __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                                                                       const __grid_constant__ CUtensorMap tmV, const FwdParams p) {
@@ -442,7 +421,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __gr
       const bool inside = t < p.a.T;
       const long long row_at = ((long long)b * p.a.H + h) * p.a.T + t;
       const int padded = (p.a.T + AT_M - 1) / AT_M * AT_M;
-      if (p.lse != nullptr && !split && t < padded) p.lse[((long long)b * p.a.H + h) * padded + t] = inside && l != 0.f ? m + log2f(l) : INFINITY;
+      if (p.lse != nullptr && !split && t < padded) p.lse[((long long)b * p.a.H + h) * padded + t] = inside && l != 0.f ? -m - log2f(l) : -INFINITY;
       if (split && inside) {
         const long long rows = (long long)p.a.B * p.a.H * p.a.T;
         float2* ml = reinterpret_cast<float2*>(p.part + p.splits * rows * 64 * DB);
@@ -523,9 +502,9 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const FwdParams p) 
   if (p.lse != nullptr && lane == 0) {
     const int padded = (p.a.T + AT_M - 1) / AT_M * AT_M;
     float* at = p.lse + row / p.a.T * padded;
-    at[t] = l != 0.f ? m + log2f(l) : INFINITY;
+    at[t] = l != 0.f ? -m - log2f(l) : -INFINITY;
     if (t == p.a.T - 1)
-      for (int i = p.a.T; i < padded; ++i) at[i] = INFINITY;
+      for (int i = p.a.T; i < padded; ++i) at[i] = -INFINITY;
   }
 }
 

@@ -49,6 +49,27 @@ __device__ __forceinline__ uint32_t visible_bits(int lo, int hi) {
   return below & ~before;
 }
 
+// 2^x of two values up to 2^7 (below 2^-126: 2^-126): x = n + r with |r| <= 1/2, a polynomial of degree 4 in r (minimax of the relative
+// error, 2.6e-6, by the exchange algorithm of Remez), times 2^n. What is no number stays so. The units that multiply and add have room where
+// the exponential unit, at 16 results per clock, is what a tile waits for.
+__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
+  float a, b;
+  unpack_f2(x, a, b);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-126.f));
+  x = pack_f2(a, b);
+  const float big = 12582912.f;  // 1.5 * 2^23: the sum's last bits are the rounded x
+  const uint64_t t = add2(x, pack_f2(big, big));
+  const uint64_t r = add2(x, mul2(add2(t, pack_f2(-big, -big)), pack_f2(-1.f, -1.f)));
+  uint64_t y = pack_f2(9.570102207362652e-3f, 9.570102207362652e-3f);
+  y = fma2(y, r, pack_f2(5.591785907745361e-2f, 5.591785907745361e-2f));
+  y = fma2(y, r, pack_f2(0.240247443318367f, 0.240247443318367f));
+  y = fma2(y, r, pack_f2(0.6931217908859253f, 0.6931217908859253f));
+  y = fma2(y, r, pack_f2(0.9999992847442627f, 0.9999992847442627f));
+  unpack_f2(t, a, b);
+  return mul2(y, pack_f2(__uint_as_float(__float_as_uint(a) * 0x800000u + 0x3f800000u), __uint_as_float(__float_as_uint(b) * 0x800000u + 0x3f800000u)));
+}
+
 // 64-wide boxes of 128 rows of one head: coordinates (column, row, head, batch); what is outside reads as zero
 inline CUtensorMap attention_map(const AttentionView& v, int d, int rows, int heads, int batch, uint32_t box_rows = AT_M) {
   return make_tmap_4d_bf16(v.p, {(uint64_t)d, (uint64_t)rows, (uint64_t)heads, (uint64_t)batch},

@@ -8,9 +8,10 @@
 // Both: warp 0 TMA producer, warp 1 tcgen05.mma, warps 4-11 softmax; a thread has one row and half of its 128 columns, and keeps
 // the fp32 probabilities in registers between S and dP. P and dS are rounded to bf16 for the products (2^-8 of each term at
 // most, which averages out over the sums); dS is formed from the unrounded P.
-// The next tile's scores are formed as soon as these are in registers. dQ has two sets of columns for dP (dS over it), so that a
-// tile's dP need not wait for the product with the last one's dS. For dK and dV, P has columns of its own with heads of up to 64, and
-// goes through shared memory with wider ones.
+// The next tile's scores are formed as soon as these are in registers, where they have the room. dQ has two sets of columns for dP (dS over it), so that a
+// tile's dP need not wait for the product with the last one's dS. For dK and dV, P has columns of its own with heads of up to 64;
+// with wider ones it lies over S, and the next scores come behind the product with P (P through shared memory, to have them earlier,
+// left no room for a third stage of query tiles: 2911 clocks a tile instead of 2500, waiting for these).
 #include <type_traits>
 
 #include "../common/per_device.h"
@@ -30,15 +31,6 @@ struct BwdParams {
   float scale2;
   int* status;
 };
-
-// D (+)= A B, A: 128 x 128 bf16 in two boxes of 64 columns, B: rows of a [128][64 DB] tile
-template <int DB>
-__device__ __forceinline__ void square_product(uint32_t d, uint32_t a, uint32_t b, bool add) {
-  constexpr uint32_t idesc = make_idesc(AT_M, 64 * DB, 1, 1, 0, 1);
-  const uint64_t da = make_smem_desc(a, 16, 1024), db = make_smem_desc(b, AT_BOX, 1024);
-#pragma unroll
-  for (int k = 0; k < 8; ++k) umma_bf16(d, da + (((k >> 2) * AT_BOX + (k & 3) * 32) >> 4), db + ((k * 2048) >> 4), idesc, k > 0 || add);
-}
 
 // TMEM column of step k of a 128 x 128 bf16 operand: two halves of 64 values, each in the first 32 columns of its 64
 __device__ __forceinline__ int half_column(int k) { return (k >> 2) * 64 + (k & 3) * 8; }
@@ -299,11 +291,12 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
                                                                       const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                                                                       const BwdParams p) {
   constexpr int TILE = DB * AT_BOX, STATS = 2 * AT_M * 4, NQ = key_stages(DB);  // lse and delta of a query tile
-  // TMEM columns: S 0-127, dP (dS over it) 128-255, P where it fits (else it is in shared memory), and the sums
-  constexpr uint32_t P_AT = 256, V_AT = DB == 1 ? 384 : 256, K_AT = DB == 1 ? 448 : 384;
+  // TMEM columns: S 0-127, dP (dS over it) 128-255, P where it fits (APART, else over S), and the sums
+  constexpr bool APART = DB == 1;
+  constexpr uint32_t P_AT = 256, V_AT = APART ? 384 : 256, K_AT = APART ? 448 : 384;
   extern __shared__ __align__(1024) uint8_t smem[];  // no other shared memory: it starts on a tile's boundary, which is looked at below
-  uint8_t *sK = smem, *sV = sK + TILE, *sQ = sV + TILE, *sG = sQ + NQ * TILE, *sP = sG + NQ * TILE;
-  float* sStat = reinterpret_cast<float*>(sP + (DB == 1 ? 0 : 2 * AT_BOX));
+  uint8_t *sK = smem, *sV = sK + TILE, *sQ = sV + TILE, *sG = sQ + NQ * TILE;
+  float* sStat = reinterpret_cast<float*>(sG + NQ * TILE);
   uint64_t* bars = reinterpret_cast<uint64_t*>(sStat + NQ * 2 * AT_M);
   uint64_t *kv_full = bars, *s_full = bars + 1, *p_ready = bars + 2, *dp_full = bars + 3, *ds_ready = bars + 4, *done = bars + 5, *s_read = bars + 6,
            *p_free = bars + 7, *q_full = bars + 8, *q_empty = q_full + NQ;
@@ -399,7 +392,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
         for (int u = 0; u < n && ok; ++u) {
           const int s = u % NQ;
           const bool next = u + 1 < n;
-          if (next) {  // the softmax warps have the scores in registers
+          if (APART && next) {  // the softmax warps have the scores in registers
             ok = warp_wait(s_read, u & 1) && arrived(u + 1);
             if (!ok) break;
             tc_fence_after_sync();
@@ -409,10 +402,15 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
           if (!ok) break;
           tc_fence_after_sync();
           issue([&] {
-            if constexpr (DB == 1) rows_product<DB, 0, 8>(tmem + V_AT, tmem + P_AT, g + s * TILE, u > 0, [](int k) { return k * 8; });
-            else square_product<DB>(tmem + V_AT, smem_u32(sP), g + s * TILE, u > 0);
-            umma_commit(p_free);
+            if constexpr (APART) rows_product<DB, 0, 8>(tmem + V_AT, tmem + P_AT, g + s * TILE, u > 0, [](int k) { return k * 8; });
+            else rows_product<DB, 0, 8>(tmem + V_AT, tmem, g + s * TILE, u > 0, half_column);
+            if (APART) umma_commit(p_free);
           });
+          if (!APART && next) {  // behind the product that reads P from the same columns
+            ok = arrived(u + 1);
+            if (!ok) break;
+            scores(u + 1);
+          }
           ok = warp_wait(ds_ready, u & 1);
           if (!ok) break;
           tc_fence_after_sync();
@@ -440,8 +438,8 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
       uint32_t x[32], y[32];
       tmem_load(tS, x, y);
       tc_fence_before_sync();
-      mbar_arrive(s_read);
-      if (u > 0) {  // the product that read the last weights is done
+      if (APART) mbar_arrive(s_read);
+      if (APART && u > 0) {  // the product that read the last weights is done
         if (!warp_wait(p_free, (u - 1) & 1)) return false;
         tc_fence_after_sync();
       }
@@ -466,18 +464,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
           o[i / 2] = pack_bf16x2(a[0], a[1]);
           o[i / 2 + 1] = pack_bf16x2(a[2], a[3]);
         }
-        if constexpr (DB == 1) {
-          tmem_st_32x32b_x16(tmem + lane_base + P_AT + half * 32 + c0 / 2, o);
-        } else {  // 16-byte pieces of the row, as TMA would have swizzled them
-          uint4* at = reinterpret_cast<uint4*>(sP + half * AT_BOX + row * 128);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) at[(c0 / 8 + i) ^ (row & 7)] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-        }
+        tmem_st_32x32b_x16((APART ? tmem + lane_base + P_AT + half * 32 : tS) + c0 / 2, o);
       };
       weights(x, 0);
       weights(y, 32);
-      if constexpr (DB == 1) tmem_st_wait();
-      else fence_proxy_async_smem();
+      tmem_st_wait();
       tc_fence_before_sync();
       mbar_arrive(p_ready);
       if (!warp_wait(dp_full, u & 1)) return false;
@@ -552,7 +543,7 @@ void run_bwd(const AttentionBwd& f, cudaStream_t s) {
   const AttentionShape& a = f.a;
   constexpr int NQ = key_stages(DB), NK = DB == 1 ? 4 : 3, NV = DB == 1 ? 3 : 2;
   constexpr int smem = (2 + NK + NV) * DB * AT_BOX + 1024;
-  constexpr int smem_kv = (2 + 2 * NQ) * DB * AT_BOX + (DB == 1 ? 0 : 2 * AT_BOX) + NQ * 2 * AT_M * 4 + (9 + 2 * NQ) * 8;
+  constexpr int smem_kv = (2 + 2 * NQ) * DB * AT_BOX + NQ * 2 * AT_M * 4 + (9 + 2 * NQ) * 8;
   static_assert(smem + 1280 <= 227 * 1024 && smem_kv <= 227 * 1024, "shared memory of a block");
   const CUtensorMap tq = attention_map(f.q, a.D, a.T, a.H, a.B), tg = attention_map(f.dout, a.D, a.T, a.H, a.B),
                     tk = attention_map(f.k, a.D, a.S, a.G, a.B), tv = attention_map(f.v, a.D, a.S, a.G, a.B);

@@ -11,6 +11,9 @@ namespace {
 using torch::Tensor;
 using OptTensor = c10::optional<Tensor>;
 
+// Queries of a key/value head from which on a call on the 8-bit cache counts as a portion of a prompt: its codes are laid out once for
+// the tensor cores, instead of being read again for every 16 queries.
+constexpr int64_t PORTION = 64;
 constexpr int64_t MOST_ROWS = 65535ll * 128;  // queries or keys of a sequence: tiles along a grid's second dimension
 
 cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
@@ -96,24 +99,20 @@ void append_rows(const tb::Kv8Cache& c, const Tensor& k, const Tensor& v, const 
   if (k.numel() > 0) tb::launch_kv8_append(c, kv, vv, (int)k.size(1), (int)k.size(3), pos, cur_stream());
 }
 
-// -> (out, lse). lse is empty where it is not asked for.
-std::vector<Tensor> attention_fwd(const Tensor& q, const Tensor& k, const Tensor& v, double scale, bool causal, int64_t window, const OptTensor& lengths,
-                                  const OptTensor& starts, int64_t start, bool want_lse, const Tensor& status) {
-  tb::AttentionFwd f{};
-  f.a = shape_of(q, k, v, scale, causal, window, lengths, starts, start);
-  c10::cuda::CUDAGuard guard(q.device());
-  Tensor hq, hk, hv;
+// Forward pass of f.a; -> out, and lse where it is asked for
+Tensor attend(tb::AttentionFwd& f, const Tensor& q, const Tensor& k, const Tensor& v, bool want_lse, const Tensor& status, Tensor& lse) {
+  Tensor hq, hk, hv, part;
   f.q = view_of(q, q, "queries", hq);
   f.k = view_of(k, q, "keys", hk);
   f.v = view_of(v, q, "values", hv);
-  Tensor out = torch::empty(q.sizes(), q.options()), lse, part;
+  Tensor out = torch::empty(q.sizes(), q.options());
   const auto f32 = q.options().dtype(at::kFloat);
   if (want_lse) lse = torch::empty({f.a.B, f.a.H, tb::attention_rows(f.a.T)}, f32);
-  if (out.numel() == 0) return {out, lse};
+  if (out.numel() == 0) return out;
   if (f.a.S == 0) {
     out.zero_();
     if (want_lse) lse.fill_(-INFINITY);
-    return {out, lse};
+    return out;
   }
   const long long bytes = tb::attention_fwd_scratch(f.a);
   if (bytes > 0) part = torch::empty({bytes / 4}, f32);
@@ -122,6 +121,16 @@ std::vector<Tensor> attention_fwd(const Tensor& q, const Tensor& k, const Tensor
   f.part = bytes > 0 ? part.data_ptr<float>() : nullptr;
   f.status = status_of(status);
   tb::launch_attention_fwd(f, cur_stream());
+  return out;
+}
+
+// -> (out, lse). lse is empty where it is not asked for.
+std::vector<Tensor> attention_fwd(const Tensor& q, const Tensor& k, const Tensor& v, double scale, bool causal, int64_t window, const OptTensor& lengths,
+                                  const OptTensor& starts, int64_t start, bool want_lse, const Tensor& status) {
+  tb::AttentionFwd f{};
+  f.a = shape_of(q, k, v, scale, causal, window, lengths, starts, start);
+  c10::cuda::CUDAGuard guard(q.device());
+  Tensor lse, out = attend(f, q, k, v, want_lse, status, lse);
   return {out, lse};
 }
 
@@ -174,9 +183,9 @@ std::vector<Tensor> kv8_expand(const Tensor& k8, const Tensor& v8, const Tensor&
   return {k, v};
 }
 
-// Appends k and v (where given), then attends. `most`: tokens a sequence may hold then; a bound that the work is split by.
+// Appends k and v (where given), then attends. `most`: a bound on the tokens a sequence holds then.
 Tensor kv8_attention(const Tensor& k8, const Tensor& v8, const Tensor& ks, const Tensor& vs, const Tensor& kt, const Tensor& vt, const Tensor& q,
-                     const OptTensor& k, const OptTensor& v, int64_t host, const OptTensor& dev, double scale, int64_t most) {
+                     const OptTensor& k, const OptTensor& v, int64_t host, const OptTensor& dev, double scale, int64_t most, const Tensor& status) {
   const tb::Kv8Cache c = cache_of(k8, v8, ks, vs, kt, vt, q);
   TORCH_CHECK(q.dim() == 4 && q.size(2) % c.G == 0, "kv8: query heads must be a multiple of the cache's");
   check_rows(c, q, q.size(2), "queries");
@@ -192,18 +201,46 @@ Tensor kv8_attention(const Tensor& k8, const Tensor& v8, const Tensor& ks, const
   a.pos = pos_of(host, dev, c.B, q);
   a.scale = (float)scale;
   a.most = (int)std::max<int64_t>(0, std::min<int64_t>(most, c.C));
-  Tensor out = torch::empty(q.sizes(), q.options());
+  Tensor out;
   if (has(k)) {
     TORCH_CHECK(has(v) && k->dim() == 4 && k->size(1) == q.size(1) && k->size(3) == q.size(3) && k->get_device() == q.get_device(),
                 "kv8: new keys and values come with the queries' tokens");
     append_rows(c, *k, *v, a.pos);
+    a.appended = k->numel() > 0;
   }
-  if (out.numel() == 0) return out;
-  a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
-  const long long bytes = tb::kv8_attention_scratch(a);
-  if (bytes > 0) part = torch::empty({bytes / 4}, q.options().dtype(at::kFloat));
-  a.part = bytes > 0 ? part.data_ptr<float>() : nullptr;
-  tb::launch_kv8_attention(a, cur_stream());
+  if (q.numel() == 0) return torch::empty(q.sizes(), q.options());
+  if (a.T * (a.H / c.G) < PORTION) {
+    out = torch::empty(q.sizes(), q.options());
+    a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
+    const long long bytes = tb::kv8_attention_scratch(a);
+    if (bytes > 0) part = torch::empty({bytes / 4}, q.options().dtype(at::kFloat));
+    a.part = bytes > 0 ? part.data_ptr<float>() : nullptr;
+    tb::launch_kv8_attention(a, cur_stream());
+    return out;
+  }
+  // a portion of a prompt: codes as bf16 numbers once, then attention on the tensor cores, which applies the blocks' scales
+  const int64_t rows = a.most, blocks = (rows + tb::KV8_BLOCK - 1) / tb::KV8_BLOCK;
+  if (rows == 0) return torch::zeros(q.sizes(), q.options());
+  Tensor codes = torch::empty({2, c.B, c.G, rows, a.D}, q.options()), scales = torch::empty({2, c.B, c.G, blocks}, q.options().dtype(at::kFloat));
+  tb::Kv8Codes to{reinterpret_cast<__nv_bfloat16*>(codes.data_ptr()), nullptr, scales.data_ptr<float>(), nullptr, nullptr, nullptr};
+  to.v = to.k + codes.numel() / 2;
+  to.v_scales = to.k_scales + scales.numel() / 2;
+  Tensor where;
+  if (a.pos.dev != nullptr) {
+    where = torch::empty({2, c.B}, q.options().dtype(at::kLong));
+    to.starts = reinterpret_cast<long long*>(where.data_ptr<int64_t>());
+    to.ends = to.starts + c.B;
+  }
+  tb::launch_kv8_codes(c, to, (int)rows, a.D, a.pos, a.T, cur_stream());
+  const Tensor kk = codes.select(0, 0).transpose(1, 2), vv = codes.select(0, 1).transpose(1, 2);
+  tb::AttentionFwd f{};
+  f.a = shape_of(q, kk, vv, scale, true, 0, c10::nullopt, c10::nullopt, a.pos.host);
+  if (a.pos.dev != nullptr) f.a.starts = to.starts, f.a.lengths = to.ends;
+  f.k_scales = to.k_scales;
+  f.v_scales = to.v_scales;
+  f.blocks = (int)blocks;
+  out = attend(f, q, kk, vv, false, status, part);
+  if (a.pos.dev != nullptr) tb::launch_kv8_outside(c, reinterpret_cast<__nv_bfloat16*>(out.data_ptr()), a.T, a.H * a.D, a.pos, cur_stream());
   return out;
 }
 

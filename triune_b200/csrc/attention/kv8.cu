@@ -2,6 +2,7 @@
 // of values; rows are read and written in 16-byte pieces (codes in 8-byte pieces).
 #include <cuda_fp8.h>
 
+#include "../common/dependent_launch.cuh"
 #include "kv8.cuh"
 
 namespace tb {
@@ -28,6 +29,7 @@ template <int P, bool E4M3>
 __global__ void __launch_bounds__(256) kv8_append_kernel(const AppendParams p) {
   constexpr int ACROSS = P / 8, PIECES = KV8_BLOCK * ACROSS / 256;
   __shared__ uint32_t most[8];
+  allow_dependents();  // attention that reads other blocks may start
   long long at = blockIdx.x;
   const int i = at % p.blocks;
   at /= p.blocks;
@@ -90,12 +92,13 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const AppendParams p) {
 
 struct ExpandParams {
   Kv8Cache c;
-  __nv_bfloat16 *k, *v;
+  Kv8Codes to;  // scales: null where values are asked for
   int rows, D, blocks;
-  Kv8Pos length;
+  Kv8Pos pos;
+  int T;  // the sequences' length is their position plus T; idle ones have none
 };
 
-template <int P, bool E4M3>
+template <int P, bool E4M3, bool CODES>
 __global__ void __launch_bounds__(256) kv8_expand_kernel(const ExpandParams p) {
   constexpr int ACROSS = P / 8, PIECES = KV8_BLOCK * ACROSS / 256;
   long long at = blockIdx.x;
@@ -103,17 +106,27 @@ __global__ void __launch_bounds__(256) kv8_expand_kernel(const ExpandParams p) {
   at /= p.blocks;
   const int side = at & 1;
   at >>= 1;  // head
-  const long long given = pos_at(p.length, at / p.c.G);
-  const int n = (int)max(0ll, min(given, (long long)p.c.C)), base = m * KV8_BLOCK;
+  const long long start = pos_at(p.pos, at / p.c.G), given = start < 0 ? 0 : start + p.T;
+  const int n = (int)min(given, (long long)p.c.C), base = m * KV8_BLOCK;
   const bool full = base + KV8_BLOCK <= n;
-  __nv_bfloat16* out = (side ? p.v : p.k) + (at * p.rows + base) * p.D;
+  __nv_bfloat16* out = (side ? p.to.v : p.to.k) + (at * p.rows + base) * p.D;
   const uint2* codes = reinterpret_cast<const uint2*>((side ? p.c.v8 : p.c.k8) + (at * p.c.C + base) * P);
   const uint4* ring = reinterpret_cast<const uint4*>((side ? p.c.vt : p.c.kt) + (at * KV8_RING + (m & 1) * KV8_BLOCK) * P);
-  const float s = full ? (side ? p.c.vs : p.c.ks)[at * (p.c.C / KV8_BLOCK) + m] : 0.f;
+  float s = full ? (side ? p.c.vs : p.c.ks)[at * (p.c.C / KV8_BLOCK) + m] : 0.f;
+  if constexpr (CODES) {
+    if (threadIdx.x == 0) {
+      (side ? p.to.v_scales : p.to.k_scales)[at * p.blocks + m] = full ? s : base < n ? 1.f : 0.f;
+      if (p.to.ends != nullptr && m == 0 && side == 0 && at % p.c.G == 0) {
+        p.to.starts[at / p.c.G] = start;
+        p.to.ends[at / p.c.G] = n;
+      }
+    }
+    s = 1.f;
+  }
 #pragma unroll
   for (int e = 0; e < PIECES; ++e) {
     const int i = threadIdx.x + 256 * e, row = i / ACROSS, piece = i % ACROSS;
-    if (base + row >= p.rows || piece * 8 >= p.D) continue;
+    if (base + row >= p.rows || piece * 8 >= p.D || (CODES && base + row >= n)) continue;
     uint4 z = make_uint4(0, 0, 0, 0);
     if (full) {
       const uint2 c = codes[i];
@@ -137,6 +150,20 @@ __global__ void __launch_bounds__(256) kv8_expand_kernel(const ExpandParams p) {
   }
 }
 
+__global__ void __launch_bounds__(128) kv8_outside_kernel(__nv_bfloat16* out, int T, int width, int C, const Kv8Pos pos) {
+  const long long row = blockIdx.x, start = pos_at(pos, row / T);
+  if (start < 0 || start + row % T < C) return;
+  for (int i = threadIdx.x; i < width; i += 128) out[row * width + i] = __float2bfloat16(__int_as_float(0x7fc00000));
+}
+
+template <bool CODES>
+void expand(const ExpandParams& p, cudaStream_t s) {
+  const unsigned grid = (unsigned)((long long)p.blocks * 2 * p.c.B * p.c.G);
+  if (p.c.P == 64) (p.c.e4m3 ? kv8_expand_kernel<64, true, CODES> : kv8_expand_kernel<64, false, CODES>)<<<grid, 256, 0, s>>>(p);
+  else (p.c.e4m3 ? kv8_expand_kernel<128, true, CODES> : kv8_expand_kernel<128, false, CODES>)<<<grid, 256, 0, s>>>(p);
+  attention_check_launch("kv8_expand");
+}
+
 }  // namespace
 
 void launch_kv8_append(const Kv8Cache& c, const AttentionView& k, const AttentionView& v, int T, int D, const Kv8Pos& pos, cudaStream_t s) {
@@ -149,12 +176,16 @@ void launch_kv8_append(const Kv8Cache& c, const AttentionView& k, const Attentio
 }
 
 void launch_kv8_expand(const Kv8Cache& c, __nv_bfloat16* k, __nv_bfloat16* v, int rows, int D, const Kv8Pos& length, cudaStream_t s) {
-  const int blocks = (rows + KV8_BLOCK - 1) / KV8_BLOCK;
-  const ExpandParams p{c, k, v, rows, D, blocks, length};
-  const unsigned grid = (unsigned)((long long)blocks * 2 * c.B * c.G);
-  if (c.P == 64) (c.e4m3 ? kv8_expand_kernel<64, true> : kv8_expand_kernel<64, false>)<<<grid, 256, 0, s>>>(p);
-  else (c.e4m3 ? kv8_expand_kernel<128, true> : kv8_expand_kernel<128, false>)<<<grid, 256, 0, s>>>(p);
-  attention_check_launch("kv8_expand");
+  expand<false>(ExpandParams{c, Kv8Codes{k, v, nullptr, nullptr, nullptr, nullptr}, rows, D, (rows + KV8_BLOCK - 1) / KV8_BLOCK, length, 0}, s);
+}
+
+void launch_kv8_codes(const Kv8Cache& c, const Kv8Codes& to, int rows, int D, const Kv8Pos& pos, int T, cudaStream_t s) {
+  expand<true>(ExpandParams{c, to, rows, D, (rows + KV8_BLOCK - 1) / KV8_BLOCK, pos, T}, s);
+}
+
+void launch_kv8_outside(const Kv8Cache& c, __nv_bfloat16* out, int T, int width, const Kv8Pos& pos, cudaStream_t s) {
+  kv8_outside_kernel<<<(unsigned)((long long)c.B * T), 128, 0, s>>>(out, T, width, c.C, pos);
+  attention_check_launch("kv8_outside");
 }
 
 }  // namespace tb

@@ -37,6 +37,18 @@ void launch_kv8_append(const Kv8Cache& c, const AttentionView& k, const Attentio
 // k, v [B, G, rows, D] contiguous: the values of the first `length` positions, zero from there on
 void launch_kv8_expand(const Kv8Cache& c, __nv_bfloat16* k, __nv_bfloat16* v, int rows, int D, const Kv8Pos& length, cudaStream_t s);
 
+// For tensor-core attention over the cache: k, v [B, G, rows, D] hold codes (and the open block's tokens) as bf16 numbers, which they
+// are exactly, k_scales and v_scales [B, G, ceil(rows / 64)] what blocks are multiplied by (1 for the open one, 0 past the end); rows
+// past a sequence's end are left as they are. starts and ends [B] (or null): positions, and those plus T (0 for idle sequences).
+struct Kv8Codes {
+  __nv_bfloat16 *k, *v;
+  float *k_scales, *v_scales;
+  long long *starts, *ends;
+};
+void launch_kv8_codes(const Kv8Cache& c, const Kv8Codes& to, int rows, int D, const Kv8Pos& pos, int T, cudaStream_t s);
+// out [B, T, width]: NaN at the positions past the capacity
+void launch_kv8_outside(const Kv8Cache& c, __nv_bfloat16* out, int T, int width, const Kv8Pos& pos, cudaStream_t s);
+
 struct Kv8Attention {
   Kv8Cache c;
   AttentionView q;     // [B, T, H, D]
@@ -46,6 +58,7 @@ struct Kv8Attention {
   Kv8Pos pos;
   float scale;
   int most;            // tokens that a sequence may hold after these: what the work is split by
+  bool appended;       // launch_kv8_append of the same tokens comes right before on the stream
 };
 long long kv8_attention_scratch(const Kv8Attention& a);
 void launch_kv8_attention(const Kv8Attention& a, cudaStream_t s);

@@ -19,6 +19,7 @@
 
 #include <algorithm>
 
+#include "../common/dependent_launch.cuh"
 #include "../common/per_device.h"
 #include "../common/ptx.cuh"
 #include "kv8.cuh"
@@ -27,6 +28,8 @@ namespace tb {
 namespace {
 
 constexpr int DW = 4, UNIT = 32;  // warps of a CTA, keys of a unit
+constexpr int MOST_SPLITS = 512;
+constexpr int step_smem(int P, int NT) { return DW * NT * 8 * (P + 4) * 4; }
 
 struct StepParams {
   Kv8Attention a;
@@ -195,7 +198,21 @@ __global__ void __launch_bounds__(DW * 32) kv8_attention_kernel(const StepParams
       }
     ks = kscale[u * UNIT / KV8_BLOCK];
   };
-  if (u < u1) load_keys(u);
+  // Blocks that were full before this call's tokens came may be read while these are still being appended; the ring, and the block
+  // that they fill, only after. What comes behind (the join) may take its place as soon as blocks leave.
+  allow_dependents();
+  const int settled = p.a.appended ? pos / KV8_BLOCK * (KV8_BLOCK / UNIT) : units;
+  bool waited = !p.a.appended;
+  auto wait_for = [&](int u) {
+    if (!waited && u >= settled) {
+      wait_predecessors();
+      waited = true;
+    }
+  };
+  if (u < u1) {
+    wait_for(u);
+    load_keys(u);
+  }
   for (; u < u1; u += DW) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -218,7 +235,10 @@ __global__ void __launch_bounds__(DW * 32) kv8_attention_kernel(const StepParams
       }
     }
     const float here = ks;
-    if (u + DW < u1) load_keys(u + DW);
+    if (u + DW < u1) {
+      wait_for(u + DW);
+      load_keys(u + DW);
+    }
     const int key = u * UNIT + g;
     const bool masked = u * UNIT + UNIT - 1 > pos;
 #pragma unroll
@@ -283,6 +303,7 @@ __global__ void __launch_bounds__(DW * 32) kv8_attention_kernel(const StepParams
   // ---- the open block: a tile of 16 keys per warp, by the CTA of the last part
   const int k0 = full + 16 * warp;
   if (split == p.splits - 1 && k0 < total) {
+    wait_for(units);
     const __nv_bfloat16 *kr = c.kt + (head * KV8_RING + (k0 & (KV8_RING - 1))) * P, *vr = c.vt + (head * KV8_RING + (k0 & (KV8_RING - 1))) * P;
     float s[1][NT][4];
 #pragma unroll
@@ -392,6 +413,7 @@ __global__ void __launch_bounds__(DW * 32) kv8_attention_kernel(const StepParams
         *reinterpret_cast<float4*>(to + 2 * i) = make_float4(o[n][i][k], o[n][i][k + 2], o[n][i + 1][k], o[n][i + 1][k + 2]);
     }
   __syncthreads();
+  if (split == p.splits - 1 && !waited) wait_predecessors();  // this grid ends after the one before it, whatever it had to read
   const long long all = (long long)c.B * c.G * p.rows;
   for (int i = threadIdx.x; i < NT * 8 * (P / 4); i += DW * 32) {
     const int q = i / (P / 4), d = i % (P / 4) * 4, r = row0 + q;
@@ -426,38 +448,78 @@ __global__ void __launch_bounds__(DW * 32) kv8_attention_kernel(const StepParams
   }
 }
 
-// A warp per query: joins the parts of its keys.
+// Joins the parts of a query's keys: four warps take every fourth part each, a lane P / 32 neighbouring columns.
 template <int P>
 __global__ void __launch_bounds__(128) kv8_join_kernel(const StepParams p) {
+  constexpr int COLS = P / 32;
+  __shared__ float weight[MOST_SPLITS], sum[4], acc[4][P];
   const Kv8Cache& c = p.a.c;
-  const long long all = (long long)c.B * c.G * p.rows, row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (row >= all) return;
-  const int lane = threadIdx.x & 31, r = row % p.rows, kvh = row / p.rows % c.G, b = row / p.rows / c.G;
+  const long long all = (long long)c.B * c.G * p.rows, row = blockIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = row % p.rows, kvh = row / p.rows % c.G, b = row / p.rows / c.G;
+  wait_predecessors();
   const float2* st = reinterpret_cast<const float2*>(p.a.part + p.splits * all * P);
-  // each lane looks after some of the parts' statistics
-  float mx = -INFINITY;
+  float mx = -INFINITY, l = 0.f;
   for (int s = lane; s < p.splits; s += 32) mx = fmaxf(mx, st[s * all + row].x);
 #pragma unroll
   for (int i = 16; i > 0; i >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, i));
-  float sum = 0.f, acc[P / 32] = {};
-  for (int s = 0; s < p.splits; ++s) {
+  for (int s = threadIdx.x; s < p.splits; s += 128) {
     const float2 x = st[s * all + row];
     const float f = x.x == -INFINITY ? (x.y == x.y ? 0.f : 1.f) : ex2(x.x - mx);
-    if (f == 0.f && x.y == x.y) continue;
-    sum += x.y * f;
-#pragma unroll
-    for (int i = 0; i < P / 32; ++i) acc[i] += p.a.part[(s * all + row) * P + (P / 32) * lane + i] * f;
+    weight[s] = f;
+    l += f == 0.f && x.y == x.y ? 0.f : x.y * f;
   }
+#pragma unroll
+  for (int i = 16; i > 0; i >>= 1) l += __shfl_xor_sync(0xffffffffu, l, i);
+  if (lane == 0) sum[warp] = l;
+  __syncthreads();
+  float x[COLS] = {};
+#pragma unroll 4
+  for (int s = warp; s < p.splits; s += 4) {
+    const float f = weight[s];
+    const float* part = p.a.part + (s * all + row) * P + COLS * lane;
+#pragma unroll
+    for (int i = 0; i < COLS; ++i) x[i] += f == 0.f ? 0.f : part[i] * f;  // a part without visible keys, or with none that counts
+  }
+#pragma unroll
+  for (int i = 0; i < COLS; ++i) acc[warp][COLS * lane + i] = x[i];
+  __syncthreads();
+  const int d = threadIdx.x;
+  if (d >= p.a.D) return;
+  const float total = sum[0] + sum[1] + sum[2] + sum[3];
   const long long start = p.a.pos.dev != nullptr ? p.a.pos.dev[(long long)b * p.a.pos.step] : p.a.pos.host;
   const int tok = r / p.rep, h = kvh * p.rep + r % p.rep;
-  float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const bool nan = start >= 0 && start + tok >= c.C;
-#pragma unroll
-  for (int i = 0; i < P / 32; ++i) {
-    const int d = (P / 32) * lane + i;
-    if (d < p.a.D)
-      p.a.out[(((long long)b * p.a.T + tok) * p.a.H + h) * p.a.D + d] = __float2bfloat16(nan ? __int_as_float(0x7fc00000) : acc[i] * inv);
+  float y = total == 0.f ? 0.f : (acc[0][d] + acc[1][d] + acc[2][d] + acc[3][d]) / total;
+  if (start >= 0 && start + tok >= c.C) y = __int_as_float(0x7fc00000);
+  p.a.out[(((long long)b * p.a.T + tok) * p.a.H + h) * p.a.D + d] = __float2bfloat16(y);
+}
+
+template <int P, bool E4M3, int NT>
+int resident_blocks() {  // of a GPU, by registers and shared memory
+  static int count[PerDeviceOnce::kMaxDevices] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= PerDeviceOnce::kMaxDevices) return 148;
+  if (count[dev] == 0) {
+    int sms = 0, per = 0;
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kv8_attention_kernel<P, E4M3, NT>, DW * 32, step_smem(P, NT));
+    count[dev] = std::max(1, sms * per);
   }
+  return count[dev];
+}
+
+// How many blocks share a head's keys: of the largest numbers that fit in one to four rounds of the resident blocks the one with the
+// least time, in units of keys per warp, where a block's start and end count as 6.
+int splits_for(long long ctas, int units, int resident) {
+  const long long most = std::min(MOST_SPLITS, std::max(1, units / (2 * DW)));
+  long long best = 1, least = (ctas + resident - 1) / resident * ((units + DW - 1) / DW + 6);
+  for (int rounds = 1; rounds <= 4; ++rounds) {
+    const long long s = std::min(most, rounds * (long long)resident / ctas);
+    if (s < 1) continue;
+    const long long t = rounds * ((units + s * DW - 1) / (s * DW) + 6);
+    if (t < least) least = t, best = s;
+  }
+  return (int)best;
 }
 
 StepParams plan(const Kv8Attention& a) {
@@ -467,23 +529,35 @@ StepParams plan(const Kv8Attention& a) {
   const int nt = p.rows > 8 ? 2 : 1;
   p.tiles = (p.rows + 8 * nt - 1) / (8 * nt);
   p.scale2 = a.scale * 1.4426950408889634f;
-  const long long ctas = (long long)a.c.B * a.c.G * p.tiles, want = 148 * 3 * 2;
-  const int most = std::max(1, std::min(a.most, a.c.C) / (UNIT * DW * 2));  // two units a warp at least
-  p.splits = (int)std::max<long long>(1, std::min<long long>((want + ctas - 1) / ctas, most));
+  const int resident = a.c.P == 64 ? (a.c.e4m3 ? (nt == 1 ? resident_blocks<64, true, 1>() : resident_blocks<64, true, 2>())
+                                               : (nt == 1 ? resident_blocks<64, false, 1>() : resident_blocks<64, false, 2>()))
+                                   : (a.c.e4m3 ? (nt == 1 ? resident_blocks<128, true, 1>() : resident_blocks<128, true, 2>())
+                                               : (nt == 1 ? resident_blocks<128, false, 1>() : resident_blocks<128, false, 2>()));
+  p.splits = splits_for((long long)a.c.B * a.c.G * p.tiles, std::min(a.most, a.c.C) / UNIT, resident);
   return p;
+}
+
+template <typename... K, typename... A>
+void launch(void (*kernel)(K...), unsigned grid, int threads, int smem, bool dependent, cudaStream_t s, const char* what, A&&... args) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = dependent ? 1 : 0;
+  cudaLaunchKernelEx(&cfg, kernel, static_cast<K>(std::forward<A>(args))...);
+  attention_check_launch(what);
 }
 
 template <int P, bool E4M3, int NT>
 void run(const StepParams& p, cudaStream_t s) {
-  constexpr int smem = DW * NT * 8 * (P + 4) * 4;
   const unsigned grid = (unsigned)((long long)p.splits * p.tiles * p.a.c.G * p.a.c.B);
-  kv8_attention_kernel<P, E4M3, NT><<<grid, DW * 32, smem, s>>>(p);
-  attention_check_launch("kv8_attention");
-  if (p.splits > 1) {
-    const long long all = (long long)p.a.c.B * p.a.c.G * p.rows;
-    kv8_join_kernel<P><<<(unsigned)((all + 3) / 4), 128, 0, s>>>(p);
-    attention_check_launch("kv8_join");
-  }
+  launch(kv8_attention_kernel<P, E4M3, NT>, grid, DW * 32, step_smem(P, NT), p.a.appended, s, "kv8_attention", p);
+  if (p.splits > 1) launch(kv8_join_kernel<P>, (unsigned)((long long)p.a.c.B * p.a.c.G * p.rows), 128, 0, true, s, "kv8_join", p);
 }
 template <int P, bool E4M3>
 void run_rows(const StepParams& p, cudaStream_t s) {

@@ -203,17 +203,12 @@ def kv8_expand(cache: Mapping[str, torch.Tensor], length: Position, head_dim: in
     return ref.kv8_expand(cache, host if dev is None else dev, head_dim, rows)
 
 
-# Queries of a key/value head from which on a call's tokens count as a portion of a prompt: the cache is expanded once and
-# tensor-core attention runs over it, instead of reading the codes again for every 16 queries.
-KV8_PORTION = 64
-
-
 def kv8_attention(q: torch.Tensor, cache: Mapping[str, torch.Tensor], pos: Position, k: Optional[torch.Tensor] = None,
                   v: Optional[torch.Tensor] = None, scale: Optional[float] = None, most: Optional[int] = None) -> torch.Tensor:
     """Causal attention of ``q`` [B, T, H, D] at positions ``pos`` .. ``pos + T - 1`` over the cached keys up to each query's own ->
     [B, T, H, D]. With ``k`` and ``v`` [B, T, G, D], the queries' tokens are appended first (:func:`kv8_append`, also on
     ``pos``); without, the cache must hold them already. ``most`` is a bound on the tokens that any sequence holds after this call, by
-    default the capacity (or ``pos + T`` where ``pos`` is a number): the work is laid out for it, results do not depend on it beyond rounding.
+    default the capacity (or ``pos + T`` where ``pos`` is a number), for which the work is laid out; tokens past it are not promised to be seen.
 
     Idle sequences (negative positions) give zeros; a query past the capacity (positions on the device only) gives NaN."""
     codes = cache["k8"]
@@ -235,22 +230,9 @@ def kv8_attention(q: torch.Tensor, cache: Mapping[str, torch.Tensor], pos: Posit
         if k is not None:
             ref.kv8_append(cache, k, v, host if dev is None else dev)
         return ref.kv8_attention(q, cache, host if dev is None else dev, scale)
-    if T * (q.shape[2] // codes.shape[1]) < KV8_PORTION:
-        out = _ext.ext().kv8_attention(*_parts(cache), q, k, v, host, dev, scale, most)
-        _tick(2 + (k is not None))
-        return out
-    if k is not None:
-        kv8_append(cache, k, v, pos)
-    if dev is None:
-        if host < 0:
-            return torch.zeros(q.shape, dtype=q.dtype, device=q.device)
-        kk, vv = kv8_expand(cache, host + T, q.shape[3])
-        return attention(q, kk, vv, scale=scale)
-    ends = torch.where(dev < 0, torch.zeros_like(dev), dev + T).expand(q.shape[0])  # idle: no keys
-    kk, vv = kv8_expand(cache, ends, q.shape[3])
-    out = attention(q, kk, vv, key_lengths=ends, query_start=dev, scale=scale)
-    past = dev.expand(q.shape[0])[:, None] + torch.arange(T, device=q.device) >= codes.shape[2]
-    return out.masked_fill_(past[:, :, None, None], float("nan"))
+    out = _ext.ext().kv8_attention(*_parts(cache), q, k, v, host, dev, scale, most, status_word(q.device))
+    _tick(2 + (k is not None))
+    return out
 
 
 def kv8_kind(cache: Mapping[str, Any]) -> str:

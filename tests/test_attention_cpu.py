@@ -1,0 +1,205 @@
+"""Softmax attention and the 8-bit key/value cache on the CPU: the PyTorch statements against the definition, refusals, the layers and
+models that use them."""
+
+import pytest
+import torch
+
+from attention_cases import attention64, cache64, kv8_attention64
+from triune_b200 import ops
+from triune_b200.config import ModelConfig
+from triune_b200.inference import GraphedGreedyDecoder, generate_tokens
+from triune_b200.models import SoftmaxAttention, kv8_state
+from triune_b200.models.layer_state import LayerState
+from triune_b200.models.universal import DenseTransformerBlock, UniversalDenseTransformer
+from triune_b200.serve.srsm import _pack, _unpack
+
+KINDS = ["int8", "e4m3"]
+
+
+def rand(*shape, seed=0, dtype=torch.float32):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed), dtype=dtype)
+
+
+@pytest.mark.parametrize("shape", [(1, 1, 1, 1, 1, 8), (2, 7, 7, 4, 2, 16), (3, 5, 20, 3, 1, 8), (2, 9, 4, 2, 2, 8)])
+@pytest.mark.parametrize("how", [{}, {"causal": False}, {"window": 3}, {"scale": 0.3}])
+def test_attention_and_its_gradients(shape, how):
+    B, T, S, H, G, D = shape
+    q, k, v = rand(B, T, H, D, dtype=torch.float64), rand(B, S, G, D, seed=1, dtype=torch.float64), rand(B, S, G, D, seed=2, dtype=torch.float64)
+    inputs = [x.requires_grad_() for x in (q, k, v)]
+    lengths, grad = [S, 0, 1][:B], rand(B, T, H, D, seed=3, dtype=torch.float64)
+    for n in (None, lengths):
+        out = ops.attention(*inputs, key_lengths=None if n is None else torch.tensor(n), **how)
+        want = attention64(*inputs, how.get("causal", True), how.get("window"), n, None, how.get("scale"), grad)
+        for got, name in zip((out, *torch.autograd.grad(out, inputs, grad)), ("o", "dq", "dk", "dv")):
+            assert torch.allclose(got, want[name][0], rtol=1e-10, atol=1e-12), name
+
+
+def test_gradients_against_differences():
+    q, k, v = (rand(1, n, h, 4, seed=h, dtype=torch.float64).requires_grad_() for n, h in ((3, 4), (5, 2), (5, 2)))
+    assert torch.autograd.gradcheck(lambda *x: ops.attention(*x, window=3, key_lengths=torch.tensor([4])), (q, k, v))
+
+
+def test_positions_and_what_masked_places_hold():
+    q, k, v = rand(2, 4, 2, 8), rand(2, 10, 1, 8, seed=1), rand(2, 10, 1, 8, seed=2)
+    starts = torch.tensor([3, 6])
+    out = ops.attention(q, k, v, query_start=starts)
+    for b in range(2):
+        assert torch.allclose(out[b : b + 1], ops.attention(q[b : b + 1], k[b : b + 1], v[b : b + 1], query_start=int(starts[b])), atol=1e-6)
+    clean = ops.attention(q, k, v, key_lengths=torch.tensor([7, 7]), causal=False)
+    k[:, 7:], v[:, 7:] = float("nan"), float("inf")
+    assert torch.equal(ops.attention(q, k, v, key_lengths=torch.tensor([7, 7]), causal=False), clean)
+    out = ops.attention(q, k[:, :8].nan_to_num(0.0), v[:, :8], query_start=4)
+    assert torch.isfinite(out[:, :3]).all() and not torch.isfinite(out[:, 3:]).any()
+
+
+@pytest.mark.parametrize("bad", [
+    dict(q=(2, 3, 4)), dict(q=(1, 3, 3, 8)), dict(q=(2, 3, 4, 8)), dict(q=(1, 3, 4, 16)), dict(v=(1, 4, 2, 8)), dict(k=(1, 5, 0, 8), v=(1, 5, 0, 8)),
+    dict(dtype=torch.float64), dict(how={"window": 0}), dict(how={"window": 2.5}), dict(how={"window": 3, "causal": False}), dict(how={"scale": 0.0}),
+    dict(how={"scale": float("nan")}), dict(how={"key_lengths": torch.tensor([1.0])}), dict(how={"key_lengths": torch.tensor([1, 2])}),
+    dict(how={"query_start": torch.tensor([1, 2, 3])}),
+])
+def test_attention_refuses(bad):
+    q, k, v = rand(*bad.get("q", (1, 3, 4, 8))), rand(*bad.get("k", (1, 5, 2, 8))), rand(*bad.get("v", (1, 5, 2, 8)))
+    with pytest.raises(ValueError):
+        ops.attention(q.to(bad.get("dtype", q.dtype)), k, v, **bad.get("how", {}))
+
+
+def rows(*shape, seed=0):
+    x = rand(*shape, seed=seed)
+    x[..., 1] *= 7.0
+    return x.bfloat16()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D", [8, 64, 80])
+def test_the_cache_and_attention_from_it(kind, D):
+    B, G, H, n = 3, 2, 4, 150
+    k, v, q = rows(B, n + 80, G, D), rows(B, n + 80, G, D, seed=1), rand(B, 5, H, D, seed=2).bfloat16()
+    cache = ops.kv8_cache(B, G, 256, D, kind)
+    ops.kv8_append(cache, k[:, :n], v[:, :n], 0)
+    for x, y in zip(ops.kv8_expand(cache, n, D), (k, v)):
+        for b in range(B):
+            assert torch.equal(x[b].transpose(0, 1), cache64(y[b].transpose(0, 1), kind, n).float().bfloat16())
+    starts = torch.tensor([n, -1, 100])  # the third sequence goes back by 50 tokens
+    at = torch.stack([torch.arange(max(0, s), max(0, s) + 5) for s in starts.tolist()])
+    new = [torch.stack([x[b, at[b]] for b in range(B)]) for x in (k, v)]
+    before = {name: t.clone() for name, t in cache.items()}
+    out = ops.kv8_attention(q, cache, starts, *new)
+    assert not out[1].any() and all(torch.equal(before[name][1].view(torch.uint8), t[1].view(torch.uint8)) for name, t in cache.items())
+    value, bound = kv8_attention64(q[0], k[0].transpose(0, 1), v[0].transpose(0, 1), kind, n)
+    assert bool(((out[0].double() - value).abs() <= bound).all())
+    past = ops.kv8_attention(q, cache, torch.tensor([254, 256, -3]), *new)
+    assert bool(torch.isnan(past[0, 2:]).all()) and not torch.isnan(past[0, :2]).any() and bool(torch.isnan(past[1]).all()) and not past[2].any()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_contents_do_not_depend_on_the_portions(kind):
+    k, v = rows(2, 300, 2, 64), rows(2, 300, 2, 64, seed=1)
+    whole = ops.kv8_cache(2, 2, 300, 64, kind)
+    ops.kv8_append(whole, k, v, 0)
+    for chunk in (1, 50, 64, 129):
+        cache = ops.kv8_cache(2, 2, 300, 64, kind)
+        for p in range(0, 300, chunk):
+            ops.kv8_append(cache, k[:, p : p + chunk], v[:, p : p + chunk], torch.tensor([p, p]))
+        assert all(torch.equal(cache[n].view(torch.uint8), whole[n].view(torch.uint8)) for n in whole)
+
+
+def test_a_block_with_what_is_no_number_reads_as_none():
+    cache = ops.kv8_cache(1, 1, 128, 8)
+    k, v = rows(1, 128, 1, 8), rows(1, 128, 1, 8)
+    v[0, 70, 0, 0] = float("inf")
+    ops.kv8_append(cache, k, v, 0)
+    got = ops.kv8_expand(cache, 128, 8)[1][0, :, 0]
+    assert torch.isfinite(got[:64]).all() and bool(torch.isnan(got[64:]).all())
+
+
+def test_the_cache_refuses():
+    cache, k = ops.kv8_cache(2, 2, 100, 64), rows(2, 3, 2, 64)
+    q = rows(2, 3, 4, 64)
+    assert cache["k8"].shape == (2, 2, 128, 64) and ops.kv8_cache(1, 1, 1, 72)["k8"].shape[3] == 128
+    for bad in (dict(kind="int4"), dict(head_dim=136), dict(head_dim=12), dict(kv_heads=0), dict(capacity=-1)):
+        with pytest.raises(ValueError):
+            ops.kv8_cache(**{**dict(batch=1, kv_heads=1, capacity=64, head_dim=64), **bad})
+    for call in (lambda: ops.kv8_append(cache, k.float(), k.float(), 0), lambda: ops.kv8_append(cache, k, k[:, :2], 0), lambda: ops.kv8_append(cache, k[:1], k[:1], 0),
+                 lambda: ops.kv8_append(cache, k, k, 126), lambda: ops.kv8_append(cache, k, k, torch.tensor([1.0])), lambda: ops.kv8_append(cache, k, k, torch.tensor([1, 2, 3])),
+                 lambda: ops.kv8_attention(q[:, :, :3], cache, 0), lambda: ops.kv8_attention(q.float(), cache, 0), lambda: ops.kv8_attention(q, cache, 0, k),
+                 lambda: ops.kv8_attention(q, cache, 0, k[:, :2], k[:, :2]), lambda: ops.kv8_attention(q, cache, 0, scale=-1.0),
+                 lambda: ops.kv8_expand(cache, 10, 60), lambda: ops.kv8_expand(cache, 129, 64), lambda: ops.kv8_expand(cache, 10, 64, 200)):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(RuntimeError, match="no gradients"):
+        ops.kv8_attention(q.requires_grad_(), cache, 0, k, k)
+
+
+# ---------------------------------------------------------------------------------------------------- layers and models
+def model(kv_cache=None, **kw):
+    torch.manual_seed(0)
+    cfg = ModelConfig(family="universal", vocab_size=61, hidden_dim=32, num_layers=2, num_heads=4, head_dim=8, num_kv_heads=2, mixer="sdpa",
+                      ffn="swiglu", dense_hidden=48, kv_cache=kv_cache, **kw).validate()
+    return UniversalDenseTransformer.from_config(cfg).eval()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@torch.no_grad()
+def test_a_layer_serves_from_8_bits_near_what_it_serves_from_16(kind):
+    """Keys and values of the full blocks are off by half a code of their block's scale: 1 / 254 (int8) of the block's largest, or 2^-4 of
+    themselves (e4m3); outputs are averages of values, so they stay within a few per cent of their size."""
+    torch.manual_seed(1)
+    layer = SoftmaxAttention(64, 8, 8, 2)
+    x = rand(2, 200, 64)
+    wide, cache = (None, 0), (kv8_state(2, 2, 8, kind), 0)
+    for part in x.split((130, 1, 1, 60, 1, 7), 1):
+        a, wide = layer(part, cache=wide)
+        b, cache = layer(part, cache=cache)
+        assert float((a - b).norm() / a.norm()) < (0.03 if kind == "int8" else 0.1)
+    assert cache[1] == 200 and isinstance(cache[0], LayerState) and cache[0].capacity >= 200
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_generation_does_not_depend_on_the_portions_of_the_prompt(kind):
+    m = model(kind)
+    ids = torch.randint(0, 61, (1, 150), generator=torch.Generator().manual_seed(3))
+    outs = [generate_tokens(m, ids, 20, temperature=0.0, repetition_penalty=1.0, count_penalty=0.0, prefill_chunk=150)[0] for _ in range(2)]
+    assert outs[0] == outs[1] and len(outs[0]) == 20
+    decoder = GraphedGreedyDecoder(m, 1)
+    for _ in range(2):  # a second request in the same buffers
+        assert decoder.generate(ids, 20)[0, 150:].tolist() == outs[0]
+
+
+def test_sessions_are_parked_and_come_back():
+    m = model("int8")
+    ids = torch.randint(0, 61, (1, 100), generator=torch.Generator().manual_seed(4))
+    with torch.no_grad():
+        _, cache = m(ids, cache=m.init_cache(1))
+        back = _unpack(*_pack(cache))
+        assert all(b[0].capacity == 128 and b[1] == 100 for b in back)
+        step = torch.tensor([[5]])
+        a, _ = m(step, cache=[(c[0].clone(), c[1]) for c in cache])
+        b, after = m(step, cache=back)
+    assert torch.equal(a, b) and after[0][1] == 101
+
+
+def test_growing_keeps_what_is_held():
+    state = kv8_state(1, 2, 8, "e4m3")
+    k, v = rows(1, 200, 2, 8), rows(1, 200, 2, 8, seed=1)
+    ops.kv8_append(state, k, v, 0)
+    want = ops.kv8_expand(state, 200, 8)
+    assert state.reserve(1000) and state.capacity == 1024 and state["ks"].shape[2] == 16 and not state.reserve(1024)
+    assert all(torch.equal(a, b) for a, b in zip(ops.kv8_expand(state, 200, 8), want))
+
+
+def test_configurations_without_such_a_cache_are_refused():
+    for bad in (dict(kv_cache="int4"), dict(kv_cache="int8", mixer="gla"), dict(kv_cache="int8", family="triune")):
+        with pytest.raises(ValueError):
+            ModelConfig(**{**dict(family="universal", hidden_dim=32, num_heads=4, head_dim=8, num_layers=8, mixer="sdpa"), **bad}).validate()
+    assert ModelConfig.from_dict(model("e4m3").cfg.to_dict()).kv_cache == "e4m3"
+
+
+def test_training_a_model_with_shared_heads():
+    m = model().train()
+    ids = torch.randint(0, 61, (2, 40), generator=torch.Generator().manual_seed(5))
+    m.forward_loss(ids[:, :-1], ids[:, 1:]).backward()
+    assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in m.parameters())
+    block = DenseTransformerBlock(32, 4, num_kv_heads=2)
+    y, state = block(rand(1, 5, 32), state=(None, 0))
+    assert y.shape == (1, 5, 32) and state[0][0].shape == (1, 5, 2, 8)

@@ -1,0 +1,96 @@
+"""Layers and models over the softmax attention kernels, and over the 8-bit cache: trained, prompted, decoded in graphs."""
+
+import pytest
+import torch
+
+from triune_b200 import _ext, ops
+from triune_b200.config import ModelConfig
+from triune_b200.inference import GraphedGreedyDecoder, advance, generate_tokens
+from triune_b200.models import SoftmaxAttention, kv8_state
+from triune_b200.models.universal import UniversalDenseTransformer
+from triune_b200.utils import place_model
+
+pytestmark = pytest.mark.gpu
+
+
+def layer(heads=8, kv_heads=2, head_dim=64, seed=0):
+    torch.manual_seed(seed)
+    return SoftmaxAttention(heads * head_dim, heads, head_dim, kv_heads).cuda().bfloat16()
+
+
+def rel(a, b):
+    return float((a.double() - b.double()).norm() / b.double().norm())
+
+
+@pytest.mark.parametrize("kv_heads,head_dim,prefix", [(2, 64, 0), (8, 64, 77), (2, 128, 300), (1, 80, 5)])
+def test_a_layer_follows_its_plain_form(kv_heads, head_dim, prefix):
+    """Against the layer in fp32 with the same weights: projections, rotations and outputs are rounded to bf16 (2^-8 at most, some
+    2^-9.3 on average), five of them on the way to an output and twice as many to a gradient, errors of which are independent."""
+    m = layer(8, kv_heads, head_dim)
+    plain = SoftmaxAttention(m.dim, 8, head_dim, kv_heads).cuda()
+    plain.load_state_dict(m.state_dict())
+    x = torch.randn(2, 150, m.dim, device="cuda").bfloat16().requires_grad_()
+    y = x.detach().float().requires_grad_()
+    past = [torch.randn(2, prefix, kv_heads, head_dim, device="cuda").bfloat16() for _ in "kv"]
+    before = ops.launch_count()
+    a, state = m(x, cache=((past[0], past[1]), prefix) if prefix else None)
+    assert ops.launch_count() > before
+    _ext.set_reference_ops(True)
+    try:
+        b, _ = plain(y, cache=((past[0].float(), past[1].float()), prefix) if prefix else None)
+        g = torch.randn_like(a)
+        want = torch.autograd.grad(b, [y, *plain.parameters()], g.float())
+    finally:
+        _ext.set_reference_ops(False)
+    assert rel(a, b) < 2e-2
+    got = torch.autograd.grad(a, [x, *m.parameters()], g)
+    assert all(rel(p, q) < 4e-2 for p, q in zip(got, want))
+    assert state is None or state[0][0].shape[1] == prefix + 150
+
+
+def model(kv_cache, head_dim=64, seed=1):
+    torch.manual_seed(seed)
+    cfg = ModelConfig(family="universal", vocab_size=512, hidden_dim=8 * head_dim, num_layers=3, num_heads=8, head_dim=head_dim, num_kv_heads=2,
+                      mixer="sdpa", ffn="swiglu", dense_hidden=768, kv_cache=kv_cache).validate()
+    return place_model(UniversalDenseTransformer.from_config(cfg), "cuda", torch.bfloat16).eval()
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+def test_decoding_in_a_graph_is_decoding_step_by_step(kind):
+    m = model(kind)
+    ids = torch.randint(0, 512, (1, 200), device="cuda", generator=torch.Generator("cuda").manual_seed(2))
+    decoder = GraphedGreedyDecoder(m, 1)
+    for n in (200, 90, 150):  # the second and third request find the buffers and the capture of the first
+        want = generate_tokens(m, ids[:, :n], 140, temperature=0.0, repetition_penalty=1.0, count_penalty=0.0, prefill_chunk=4096)[0]
+        assert decoder.generate(ids[:, :n], 140)[0, n:].tolist() == want
+
+
+@pytest.mark.parametrize("kind,limit", [("int8", 0.05), ("e4m3", 0.15)])
+@torch.no_grad()
+def test_logits_from_8_bits_are_near_those_from_16(kind, limit):
+    narrow, wide = model(kind), model(None)
+    ids = torch.randint(0, 512, (2, 300), device="cuda", generator=torch.Generator("cuda").manual_seed(3))
+    caches = [m.init_cache(2) for m in (narrow, wide)]
+    for part in ids.split((200, 3, 1, 96), 1):
+        (a, caches[0]), (b, caches[1]) = (advance(m, part, c) for m, c in zip((narrow, wide), caches))
+        assert rel(a, b) < limit
+
+
+@torch.no_grad()
+def test_a_cache_on_another_stream_and_one_that_grows():
+    m = layer()
+    x = torch.randn(1, 700, m.dim, device="cuda").bfloat16()
+    outs = []
+    for side in (False, True):
+        stream = torch.cuda.Stream() if side else torch.cuda.current_stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            cache = (kv8_state(1, 2, 64, "int8", "cuda"), 0)
+            out = []
+            for part in x.split((1, 255, 2, 300, 142), 1):
+                y, cache = m(part, cache=cache)
+                out.append(y)
+            outs.append(torch.cat(out, 1))
+        torch.cuda.current_stream().wait_stream(stream)
+        assert cache[1] == 700 and cache[0].capacity >= 700
+    assert torch.equal(*outs)

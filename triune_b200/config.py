@@ -122,6 +122,7 @@ class ModelConfig:
     mixer: str = "gla"  # "gla" | "gated_deltanet" | "sdpa"
     ffn: str = "gelu"  # dense FFN activation: "gelu" | "swiglu"
     num_kv_heads: Optional[int] = None  # sdpa mixer only (GQA)
+    kv_cache: Optional[str] = None  # sdpa mixer only: keys and values cached in 8 bits, "int8" | "e4m3" (None: as they come)
     use_rope: bool = True
     gla_scale: str = "none"  # "fla": GLA outputs times head_dim ** -0.5 (models trained by the reference with flash-linear-attention)
     rope_base: float = ROPE_BASE
@@ -227,6 +228,11 @@ class ModelConfig:
             raise ValueError("use_fp4 and use_fp8 are mutually exclusive")
         if self.mixer not in ("gla", "gated_deltanet", "sdpa"):
             raise ValueError(f"unknown mixer {self.mixer!r}")
+        if self.kv_cache is not None:
+            if self.kv_cache not in ("int8", "e4m3"):
+                raise ValueError(f"kv_cache must be 'int8', 'e4m3' or None, got {self.kv_cache!r}")
+            if self.family != "universal" or self.mixer != "sdpa" or self.head_dim % 8 or self.head_dim > 128:
+                raise ValueError("kv_cache needs a universal model with the sdpa mixer and heads of a multiple of 8 up to 128")
         return self
 
     def to_dict(self) -> Dict[str, Any]:

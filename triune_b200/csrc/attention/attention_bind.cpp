@@ -99,57 +99,64 @@ void append_rows(const tb::Kv8Cache& c, const Tensor& k, const Tensor& v, const 
   if (k.numel() > 0) tb::launch_kv8_append(c, kv, vv, (int)k.size(1), (int)k.size(3), pos, cur_stream());
 }
 
-// Forward pass of f.a; -> out, and lse where it is asked for
-Tensor attend(tb::AttentionFwd& f, const Tensor& q, const Tensor& k, const Tensor& v, bool want_lse, const Tensor& status, Tensor& lse) {
+// Forward pass of f.a; -> out, and what the backward pass wants where it will come
+Tensor attend(tb::AttentionFwd& f, const Tensor& q, const Tensor& k, const Tensor& v, bool train, const Tensor& status, Tensor& lse, Tensor& rest) {
   Tensor hq, hk, hv, part;
   f.q = view_of(q, q, "queries", hq);
   f.k = view_of(k, q, "keys", hk);
   f.v = view_of(v, q, "values", hv);
   Tensor out = torch::empty(q.sizes(), q.options());
   const auto f32 = q.options().dtype(at::kFloat);
-  if (want_lse) lse = torch::empty({f.a.B, f.a.H, tb::attention_rows(f.a.T)}, f32);
+  if (train) {
+    lse = torch::empty({f.a.B, f.a.H, tb::attention_rows(f.a.T)}, f32);
+    rest = torch::empty(q.sizes(), q.options());
+  }
   if (out.numel() == 0) return out;
   if (f.a.S == 0) {
-    out.zero_();
-    if (want_lse) lse.fill_(-INFINITY);
-    return out;
+    if (train) {
+      lse.fill_(-INFINITY);
+      rest.zero_();
+    }
+    return out.zero_();
   }
   const long long bytes = tb::attention_fwd_scratch(f.a);
   if (bytes > 0) part = torch::empty({bytes / 4}, f32);
   f.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
-  f.lse = want_lse ? lse.data_ptr<float>() : nullptr;
+  f.lse = train ? lse.data_ptr<float>() : nullptr;
+  f.rest = train ? reinterpret_cast<__nv_bfloat16*>(rest.data_ptr()) : nullptr;
   f.part = bytes > 0 ? part.data_ptr<float>() : nullptr;
   f.status = status_of(status);
   tb::launch_attention_fwd(f, cur_stream());
   return out;
 }
 
-// -> (out, lse). lse is empty where it is not asked for.
+// -> (out, lse, rest); the last two, for the backward pass, are empty without `train`.
 std::vector<Tensor> attention_fwd(const Tensor& q, const Tensor& k, const Tensor& v, double scale, bool causal, int64_t window, const OptTensor& lengths,
-                                  const OptTensor& starts, int64_t start, bool want_lse, const Tensor& status) {
+                                  const OptTensor& starts, int64_t start, bool train, const Tensor& status) {
   tb::AttentionFwd f{};
   f.a = shape_of(q, k, v, scale, causal, window, lengths, starts, start);
   c10::cuda::CUDAGuard guard(q.device());
-  Tensor lse, out = attend(f, q, k, v, want_lse, status, lse);
-  return {out, lse};
+  Tensor lse, rest, out = attend(f, q, k, v, train, status, lse, rest);
+  return {out, lse, rest};
 }
 
 // -> (dq, dk, dv)
-std::vector<Tensor> attention_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out, const Tensor& dout, const Tensor& lse, double scale,
+std::vector<Tensor> attention_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out, const Tensor& rest, const Tensor& dout, const Tensor& lse, double scale,
                                   bool causal, int64_t window, const OptTensor& lengths, const OptTensor& starts, int64_t start, const Tensor& status) {
   tb::AttentionBwd f{};
   f.a = shape_of(q, k, v, scale, causal, window, lengths, starts, start);
-  TORCH_CHECK(out.sizes() == q.sizes() && dout.sizes() == q.sizes(), "attention: outputs and their gradients have the queries' shape");
+  TORCH_CHECK(out.sizes() == q.sizes() && rest.sizes() == q.sizes() && dout.sizes() == q.sizes(), "attention: outputs and their gradients have the queries' shape");
   TORCH_CHECK(lse.is_cuda() && lse.get_device() == q.get_device() && lse.scalar_type() == at::kFloat && lse.is_contiguous() &&
                   lse.numel() == (int64_t)f.a.B * f.a.H * tb::attention_rows(f.a.T) && (reinterpret_cast<uintptr_t>(lse.data_ptr()) & 15) == 0,
               "attention: the forward pass's sums");
   c10::cuda::CUDAGuard guard(q.device());
-  Tensor held[5];
+  Tensor held[6];
   f.q = view_of(q, q, "queries", held[0]);
   f.k = view_of(k, q, "keys", held[1]);
   f.v = view_of(v, q, "values", held[2]);
   f.out = view_of(out, q, "outputs", held[3]);
   f.dout = view_of(dout, q, "gradients", held[4]);
+  f.rest = view_of(rest, q, "outputs", held[5]);
   Tensor dq = torch::empty(q.sizes(), q.options()), dk = torch::empty(k.sizes(), k.options()), dv = torch::empty(v.sizes(), v.options());
   if (dq.numel() == 0 || dk.numel() == 0) return {dq.zero_(), dk.zero_(), dv.zero_()};
   Tensor delta = torch::empty(lse.sizes(), lse.options());
@@ -239,7 +246,7 @@ Tensor kv8_attention(const Tensor& k8, const Tensor& v8, const Tensor& ks, const
   f.k_scales = to.k_scales;
   f.v_scales = to.v_scales;
   f.blocks = (int)blocks;
-  out = attend(f, q, kk, vv, false, status, part);
+  out = attend(f, q, kk, vv, false, status, part, part);
   if (a.pos.dev != nullptr) tb::launch_kv8_outside(c, reinterpret_cast<__nv_bfloat16*>(out.data_ptr()), a.T, a.H * a.D, a.pos, cur_stream());
   return out;
 }

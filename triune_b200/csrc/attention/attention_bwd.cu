@@ -24,7 +24,7 @@ constexpr int BW_THREADS = 384;
 
 struct BwdParams {
   AttentionShape a;
-  AttentionView out, dout;
+  AttentionView out, rest, dout;
   const float* lse;
   float* delta;
   __nv_bfloat16 *dq, *dk, *dv;
@@ -176,15 +176,16 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
     float dot = 0.f;
     if (t < p.a.T) {
       const uint4* o = reinterpret_cast<const uint4*>((const __nv_bfloat16*)p.out.p + b * p.out.sb + t * p.out.sr + h * p.out.sh);
+      const uint4* l = reinterpret_cast<const uint4*>((const __nv_bfloat16*)p.rest.p + b * p.rest.sb + t * p.rest.sr + h * p.rest.sh);
       const uint4* g = reinterpret_cast<const uint4*>((const __nv_bfloat16*)p.dout.p + b * p.dout.sb + t * p.dout.sr + h * p.dout.sh);
       const int pieces = p.a.D / 8, mid = (pieces + 1) / 2;
       for (int i = half * mid; i < (half == 0 ? mid : pieces); ++i) {
-        const uint4 x = o[i], y = g[i];
-        const uint32_t *xp = &x.x, *yp = &y.x;
+        const uint4 x = o[i], y = g[i], z = l[i];
+        const uint32_t *xp = &x.x, *yp = &y.x, *zp = &z.x;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          dot = fmaf(__uint_as_float(xp[e] << 16), __uint_as_float(yp[e] << 16), dot);
-          dot = fmaf(__uint_as_float(xp[e] & 0xffff0000u), __uint_as_float(yp[e] & 0xffff0000u), dot);
+          dot = fmaf(__uint_as_float(xp[e] << 16) + __uint_as_float(zp[e] << 16), __uint_as_float(yp[e] << 16), dot);
+          dot = fmaf(__uint_as_float(xp[e] & 0xffff0000u) + __uint_as_float(zp[e] & 0xffff0000u), __uint_as_float(yp[e] & 0xffff0000u), dot);
         }
       }
     }
@@ -547,7 +548,7 @@ void run_bwd(const AttentionBwd& f, cudaStream_t s) {
   static_assert(smem + 1280 <= 227 * 1024 && smem_kv <= 227 * 1024, "shared memory of a block");
   const CUtensorMap tq = attention_map(f.q, a.D, a.T, a.H, a.B), tg = attention_map(f.dout, a.D, a.T, a.H, a.B),
                     tk = attention_map(f.k, a.D, a.S, a.G, a.B), tv = attention_map(f.v, a.D, a.S, a.G, a.B);
-  const BwdParams p{a, f.out, f.dout, f.lse, f.delta, f.dq, f.dk, f.dv, a.scale * LOG2E, f.status};
+  const BwdParams p{a, f.out, f.rest, f.dout, f.lse, f.delta, f.dq, f.dk, f.dv, a.scale * LOG2E, f.status};
   static PerDeviceOnce once;
   if (once.first_use()) {
     cudaFuncSetAttribute(attention_dq_kernel<DB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);

@@ -31,7 +31,7 @@ constexpr int FW_POLY = 4;  // of so many pairs of exponentials one is a polynom
 
 struct FwdParams {
   AttentionShape a;
-  __nv_bfloat16* out;
+  __nv_bfloat16 *out, *rest;
   float* lse;
   float* part;  // [splits, B, H, T, 64 * DB] sums, then [splits, B, H, T, 2] maxima and weights
   const __nv_bfloat16* v;
@@ -463,6 +463,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __gr
           for (int g = 0; g < 4; ++g) reinterpret_cast<uint4*>(po + c)[g] = make_uint4(x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]);
         } else {
           store_row16(o, c, p.a.D, x, r);
+          if (p.rest != nullptr) store_rest16(p.rest + (o - p.out), c, p.a.D, x, r);
         }
       }
     }
@@ -498,7 +499,12 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const FwdParams p) 
   const float r = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
   for (int i = 0; i < 2 * DB; ++i)
-    if (lane + 32 * i < p.a.D) p.out[((b * p.a.T + t) * p.a.H + h) * p.a.D + lane + 32 * i] = __float2bfloat16(acc[i] * r);
+    if (lane + 32 * i < p.a.D) {
+      const long long at = ((b * p.a.T + t) * p.a.H + h) * p.a.D + lane + 32 * i;
+      const __nv_bfloat16 y = __float2bfloat16(acc[i] * r);
+      p.out[at] = y;
+      if (p.rest != nullptr) p.rest[at] = __float2bfloat16(acc[i] * r - __bfloat162float(y));
+    }
   if (p.lse != nullptr && lane == 0) {
     const int padded = (p.a.T + AT_M - 1) / AT_M * AT_M;
     float* at = p.lse + row / p.a.T * padded;
@@ -543,7 +549,7 @@ void run_width(const AttentionFwd& f, cudaStream_t s) {
   const AttentionShape& a = f.a;
   const CUtensorMap tq = attention_map(f.q, a.D, a.T, a.H, a.B), tk = attention_map(f.k, a.D, a.S, a.G, a.B), tv = attention_map(f.v, a.D, a.S, a.G, a.B);
   bool pair;
-  FwdParams p{a, f.out, f.lse, f.part, (const __nv_bfloat16*)f.v.p, f.v.sr, f.v.sh, f.v.sb, f.k_scales, f.v_scales, f.blocks, fwd_splits(a, pair), a.scale * LOG2E, f.status};
+  FwdParams p{a, f.out, f.rest, f.lse, f.part, (const __nv_bfloat16*)f.v.p, f.v.sr, f.v.sh, f.v.sb, f.k_scales, f.v_scales, f.blocks, fwd_splits(a, pair), a.scale * LOG2E, f.status};
   if (pair) return run<DB, true, SCALED>(p, tq, tk, tv, s);
   run<DB, false, SCALED>(p, tq, tk, tv, s);
   if (p.splits > 1) {

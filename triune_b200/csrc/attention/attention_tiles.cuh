@@ -166,6 +166,22 @@ __device__ __forceinline__ void named_barrier(int id) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory");
 }
 
+// What bf16 loses of 16 values times r, as bf16, at `o + c` of a row of D values
+__device__ __forceinline__ void store_rest16(__nv_bfloat16* o, int c, int D, const uint32_t (&v)[16], float r) {
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+    if (c + 8 * g < D) {
+      uint4 u;
+      uint32_t* up = &u.x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float a = __uint_as_float(v[8 * g + 2 * i]) * r, b = __uint_as_float(v[8 * g + 2 * i + 1]) * r;
+        const uint32_t x = pack_bf16x2(a, b);
+        up[i] = pack_bf16x2(a - __uint_as_float(x << 16), b - __uint_as_float(x & 0xffff0000u));
+      }
+      *reinterpret_cast<uint4*>(o + c + 8 * g) = u;
+    }
+}
 // 16 bytes (8 bf16) at `o + c` of a row of D values from fp32 registers
 __device__ __forceinline__ void store_row16(__nv_bfloat16* o, int c, int D, const uint32_t (&v)[16], float r) {
 #pragma unroll

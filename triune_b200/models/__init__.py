@@ -1,7 +1,7 @@
 """Model families: multi-exit MoE ``TriuneTransformer``, dense ``UniversalTransformer`` and ``HybridTransformer`` with
 layers that differ (``Bubitar``, ``Famalorn``)."""
 
-from .attention import HybridAttention, SoftmaxAttention, VectorisedGLA
+from .attention import HybridAttention, SoftmaxAttention, VectorisedGLA, kv8_state
 from .block import DenseFFN, TransformerBlock
 from .bubitar import Bubitar
 from .famalorn import Famalorn
@@ -13,6 +13,6 @@ from .router import GumbelSoftmaxRouter
 from .transformer import TriuneTransformer
 
 __all__ = [
-    "Bubitar", "Famalorn", "HybridTransformer", "HybridAttention", "SoftmaxAttention", "VectorisedGLA", "DenseFFN", "TransformerBlock", "MoE_FFN",
+    "Bubitar", "Famalorn", "HybridTransformer", "HybridAttention", "SoftmaxAttention", "VectorisedGLA", "kv8_state", "DenseFFN", "TransformerBlock", "MoE_FFN",
     "RoutingResult", "RMSNorm", "RotaryEmbedding", "GumbelSoftmaxRouter", "TriuneTransformer",
 ]

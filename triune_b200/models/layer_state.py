@@ -15,11 +15,12 @@ KV_GRAIN = 64  # capacities are multiples of this many positions
 
 
 class LayerState:
-    """``tensors``: the state proper. Names in ``growable`` are [B, groups, capacity, head] and hold ``position`` valid
-    entries along dimension 2. ``scratch``: work space of the step kernels, not part of the state."""
+    """``tensors``: the state proper. Names in ``growable`` are [B, groups, capacity, ...] and hold ``position`` valid
+    entries along dimension 2; those in ``per`` have one entry for so many positions there. ``scratch``: work space of the step
+    kernels, not part of the state."""
 
-    def __init__(self, tensors: Dict[str, torch.Tensor], growable: Tuple[str, ...] = ()):
-        self.tensors, self.growable = tensors, tuple(growable)
+    def __init__(self, tensors: Dict[str, torch.Tensor], growable: Tuple[str, ...] = (), per: Optional[Dict[str, int]] = None):
+        self.tensors, self.growable, self.per = tensors, tuple(growable), dict(per or {})
         self.scratch: Dict[str, torch.Tensor] = {}
 
     def __getitem__(self, name: str) -> torch.Tensor:
@@ -30,7 +31,7 @@ class LayerState:
 
     @property
     def capacity(self) -> Optional[int]:
-        return self.tensors[self.growable[0]].shape[2] if self.growable else None
+        return self.tensors[self.growable[0]].shape[2] * self.per.get(self.growable[0], 1) if self.growable else None
 
     def reserve(self, positions: int) -> bool:
         """Make room for ``positions`` in all; doubles, so that appending costs amortised constant time. True when the
@@ -41,13 +42,13 @@ class LayerState:
         new = -(-max(positions, 2 * cap) // KV_GRAIN) * KV_GRAIN
         for n in self.growable:
             old = self.tensors[n]
-            t = torch.zeros(*old.shape[:2], new, old.shape[3], dtype=old.dtype, device=old.device)
-            t[:, :, :cap].copy_(old)
+            t = torch.zeros(*old.shape[:2], new // self.per.get(n, 1), *old.shape[3:], dtype=old.dtype, device=old.device)
+            t[:, :, : old.shape[2]].copy_(old)
             self.tensors[n] = t
         return True
 
     def clone(self) -> "LayerState":
-        return LayerState({k: t.clone() for k, t in self.tensors.items()}, self.growable)
+        return LayerState({k: t.clone() for k, t in self.tensors.items()}, self.growable, self.per)
 
     def copy_(self, other: "LayerState") -> "LayerState":
         """Take over ``other``'s values in place. A growable tensor keeps its own, larger capacity."""
@@ -66,15 +67,19 @@ class LayerState:
         return sum(t.numel() * t.element_size() for t in self.tensors.values())
 
     def pack(self, position: int) -> Tuple[List[torch.Tensor], List[Any]]:
-        """-> (flat tensors, layout); key/value caches are cut to their valid positions."""
+        """-> (flat tensors, layout); key/value caches are cut to their valid positions (whole entries of ``per``). The layout's last
+        field is the number of positions per entry of a growable tensor, and 0 for others."""
         flats, layout = [], []
+        block = max(self.per.values(), default=1)
+        position = -(-position // block) * block
         for n, t in self.tensors.items():
-            cut = t[:, :, :position] if n in self.growable else t
+            per = self.per.get(n, 1) if n in self.growable else 0
+            cut = t[:, :, : position // per] if per else t
             flats.append(cut.detach().reshape(-1))
-            layout.append((n, tuple(cut.shape), t.dtype, n in self.growable))
+            layout.append((n, tuple(cut.shape), t.dtype, per))
         return flats, layout
 
     @classmethod
     def unpack(cls, flats: List[torch.Tensor], layout: List[Any]) -> "LayerState":
         tensors = {n: f.view(shape).to(dt).contiguous() for f, (n, shape, dt, _) in zip(flats, layout)}
-        return cls(tensors, tuple(n for n, _, _, g in layout if g))
+        return cls(tensors, tuple(n for n, _, _, per in layout if per), {n: per for n, _, _, per in layout if per > 1})

@@ -18,7 +18,7 @@ import torch.nn.functional as F
 from .. import ops
 from ..config import ModelConfig
 from . import native_block
-from .attention import SoftmaxAttention, VectorisedGLA
+from .attention import SoftmaxAttention, VectorisedGLA, kv8_state
 from .block import DenseFFN
 from .norms import RMSNorm
 
@@ -166,6 +166,10 @@ class UniversalDenseTransformer(nn.Module):
                 nn.init.zeros_(m.bias)
 
     def init_cache(self, batch_size: int = 1) -> List[Any]:
+        """One ``(state, position)`` per layer. With ``kv_cache`` in the configuration, softmax mixers keep keys and values in 8 bits."""
+        if self.cfg.kv_cache:
+            dev = self.embed_tokens.weight.device
+            return [(kv8_state(batch_size, layer.attn.kv_heads, layer.attn.head_dim, self.cfg.kv_cache, dev), 0) for layer in self.layers]
         return [(None, 0) for _ in range(self.num_layers)]
 
     def enable_gradient_checkpointing(self, flag: bool = True):

@@ -1173,4 +1173,4 @@ def lora_linear(x, w, bias, A, B, scaling: float):
 
 
 # at the end: it builds on the names above
-from .softmax_attention import attention, attention_supported, kv8_append, kv8_attention, kv8_cache, kv8_expand, kv8_kind  # noqa: E402,F401
+from .softmax_attention import KV8_BLOCK, attention, attention_supported, kv8_append, kv8_attention, kv8_cache, kv8_expand, kv8_kind  # noqa: E402,F401

@@ -60,18 +60,18 @@ def attention_supported(q: torch.Tensor) -> bool:
 class _AttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, scale, causal, window, lengths, starts, start):
-        out, lse = _ext.ext().attention_fwd(q, k, v, scale, causal, window, lengths, starts, start, True, status_word(q.device))
+        out, lse, rest = _ext.ext().attention_fwd(q, k, v, scale, causal, window, lengths, starts, start, True, status_word(q.device))
         _tick()
-        ctx.save_for_backward(q, k, v, out, lse, lengths, starts)
+        ctx.save_for_backward(q, k, v, out, rest, lse, lengths, starts)
         ctx.how = (scale, causal, window, start)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        q, k, v, out, lse, lengths, starts = ctx.saved_tensors
+        q, k, v, out, rest, lse, lengths, starts = ctx.saved_tensors
         scale, causal, window, start = ctx.how
-        grads = _ext.ext().attention_bwd(q, k, v, out, grad.to(q.dtype), lse, scale, causal, window, lengths, starts, start, status_word(q.device))
+        grads = _ext.ext().attention_bwd(q, k, v, out, rest, grad.to(q.dtype), lse, scale, causal, window, lengths, starts, start, status_word(q.device))
         _tick(2)
         return (*grads, None, None, None, None, None, None)
 
@@ -107,7 +107,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     if _kernels(q):
         how = (scale, bool(causal), int(window or 0), lengths, starts, start)
         if inference_call(q, k, v):
-            out, _ = _ext.ext().attention_fwd(q, k, v, *how, False, status_word(q.device))
+            out, _, _ = _ext.ext().attention_fwd(q, k, v, *how, False, status_word(q.device))
             _tick()
             return out
         return _AttentionFn.apply(q, k, v, *how)

@@ -1,6 +1,8 @@
 // Python bindings of softmax attention and of the 8-bit key/value cache.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <cmath>
@@ -170,6 +172,39 @@ std::vector<Tensor> attention_bwd(const Tensor& q, const Tensor& k, const Tensor
   return {dq, dk, dv};
 }
 
+// Attention with its gradient as one node of the graph, without Python in the backward pass: of a small call's time (2 x 37 tokens, forward
+// and backward), most was Python.
+class AttentionNode : public torch::autograd::Function<AttentionNode> {
+ public:
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, double scale, bool causal, int64_t window,
+                        const OptTensor& lengths, const OptTensor& starts, int64_t start, const Tensor& status) {
+    std::vector<Tensor> r = attention_fwd(q, k, v, scale, causal, window, lengths, starts, start, true, status);
+    ctx->save_for_backward({q, k, v, r[0], r[2], r[1], has(lengths) ? *lengths : Tensor(), has(starts) ? *starts : Tensor(), status});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["causal"] = causal;
+    ctx->saved_data["window"] = window;
+    ctx->saved_data["start"] = start;
+    return r[0];
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto x = ctx->get_saved_variables();
+    std::vector<Tensor> r = attention_bwd(x[0], x[1], x[2], x[3], x[4], grads[0].to(x[0].scalar_type()), x[5], ctx->saved_data["scale"].toDouble(),
+                                          ctx->saved_data["causal"].toBool(), ctx->saved_data["window"].toInt(), x[6], x[7], ctx->saved_data["start"].toInt(), x[8]);
+    if (torch::GradMode::is_enabled()) {  // a graph of the gradients is asked for: they have none, and say so when it is used
+      torch::autograd::variable_list leaves;
+      for (Tensor& t : r) leaves.push_back(t.detach().requires_grad_(true));
+      r = (*std::make_shared<torch::autograd::DelayedError>("attention is differentiable once: its gradients have none", (int64_t)leaves.size()))(std::move(leaves));
+    }
+    const Tensor none;
+    return {r[0], r[1], r[2], none, none, none, none, none, none, none};
+  }
+};
+
+Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, double scale, bool causal, int64_t window, const OptTensor& lengths,
+                 const OptTensor& starts, int64_t start, const Tensor& status) {
+  return AttentionNode::apply(q, k, v, scale, causal, window, lengths, starts, start, status);
+}
+
 void kv8_append(const Tensor& k8, const Tensor& v8, const Tensor& ks, const Tensor& vs, const Tensor& kt, const Tensor& vt, const Tensor& k, const Tensor& v,
                 int64_t host, const OptTensor& dev) {
   const tb::Kv8Cache c = cache_of(k8, v8, ks, vs, kt, vt, k);
@@ -256,6 +291,7 @@ Tensor kv8_attention(const Tensor& k8, const Tensor& v8, const Tensor& ks, const
 void register_attention(pybind11::module& m) {
   m.def("attention_fwd", &attention_fwd);
   m.def("attention_bwd", &attention_bwd);
+  m.def("attention", &attention);
   m.def("kv8_append", &kv8_append);
   m.def("kv8_expand", &kv8_expand);
   m.def("kv8_attention", &kv8_attention);

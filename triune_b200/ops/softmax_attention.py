@@ -10,6 +10,7 @@ import math
 from typing import Any, Mapping, Optional, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _ext
 from . import _tick, inference_call
@@ -58,6 +59,9 @@ def attention_supported(q: torch.Tensor) -> bool:
 
 
 class _AttentionFn(torch.autograd.Function):
+    """What is traced: a trace records the function. Calls that are not go through the extension's own node of the graph, which
+    does the same without Python in the backward pass."""
+
     @staticmethod
     def forward(ctx, q, k, v, scale, causal, window, lengths, starts, start):
         out, lse, rest = _ext.ext().attention_fwd(q, k, v, scale, causal, window, lengths, starts, start, True, status_word(q.device))
@@ -110,7 +114,10 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
             out, _, _ = _ext.ext().attention_fwd(q, k, v, *how, False, status_word(q.device))
             _tick()
             return out
-        return _AttentionFn.apply(q, k, v, *how)
+        if torch.jit.is_tracing() or forward_ad._current_level >= 0:  # tangents: refused
+            return _AttentionFn.apply(q, k, v, *how)
+        _tick(3)  # with its backward pass, which is launched without Python
+        return _ext.ext().attention(q, k, v, *how, status_word(q.device))
     return ref.attention(q, k, v, bool(causal), window, lengths, start if starts is None else starts, scale)
 
 

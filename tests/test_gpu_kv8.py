@@ -5,6 +5,7 @@ import torch
 
 from attention_cases import BLOCK, RING, attention64, cache64, coded64, kv8_attention64, near
 from triune_b200 import ops
+from triune_b200.ops import reference
 
 pytestmark = pytest.mark.gpu
 KINDS = ["int8", "e4m3"]
@@ -166,6 +167,26 @@ def test_blocks_whose_scales_differ_and_blocks_of_zeros():
     ops.kv8_append(cache, k, v, 0)
     q = rows(1, 1, 3, 64, 3, False)
     near(ops.kv8_attention(q, cache, 329)[0], kv8_attention64(q[0], k[0].transpose(0, 1), v[0].transpose(0, 1), "int8", 329))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("exponent", [0, 1, 4, 9, 127, 200, 254])  # of the largest number of a block, from subnormal ones on
+def test_codes_of_every_number_at_every_scale(kind, exponent):
+    """A block for each of the 128 fractions of its largest number; the others are numbers of all kinds not above it."""
+    gen = torch.Generator(device="cuda").manual_seed(exponent)
+    top = torch.arange(128, device="cuda") + 128 * exponent
+    x = (torch.rand(1, 128, BLOCK * 128, generator=gen, device="cuda") * 26 * 128).long()  # bf16 numbers' bits, 26 powers of two of them
+    x = (top[None, :, None] - x).clamp(min=0)
+    x[..., 0] = top
+    x = x | (torch.rand(x.shape, generator=gen, device="cuda") < 0.5).long() << 15
+    x = x.int().short().view(torch.bfloat16).view(1, 128 * BLOCK, 1, 128)
+    cache = ops.kv8_cache(1, 1, x.shape[1], 128, kind, device="cuda")
+    ops.kv8_append(cache, x, -x, 0)
+    blocks = x.view(128, BLOCK, 128)
+    codes, scale = reference.kv8_codes(blocks, cache["k8"].dtype)
+    assert torch.equal(cache["ks"].flatten(), scale.flatten()) and torch.equal(cache["vs"].flatten(), scale.flatten())
+    assert torch.equal(bits(cache)["k8"].view(-1), codes.view(torch.uint8).view(-1))
+    assert torch.equal(bits(cache)["v8"].view(-1), reference.kv8_codes(-blocks, cache["k8"].dtype)[0].view(torch.uint8).view(-1))
 
 
 @pytest.mark.parametrize("kind", KINDS)

@@ -18,10 +18,47 @@ struct AppendParams {
 __device__ __forceinline__ long long pos_at(const Kv8Pos& p, int b) { return p.dev != nullptr ? p.dev[(long long)b * p.step] : p.host; }
 
 template <bool E4M3>
-__device__ __forceinline__ uint32_t code_of(float x, float s) {
-  const float y = s > 0.f ? __fdiv_rn(x, s) : 0.f;  // the whole block is zero, or reads as NaN whatever its codes
+__device__ __forceinline__ uint32_t code_of(float y) {
   if constexpr (E4M3) return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
   return (uint32_t)__float2int_rn(y) & 0xffu;
+}
+
+// Four codes: the nearest ones to the quotients x / s, rounded to fp32 first. Divisions and conversions to integers took 85 % of the issue
+// slots (37 us for 67 MB), so quotients are products with 1 / s, off by less than 2^-22 of themselves, and codes come from the last
+// bits of a sum with 1.5 * 2^23, or in pairs (e4m3). Where a product is so near the border between two codes that the quotient might
+// lie beyond it, the codes are formed from divisions.
+template <bool E4M3>
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[4], float s, float inv) {
+  float y[4];
+  bool near = false;
+  uint32_t code;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = x[i] * inv;
+  if constexpr (E4M3) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // borders: halfway between numbers of three bits; below the least normal number they are others
+      const uint32_t bits = __float_as_uint(y[i]) & 0x7fffffffu;
+      near = near || (bits & 0xfffffu) - 0x7fff0u <= 0x20u || (bits < 0x3c800000u && bits != 0) || bits > 0x7f800000u;
+    }
+    code = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3) |
+           (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3) << 16;
+  } else {
+    const float big = 12582912.f;
+    float t[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      t[i] = __fadd_rn(y[i], big);
+      near = near || !(fabsf(y[i] - __fadd_rn(t[i], -big)) <= 0.4999f);
+    }
+    code = __byte_perm(__byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040), __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040), 0x5410);
+  }
+  if (near)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t c = code_of<E4M3>(__fdiv_rn(x[i], s));
+      code = i == 0 ? c : code | c << (8 * i);
+    }
+  return code;
 }
 
 // A thread has PIECES pieces of 8 columns of a block.
@@ -67,14 +104,20 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const AppendParams p) {
     const float s = top >= 0x7f80u ? __int_as_float(0x7fc00000) : __fdiv_rn(__uint_as_float(top << 16), E4M3 ? 448.f : 127.f);
     if (threadIdx.x == 0) (side ? p.c.vs : p.c.ks)[head * (p.c.C / KV8_BLOCK) + m] = s;
     uint2* codes = reinterpret_cast<uint2*>((side ? p.c.v8 : p.c.k8) + (head * p.c.C + base) * P);
+    // 1 / s is a normal number, or the block is zero throughout, reads as NaN whatever its codes, or is too small to be told from zero
+    // in products: then divisions
+    const float inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
+    const bool tiny = s > 0.f && s < 1e-36f;
 #pragma unroll
     for (int e = 0; e < PIECES; ++e) {
       const uint32_t* w = &z[e].x;
       uint32_t o[2];
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-        o[k] = code_of<E4M3>(__uint_as_float(w[2 * k] << 16), s) | code_of<E4M3>(__uint_as_float(w[2 * k] & 0xffff0000u), s) << 8 |
-               code_of<E4M3>(__uint_as_float(w[2 * k + 1] << 16), s) << 16 | code_of<E4M3>(__uint_as_float(w[2 * k + 1] & 0xffff0000u), s) << 24;
+      for (int k = 0; k < 2; ++k) {
+        const float x[4] = {__uint_as_float(w[2 * k] << 16), __uint_as_float(w[2 * k] & 0xffff0000u), __uint_as_float(w[2 * k + 1] << 16),
+                            __uint_as_float(w[2 * k + 1] & 0xffff0000u)};
+        o[k] = s > 0.f ? codes_of<E4M3>(x, s, tiny ? __int_as_float(0x7fc00000) : inv) : 0u;
+      }
       codes[threadIdx.x + 256 * e] = make_uint2(o[0], o[1]);
     }
   }
@@ -131,11 +174,16 @@ __global__ void __launch_bounds__(256) kv8_expand_kernel(const ExpandParams p) {
     if (full) {
       const uint2 c = codes[i];
       float x[8];
+      if constexpr (E4M3) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const uint32_t byte = ((k < 4 ? c.x : c.y) >> (8 * (k & 3))) & 0xffu;
-        if constexpr (E4M3) x[k] = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));
-        else x[k] = (float)(int8_t)byte;
+        for (int k = 0; k < 4; ++k) {
+          const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((k < 2 ? c.x : c.y) >> (16 * (k & 1))), __NV_E4M3);
+          const float2 y = __half22float2(__half2(r));
+          x[2 * k] = y.x, x[2 * k + 1] = y.y;
+        }
+      } else {  // code + 128 in the last bits of 2^23 + ..
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = __uint_as_float(__byte_perm((k < 4 ? c.x : c.y) ^ 0x80808080u, 0x4b000000u, 0x7440 | (k & 3))) - 8388736.f;
       }
       uint32_t* w = &z.x;
 #pragma unroll

@@ -64,6 +64,15 @@ def test_attention_refuses(bad):
         ops.attention(q.to(bad.get("dtype", q.dtype)), k, v, **bad.get("how", {}))
 
 
+@pytest.mark.parametrize("scale", [1e-40, 1e38, float("inf")])
+def test_scales_that_are_no_numbers_in_32_bits_are_refused(scale):
+    q = rand(1, 3, 2, 8)
+    with pytest.raises(ValueError, match="scale"):
+        ops.attention(q, q, q, scale=scale)
+    with pytest.raises(ValueError, match="scale"):
+        ops.kv8_attention(q.bfloat16(), ops.kv8_cache(1, 2, 64, 8), 0, scale=scale)
+
+
 def rows(*shape, seed=0):
     x = rand(*shape, seed=seed)
     x[..., 1] *= 7.0

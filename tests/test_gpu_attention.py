@@ -71,6 +71,13 @@ def test_positions_given_as_numbers_and_on_the_device(start):
         check(qkv, grad, start=torch.tensor([start, start // 2], device="cuda"), window=31)
 
 
+@pytest.mark.parametrize("window", [2 ** 31 - 1000, 2 ** 31 - 100, 2 ** 31 + 50, 2 ** 40, 2 ** 62])
+def test_windows_as_far_as_positions(window):
+    qkv, grad = make(2, 70, 200, 2, 1, 64, seed=3)
+    got = check(qkv, grad, start=torch.tensor([2 ** 31, 2 ** 31 + 7], device="cuda"), window=window)
+    assert got["o"].any() == (window > 2 ** 31 - 200)  # the first query sees the keys j > 2^31 - window, of 200
+
+
 def test_scale_is_the_callers():
     check(*make(1, 150, 150, 2, 2, 64, seed=4), scale=0.7)
 

@@ -204,6 +204,18 @@ def test_idle_sequences_and_tokens_past_the_capacity_leave_the_rest_alone(kind, 
     assert all(torch.equal(before[n][2], t[2]) for n, t in bits(cache).items())
 
 
+@pytest.mark.parametrize("T", [1, 5, 100])
+def test_idle_by_a_number_and_bounds_beyond_what_is_held(T):
+    cache, k, v = filled(2, 2, 64, 100, "int8", capacity=512)
+    before = {n: t.clone() for n, t in bits(cache).items()}
+    q, nk, nv = rows(2, T, 4, 64, 3, False), rows(2, T, 2, 64, 4), rows(2, T, 2, 64, 5)
+    assert not ops.kv8_attention(q, cache, -3, nk, nv).any() and all(torch.equal(before[n], t) for n, t in bits(cache).items())
+    pad = torch.zeros(2, T, 4, 136, device="cuda", dtype=torch.bfloat16)  # rows whose addresses are no multiples of 16 bytes: copied
+    copies = [pad[:, :, : x.shape[2], 3:67].copy_(x) for x in (nk,)] + [nv.clone()]
+    out = ops.kv8_attention(q, {n: t.clone() for n, t in cache.items()}, 100, *copies, most=512)
+    assert torch.equal(out, ops.kv8_attention(q, cache, 100, nk, nv))
+
+
 @pytest.mark.parametrize("what", [float("nan"), float("inf")])
 def test_tokens_that_are_no_numbers(what):
     for T in (4, 100):

@@ -24,7 +24,7 @@ struct AttentionShape {
   int B, T, S, H, G, D;
   float scale;  // > 0
   bool causal;
-  int window;                    // 0: none
+  long long window;              // 0: none; up to 2^61
   const long long* lengths;      // [B] or null (S)
   const long long* starts;       // [B] or null (`start` for all)
   long long start;

@@ -53,7 +53,7 @@ tb::AttentionShape shape_of(const Tensor& q, const Tensor& k, const Tensor& v, d
   TORCH_CHECK(G > 0 && H % G == 0, "attention: query heads must be a multiple of the key/value heads");
   TORCH_CHECK(T <= MOST_ROWS && S <= MOST_ROWS && q.size(0) * H < (1ll << 31), "attention: too many rows");
   TORCH_CHECK(std::isfinite(scale) && scale > 0, "attention: the scale must be positive");
-  tb::AttentionShape a{(int)q.size(0), (int)T, (int)S, (int)H, (int)G, (int)D, (float)scale, causal, (int)std::min<int64_t>(window, 1 << 30)};
+  tb::AttentionShape a{(int)q.size(0), (int)T, (int)S, (int)H, (int)G, (int)D, (float)scale, causal, std::min<int64_t>(window, 1ll << 61)};
   a.lengths = numbers(lengths, a.B, q, "key_lengths");
   a.starts = numbers(starts, a.B, q, "query_start");
   a.start = start;
@@ -93,11 +93,11 @@ void check_rows(const tb::Kv8Cache& c, const Tensor& x, int64_t heads, const cha
   TORCH_CHECK(x.size(1) < (1ll << 30), "kv8: too many tokens");
 }
 
-void append_rows(const tb::Kv8Cache& c, const Tensor& k, const Tensor& v, const tb::Kv8Pos& pos) {
+// `held`: copies that have to live until all that may run beside the append is launched; their memory is handed out again from then on
+void append_rows(const tb::Kv8Cache& c, const Tensor& k, const Tensor& v, const tb::Kv8Pos& pos, Tensor (&held)[2]) {
   check_rows(c, k, c.G, "keys");
   TORCH_CHECK(v.sizes() == k.sizes(), "kv8: keys and values differ in shape");
-  Tensor hk, hv;
-  const tb::AttentionView kv = view_of(k, k, "keys", hk), vv = view_of(v, k, "values", hv);
+  const tb::AttentionView kv = view_of(k, k, "keys", held[0]), vv = view_of(v, k, "values", held[1]);
   if (k.numel() > 0) tb::launch_kv8_append(c, kv, vv, (int)k.size(1), (int)k.size(3), pos, cur_stream());
 }
 
@@ -209,7 +209,8 @@ void kv8_append(const Tensor& k8, const Tensor& v8, const Tensor& ks, const Tens
                 int64_t host, const OptTensor& dev) {
   const tb::Kv8Cache c = cache_of(k8, v8, ks, vs, kt, vt, k);
   c10::cuda::CUDAGuard guard(k.device());
-  append_rows(c, k, v, pos_of(host, dev, c.B, k));
+  Tensor held[2];
+  append_rows(c, k, v, pos_of(host, dev, c.B, k), held);
 }
 
 // -> k, v [B, G, rows, D]
@@ -235,7 +236,7 @@ Tensor kv8_attention(const Tensor& k8, const Tensor& v8, const Tensor& ks, const
   c10::cuda::CUDAGuard guard(q.device());
   tb::Kv8Attention a{};
   a.c = c;
-  Tensor hq, part;
+  Tensor hq, held[2], part;
   a.q = view_of(q, q, "queries", hq);
   a.T = (int)q.size(1);
   a.H = (int)q.size(2);
@@ -247,10 +248,11 @@ Tensor kv8_attention(const Tensor& k8, const Tensor& v8, const Tensor& ks, const
   if (has(k)) {
     TORCH_CHECK(has(v) && k->dim() == 4 && k->size(1) == q.size(1) && k->size(3) == q.size(3) && k->get_device() == q.get_device(),
                 "kv8: new keys and values come with the queries' tokens");
-    append_rows(c, *k, *v, a.pos);
+    append_rows(c, *k, *v, a.pos, held);
     a.appended = k->numel() > 0;
   }
   if (q.numel() == 0) return torch::empty(q.sizes(), q.options());
+  if (a.pos.dev == nullptr && host < 0) return torch::zeros(q.sizes(), q.options());  // idle
   if (a.T * (a.H / c.G) < PORTION) {
     out = torch::empty(q.sizes(), q.options());
     a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());

@@ -19,21 +19,23 @@ __device__ __forceinline__ T uniform(T x) {
 }
 
 struct Visible {  // of one sequence
-  int start, length, window;
-  bool causal;
-  __device__ __forceinline__ Visible(const AttentionShape& a, int b) : window(a.window), causal(a.causal) {
+  int start, before, length;  // before: what a query's first visible key is ahead of its number
+  bool causal, window;
+  __device__ __forceinline__ Visible(const AttentionShape& a, int b) : causal(a.causal), window(a.window > 0) {
     // positions past these limits see what those at the limits see
-    const long long s0 = a.starts != nullptr ? a.starts[b] : a.start, lim = 1ll << 30;
+    const long long lim = 1ll << 30, far = 1ll << 61, given = a.starts != nullptr ? a.starts[b] : a.start;
+    const long long s0 = given < -far ? -far : given > far ? far : given, w0 = s0 - a.window + 1;
     start = uniform((int)(s0 < -lim ? -lim : s0 > lim ? lim : s0));
+    before = uniform((int)(w0 < -lim ? -lim : w0 > lim ? lim : w0));
     const long long n = a.lengths != nullptr ? a.lengths[b] : a.S;
     length = uniform((int)(n < 0 ? 0 : n > a.S ? a.S : n));
   }
   // keys low(t) .. high(t) are visible to query t; both grow with t
-  __device__ __forceinline__ int low(int t) const { return window > 0 ? max(0, start + t - window + 1) : 0; }
+  __device__ __forceinline__ int low(int t) const { return window ? max(0, before + t) : 0; }
   __device__ __forceinline__ int high(int t) const { return causal ? min(length - 1, start + t) : length - 1; }
   // queries first(j) .. last(j, T) see key j
   __device__ __forceinline__ int first(int j) const { return causal ? max(0, j - start) : 0; }
-  __device__ __forceinline__ int last(int j, int T) const { return window > 0 ? (int)min((long long)T - 1, (long long)j + window - 1 - start) : T - 1; }
+  __device__ __forceinline__ int last(int j, int T) const { return window ? min(T - 1, j - before) : T - 1; }
   // tiles [x, y) of keys that queries t0 .. t1 see
   __device__ __forceinline__ int2 tiles(int t0, int t1) const {
     const int lo = low(t0), hi = high(t1);

@@ -6,7 +6,6 @@ in :mod:`triune_b200.ops.reference`. This is the role of the library call in the
 
 from __future__ import annotations
 
-import math
 from typing import Any, Mapping, Optional, Tuple, Union
 
 import torch
@@ -35,8 +34,8 @@ def _shapes(q, k, v) -> None:
 
 def _scale(scale: Optional[float], D: int) -> float:
     scale = D ** -0.5 if scale is None else float(scale)
-    if not (math.isfinite(scale) and scale > 0):
-        raise ValueError(f"the scale of the scores must be positive, got {scale}")
+    if not 1e-30 <= scale <= 1e30:  # an fp32 number, also times log2(e)
+        raise ValueError(f"the scale of the scores must be positive (1e-30 to 1e30), got {scale}")
     return scale
 
 
@@ -109,7 +108,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     elif query_start is not None:
         start = int(query_start)
     if _kernels(q):
-        how = (scale, bool(causal), int(window or 0), lengths, starts, start)
+        how = (scale, bool(causal), min(int(window or 0), 1 << 61), lengths, starts, start)
         if inference_call(q, k, v):
             out, _, _ = _ext.ext().attention_fwd(q, k, v, *how, False, status_word(q.device))
             _tick()
@@ -232,7 +231,8 @@ def kv8_attention(q: torch.Tensor, cache: Mapping[str, torch.Tensor], pos: Posit
         if k.shape[1] != T or k.shape[3] != q.shape[3]:
             raise ValueError(f"new keys {tuple(k.shape)} for queries {tuple(q.shape)}")
     host, dev = _at(pos, "position", cache, T)
-    most = (codes.shape[2] if dev is not None else max(0, host + T)) if most is None else min(int(most), codes.shape[2])
+    room = codes.shape[2] if dev is not None else max(0, host + T)
+    most = room if most is None else min(int(most), room)
     if not _kv8_kernels(cache):
         if k is not None:
             ref.kv8_append(cache, k, v, host if dev is None else dev)

@@ -21,15 +21,19 @@ KV8_TYPES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
 Position = Union[int, torch.Tensor]
 
 
-def _shapes(q, k, v) -> None:
-    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
-        raise ValueError(f"attention takes queries [B, T, H, D] and keys and values [B, S, G, D], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    if q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
-        raise ValueError(f"queries {tuple(q.shape)} and keys {tuple(k.shape)} differ in batch or head size")
-    if k.shape[2] == 0 or q.shape[2] % k.shape[2]:
-        raise ValueError(f"query heads ({q.shape[2]}) must be a multiple of the key/value heads ({k.shape[2]})")
+def _shapes(q, k, v) -> Tuple[int, int, int, int]:
+    """-> B, T, S, D"""
+    qs, ks, vs = q.shape, k.shape, v.shape
+    if len(qs) != 4 or len(ks) != 4 or vs != ks:
+        raise ValueError(f"attention takes queries [B, T, H, D] and keys and values [B, S, G, D], got {tuple(qs)}, {tuple(ks)}, {tuple(vs)}")
+    (B, T, H, D), (Bk, S, G, Dk) = qs, ks
+    if B != Bk or D != Dk:
+        raise ValueError(f"queries {tuple(qs)} and keys {tuple(ks)} differ in batch or head size")
+    if G == 0 or H % G:
+        raise ValueError(f"query heads ({H}) must be a multiple of the key/value heads ({G})")
     if not q.dtype == k.dtype == v.dtype or not q.device == k.device == v.device:
         raise ValueError("queries, keys and values must have one type and device")
+    return B, T, S, D
 
 
 def _scale(scale: Optional[float], D: int) -> float:
@@ -93,9 +97,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     What keys and values past ``key_lengths`` hold does not matter, whatever it is. A value that is an infinity or NaN reaches the
     outputs of the queries that see it and of no others; gradients are not kept apart in this way. On CUDA, weights and their gradients are rounded to bf16 for
     the matrix products, sums and statistics are fp32, and results do not depend on the order in which blocks run."""
-    _shapes(q, k, v)
-    B, T, S = q.shape[0], q.shape[1], k.shape[1]
-    scale = _scale(scale, q.shape[3])
+    B, T, S, D = _shapes(q, k, v)
+    scale = _scale(scale, D)
     if window is not None and (int(window) != window or window < 1):
         raise ValueError(f"a window is a number of keys (at least 1), got {window}")
     if window is not None and not causal:
@@ -166,9 +169,10 @@ def _at(pos: Position, name: str, cache, tokens: int = 0) -> Tuple[int, Optional
 
 def _new_rows(cache, k, v) -> None:
     codes = cache["k8"]
-    if k.dim() != 4 or v.shape != k.shape or k.shape[0] != codes.shape[0] or k.shape[2] != codes.shape[1] or k.shape[3] > codes.shape[3] or k.shape[3] % 8:
-        raise ValueError(f"keys and values [B, T, G, D] that fit a cache of codes {tuple(codes.shape)}, got {tuple(k.shape)} and {tuple(v.shape)}")
-    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or k.device != codes.device or v.device != codes.device:
+    cs, ks, vs, device = codes.shape, k.shape, v.shape, codes.device
+    if len(ks) != 4 or vs != ks or ks[0] != cs[0] or ks[2] != cs[1] or ks[3] > cs[3] or ks[3] % 8:
+        raise ValueError(f"keys and values [B, T, G, D] that fit a cache of codes {tuple(cs)}, got {tuple(ks)} and {tuple(vs)}")
+    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or k.device != device or v.device != device:
         raise ValueError("keys and values of an 8-bit cache are bfloat16 on the cache's device")
 
 
@@ -218,20 +222,22 @@ def kv8_attention(q: torch.Tensor, cache: Mapping[str, torch.Tensor], pos: Posit
 
     Idle sequences (negative positions) give zeros; a query past the capacity (positions on the device only) gives NaN."""
     codes = cache["k8"]
-    if q.dim() != 4 or q.shape[0] != codes.shape[0] or q.shape[2] % codes.shape[1] or q.shape[3] > codes.shape[3] or q.shape[3] % 8 or q.shape[3] < 8:
-        raise ValueError(f"queries [B, T, H, D] that fit a cache of codes {tuple(codes.shape)}, got {tuple(q.shape)}")
+    cs, qs = codes.shape, q.shape
+    if len(qs) != 4 or qs[0] != cs[0] or qs[2] % cs[1] or qs[3] > cs[3] or qs[3] % 8 or qs[3] < 8:
+        raise ValueError(f"queries [B, T, H, D] that fit a cache of codes {tuple(cs)}, got {tuple(qs)}")
     if q.dtype != torch.bfloat16 or q.device != codes.device:
         raise ValueError("queries of an 8-bit cache are bfloat16 on the cache's device")
     if (k is None) != (v is None):
         raise ValueError("new keys come with new values")
     _no_gradients(q, k, v)
-    scale, T = _scale(scale, q.shape[3]), q.shape[1]
+    scale, T = _scale(scale, qs[3]), qs[1]
     if k is not None:
         _new_rows(cache, k, v)
-        if k.shape[1] != T or k.shape[3] != q.shape[3]:
-            raise ValueError(f"new keys {tuple(k.shape)} for queries {tuple(q.shape)}")
+        ks = k.shape
+        if ks[1] != T or ks[3] != qs[3]:
+            raise ValueError(f"new keys {tuple(ks)} for queries {tuple(qs)}")
     host, dev = _at(pos, "position", cache, T)
-    room = codes.shape[2] if dev is not None else max(0, host + T)
+    room = cs[2] if dev is not None else max(0, host + T)
     most = room if most is None else min(int(most), room)
     if not _kv8_kernels(cache):
         if k is not None:

@@ -202,6 +202,19 @@ def test_the_same_bits_every_time_on_another_stream_and_in_a_graph():
     assert all(torch.equal(a, b) for a, b in zip(graphs[0][1], call()))
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("window", [5, 64, None])
+def test_the_same_bits_however_warps_run_ahead(D, window):
+    """Many short walks over keys, most of whose tiles are masked for some rows: warps that differ in speed."""
+    (q, k, v), grad = make(40, 512, 512, 4, 4, D, seed=12)
+    out = ops.attention(q, k, v, window=window)
+    first = torch.autograd.grad(out, (q, k, v), grad, retain_graph=True)
+    assert all(torch.isfinite(x).all() for x in first)
+    for _ in range(60):
+        again = torch.autograd.grad(out, (q, k, v), grad, retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
 @pytest.mark.parametrize("shape", [(0, 4, 4, 2, 1, 64), (2, 0, 5, 2, 1, 64), (2, 5, 0, 2, 1, 64)])
 def test_nothing_to_attend(shape):
     qkv, grad = make(*shape)

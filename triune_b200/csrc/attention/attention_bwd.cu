@@ -45,9 +45,9 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   uint8_t *sQ = smem, *sG = sQ + TILE, *sK = sG + TILE, *sV = sK + NK * TILE;  // G: dO
-  __shared__ __align__(8) uint64_t bars[10 + 2 * NK + 2 * NV];
+  __shared__ __align__(8) uint64_t bars[11 + 2 * NK + 2 * NV];
   uint64_t *q_full = bars, *s_full = bars + 1, *s_read = bars + 2, *dp_full = bars + 3, *dp_next = bars + 4, *ds_ready = bars + 5, *done = bars + 6,
-           *k_clean = bars + 7, *end_full = bars + 8, *k_full = bars + 10, *k_empty = k_full + NK, *v_full = k_empty + NK, *v_empty = v_full + NV;
+           *k_clean = bars + 7, *end_full = bars + 8, *ds_next = bars + 9, *k_full = bars + 11, *k_empty = k_full + NK, *v_full = k_empty + NK, *v_empty = v_full + NV;
   __shared__ uint32_t tmem_slot;
   __shared__ float part[AT_M];
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -74,6 +74,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
     mbar_init(s_read, 256);
     mbar_init(dp_full, 1);
     mbar_init(ds_ready, 256);
+    mbar_init(ds_next, 256);
     mbar_init(done, 1);
     mbar_init(k_clean, 64);
     mbar_init(end_full, 1);
@@ -142,7 +143,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
       if (ok) {
         for (int u = 0; u < n && ok; ++u) {
           if (u + 1 < n) ok = warp_wait(s_read, u & 1) && scores(u + 1);  // the other dP columns were read by the product before
-          ok = ok && warp_wait(ds_ready, u & 1);
+          ok = ok && warp_wait(u & 1 ? ds_next : ds_ready, (u >> 1) & 1);
           if (!ok) break;
           tc_fence_after_sync();
           issue([&] {
@@ -251,7 +252,8 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
       slopes(y, 32);
       tmem_st_wait();
       tc_fence_before_sync();
-      mbar_arrive(ds_ready);
+      // a warp may be done with the next tile before another is with this one: each of the two sets has its barrier
+      mbar_arrive(u & 1 ? ds_next : ds_ready);
       return true;
     };
     for (int u = 0; u < n; ++u) {

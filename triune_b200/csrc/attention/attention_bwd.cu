@@ -5,13 +5,16 @@
 // Two kernels, each of which keeps its sums in TMEM and writes every gradient once: one per 128 queries (dQ; it also forms delta),
 // one per 128 keys (dK, dV). S and dP are formed in both, so there are seven tile products instead of the five of a kernel that
 // adds dQ up in global memory: no atomics, the same bits every time, no fp32 copy of dQ.
-// Both: warp 0 TMA producer, warp 1 tcgen05.mma, warps 4-11 softmax; a thread has one row and half of its 128 columns, and keeps
+// Both: warp 0 TMA producer, warp 1 tcgen05.mma, the warps from 4 on softmax; a thread has 64 columns of one row, and keeps
 // the fp32 probabilities in registers between S and dP. P and dS are rounded to bf16 for the products (2^-8 of each term at
 // most, which averages out over the sums); dS is formed from the unrounded P.
-// The next tile's scores are formed as soon as these are in registers, where they have the room. dQ has two sets of columns for dP (dS over it), so that a
-// tile's dP need not wait for the product with the last one's dS. For dK and dV, P has columns of its own with heads of up to 64;
-// with wider ones it lies over S, and the next scores come behind the product with P (P through shared memory, to have them earlier,
-// left no room for a third stage of query tiles: 2911 clocks a tile instead of 2500, waiting for these).
+// For dQ the next tile's scores are formed as soon as these are in registers, and there are two sets of columns for dP (dS over it), so that
+// a tile's dP need not wait for the product with the last one's dS. For dK and dV, P lies over S, and the next scores come behind
+// the product with P unless P has columns of its own (P through shared memory, to have them earlier, left no room for a third stage of
+// query tiles with heads of 128: 2911 clocks a tile instead of 2500, waiting for these).
+// Bound by the chain from scores to slopes and, with heads of 128, by the products (1.26 and 1.37 PFLOP/s). With a cold L2, dQ and dK, dV:
+// 8192 tokens, 16 heads on 4 of 128, causal: 332 and 407 us, of which the last 50 have SMs without work (the first keys' tile of a shared
+// head is seen by 256 query tiles, the mean of an SM is 225).
 #include <type_traits>
 
 #include "../common/per_device.h"
@@ -20,7 +23,12 @@
 namespace tb {
 namespace {
 
-constexpr int BW_THREADS = 384;
+// TWO: tiles have 64 rows along the axis that is walked (keys for dQ, queries for dK and dV) instead of 128, four softmax warps instead of eight,
+// and two CTAs share an SM, each with half of the tensor memory: one's exponentials run under the other's products, loads and stores.
+// Wider heads' tiles and sums do not fit twice.
+__host__ __device__ constexpr int bwd_tile(bool two) { return two ? 64 : 128; }
+__host__ __device__ constexpr int bwd_threads(bool two) { return 128 + 2 * bwd_tile(two); }
+constexpr int BW_FEW = 56, BW_MANY = 200;  // registers of a thread of the first four warps and of the others, of 128 each at launch
 
 struct BwdParams {
   AttentionShape a;
@@ -32,19 +40,20 @@ struct BwdParams {
   int* status;
 };
 
-// TMEM column of step k of a 128 x 128 bf16 operand: two halves of 64 values, each in the first 32 columns of its 64
+// TMEM column of step k of a 128 x 128 (or 64) bf16 operand: halves of 64 values, each in the first 32 columns of its 64
 __device__ __forceinline__ int half_column(int k) { return (k >> 2) * 64 + (k & 3) * 8; }
 
 // ---------------------------------------------------------------------------------------------------------------- queries
-template <int DB>
-__global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
+template <int DB, bool TWO>
+__global__ void __launch_bounds__(bwd_threads(TWO), TWO ? 2 : 1) attention_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
                                                                      const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                                                                      const BwdParams p) {
   // K is held until the product with dS, V only until dP is there: longer and shorter rings
-  constexpr int TILE = DB * AT_BOX, NK = DB == 1 ? 4 : 3, NV = DB == 1 ? 3 : 2;
+  constexpr int BN = bwd_tile(TWO), HALVES = BN / 64, BOX = BN * 128, TILE = DB * AT_BOX, KTILE = DB * BOX, NK = DB == 1 ? 4 : 3, NV = DB == 1 ? 3 : 2;
+  constexpr uint32_t P_AT = BN, Q_AT = 3 * BN, COLUMNS = 4 * BN;  // TMEM columns: S 0 .., dP (dS over it) twice, the sums
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  uint8_t *sQ = smem, *sG = sQ + TILE, *sK = sG + TILE, *sV = sK + NK * TILE;  // G: dO
+  uint8_t *sQ = smem, *sG = sQ + TILE, *sK = sG + TILE, *sV = sK + NK * KTILE;  // G: dO
   __shared__ __align__(8) uint64_t bars[11 + 2 * NK + 2 * NV];
   uint64_t *q_full = bars, *s_full = bars + 1, *s_read = bars + 2, *dp_full = bars + 3, *dp_next = bars + 4, *ds_ready = bars + 5, *done = bars + 6,
            *k_clean = bars + 7, *end_full = bars + 8, *ds_next = bars + 9, *k_full = bars + 11, *k_empty = k_full + NK, *v_full = k_empty + NK, *v_empty = v_full + NV;
@@ -54,11 +63,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
   const int h = blockIdx.x % p.a.H, b = blockIdx.x / p.a.H, kvh = h / (p.a.H / p.a.G);
   const int q0 = (gridDim.y - 1 - blockIdx.y) * AT_M;
   const Visible vis(p.a, b);
-  const int2 range = vis.tiles(q0, min(p.a.T, q0 + AT_M) - 1);
+  const int2 range = vis.tiles(q0, min(p.a.T, q0 + AT_M) - 1, BN);
   const int n = range.y - range.x;
   // the tile, if any, in which the sequence ends before the tile does: its other keys may hold anything and are set to zero. It is
   // the last of all and has barriers of its own, whose only phase the warps that wait for nothing else cannot miss.
-  const int ragged = vis.length % AT_M != 0 && vis.length < p.a.S ? vis.length / AT_M - range.x : -1;
+  const int ragged = vis.length % BN != 0 && vis.length < p.a.S ? vis.length / BN - range.x : -1;
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -71,10 +80,10 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
       mbar_init(v_empty + i, 1);
     }
     mbar_init(s_full, 1);
-    mbar_init(s_read, 256);
+    mbar_init(s_read, 128 * HALVES);
     mbar_init(dp_full, 1);
-    mbar_init(ds_ready, 256);
-    mbar_init(ds_next, 256);
+    mbar_init(ds_ready, 128 * HALVES);
+    mbar_init(ds_next, 128 * HALVES);
     mbar_init(done, 1);
     mbar_init(k_clean, 64);
     mbar_init(end_full, 1);
@@ -82,13 +91,14 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
     mbar_fence_init();
   }
   if (warp == 2) {
-    tmem_alloc(&tmem_slot, 512);
+    tmem_alloc(&tmem_slot, COLUMNS);
     tmem_relinquish();
   }
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = uniform(tmem_slot);
 
+  if (warp < 4) {
   if (warp == 0) {
     if (lane == 0 && n > 0) {
       prefetch_tmap(&tmQ);
@@ -107,10 +117,10 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
         if (u >= NK) ok = mbar_wait(k_empty + ks, ((u / NK) & 1) ^ 1);
         if (u >= NV) ok = ok && mbar_wait(v_empty + vs, ((u / NV) & 1) ^ 1);
         if (!ok) break;
-        mbar_expect_tx(kf, u == ragged ? 2 * TILE : TILE);
-        if (u != ragged) mbar_expect_tx(vf, TILE);
-        for (int d = 0; d < DB; ++d) tma_load_4d(sK + ks * TILE + d * AT_BOX, &tmK, kf, d * 64, (range.x + u) * AT_M, kvh, b);
-        for (int d = 0; d < DB; ++d) tma_load_4d(sV + vs * TILE + d * AT_BOX, &tmV, vf, d * 64, (range.x + u) * AT_M, kvh, b);
+        mbar_expect_tx(kf, u == ragged ? 2 * KTILE : KTILE);
+        if (u != ragged) mbar_expect_tx(vf, KTILE);
+        for (int d = 0; d < DB; ++d) tma_load_4d(sK + ks * KTILE + d * BOX, &tmK, kf, d * 64, (range.x + u) * BN, kvh, b);
+        for (int d = 0; d < DB; ++d) tma_load_4d(sV + vs * KTILE + d * BOX, &tmV, vf, d * 64, (range.x + u) * BN, kvh, b);
       }
       // nothing may arrive once the block is gone
       for (int u = max(0, n - NK); u < n && ok; ++u) ok = mbar_wait(k_empty + u % NK, (u / NK) & 1);
@@ -128,12 +138,12 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
         if (!(u == ragged ? warp_wait(end_full, 0) && warp_wait(k_clean, 0) : warp_wait(k_full + ks_at, (u / NK) & 1))) return false;
         tc_fence_after_sync();
         issue([&] {
-          scores_product<DB>(tmem, q, k + ks_at * TILE, ks);
+          scores_product<DB, BN>(tmem, q, k + ks_at * KTILE, ks);
           umma_commit(s_full);
         });
         if (u != ragged && !warp_wait(v_full + vs_at, (u / NV) & 1)) return false;
         issue([&] {
-          scores_product<DB>(tmem + 128 + (u & 1) * 128, g, v + vs_at * TILE, ks);
+          scores_product<DB, BN>(tmem + P_AT + (u & 1) * BN, g, v + vs_at * KTILE, ks);
           umma_commit(u & 1 ? dp_next : dp_full);  // one for each set of columns
           umma_commit(v_empty + vs_at);
         });
@@ -147,7 +157,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
           if (!ok) break;
           tc_fence_after_sync();
           issue([&] {
-            rows_product<DB, 0, 8>(tmem + 384, tmem + 128 + (u & 1) * 128, k + u % NK * TILE, u > 0, half_column);
+            rows_product<DB, 0, BN / 16>(tmem + Q_AT, tmem + P_AT + (u & 1) * BN, k + u % NK * KTILE, u > 0, half_column);
             umma_commit(k_empty + u % NK);
           });
         }
@@ -155,17 +165,18 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
       }
       if (!ok && p.status) *p.status = ST_TIMEOUT_FULL;
     }
-  } else if (warp < 4) {
+  } else {
     if (ragged >= 0 && ragged < n) {
-      const int s = ragged % NK, keep = vis.length % AT_M;
+      const int s = ragged % NK, keep = vis.length % BN;
       const bool ok = mbar_wait(end_full, 0);
       if (ok)
-        for (int i = threadIdx.x - 64; i < TILE / 16; i += 64)
-          if (((i >> 3) & (AT_M - 1)) >= keep) reinterpret_cast<uint4*>(sK + s * TILE)[i] = make_uint4(0, 0, 0, 0);
+        for (int i = threadIdx.x - 64; i < KTILE / 16; i += 64)
+          if (((i >> 3) & (BN - 1)) >= keep) reinterpret_cast<uint4*>(sK + s * KTILE)[i] = make_uint4(0, 0, 0, 0);
       fence_proxy_async_smem();
       mbar_arrive(k_clean);
       if (!ok && p.status) *p.status = ST_TIMEOUT_FULL;
     }
+  }
   } else {
     const int half = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane, t = q0 + row;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
@@ -173,13 +184,13 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
     const int padded = (p.a.T + AT_M - 1) / AT_M * AT_M;
     const long long at = ((long long)b * p.a.H + h) * padded + t;
     const float lse = p.lse[at];
-    // delta: each half of the row's columns by one of its two threads
+    // delta: its share of the row's columns by each of the row's threads
     float dot = 0.f;
     if (t < p.a.T) {
       const uint4* o = reinterpret_cast<const uint4*>((const __nv_bfloat16*)p.out.p + b * p.out.sb + t * p.out.sr + h * p.out.sh);
       const uint4* l = reinterpret_cast<const uint4*>((const __nv_bfloat16*)p.rest.p + b * p.rest.sb + t * p.rest.sr + h * p.rest.sh);
       const uint4* g = reinterpret_cast<const uint4*>((const __nv_bfloat16*)p.dout.p + b * p.dout.sb + t * p.dout.sr + h * p.dout.sh);
-      const int pieces = p.a.D / 8, mid = (pieces + 1) / 2;
+      const int pieces = p.a.D / 8, mid = (pieces + HALVES - 1) / HALVES;
       for (int i = half * mid; i < (half == 0 ? mid : pieces); ++i) {
         const uint4 x = o[i], y = g[i], z = l[i];
         const uint32_t *xp = &x.x, *yp = &y.x, *zp = &z.x;
@@ -190,22 +201,22 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
         }
       }
     }
-    if (half == 1) part[row] = dot;
-    named_barrier<256>(1);
-    if (half == 0) {
-      dot += part[row];
-      part[row] = dot;
-      p.delta[at] = -dot;
+    if constexpr (HALVES == 2) {
+      if (half == 1) part[row] = dot;
+      named_barrier<256>(1);
+      if (half == 0) part[row] += dot;
+      named_barrier<256>(1);
+      dot = part[row];
     }
-    named_barrier<256>(1);
-    const float delta = -part[row];
+    const float delta = -dot;
+    if (half == 0) p.delta[at] = delta;
     const int lo = vis.low(t), hi = vis.high(t);
     bool ok = true;
     const uint64_t cc = pack_f2(p.scale2, p.scale2), mm = pack_f2(lse, lse), dd = pack_f2(delta, delta);
     // MASKED: not all keys of the tile are visible to all queries. Invisible ones have weight and slope zero, whatever they hold.
     auto tile = [&](auto some, int u, int c_lo, int c_hi) {
       constexpr bool MASKED = decltype(some)::value;
-      const uint32_t tP = tS + 128 + (u & 1) * 128;
+      const uint32_t tP = tS + P_AT + (u & 1) * BN;
       uint32_t x[32], y[32];
       tmem_load(tS, x, y);
       tc_fence_before_sync();
@@ -257,22 +268,22 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
       return true;
     };
     for (int u = 0; u < n; ++u) {
-      const int key = (range.x + u) * AT_M;
+      const int key = (range.x + u) * BN;
       ok = warp_wait(s_full, u & 1);
       if (!ok) break;
       tc_fence_after_sync();
-      if (vis.whole(q0, q0 + AT_M - 1, key)) ok = tile(std::false_type{}, u, 0, 0);
+      if (vis.whole(q0, q0 + AT_M - 1, key, BN)) ok = tile(std::false_type{}, u, 0, 0);
       else ok = tile(std::true_type{}, u, lo - key - half * 64, hi - key - half * 64);
       if (!ok) break;
     }
     if (ok && n > 0) ok = warp_wait(done, 0);
     tc_fence_after_sync();
     __nv_bfloat16* o = p.dq + (((long long)b * p.a.T + t) * p.a.H + h) * p.a.D;
-    for (int c = half * 32 * DB; c < (half + 1) * 32 * DB; c += 16) {
+    for (int c = half * 32 * DB; c < (half + 1) * (64 / HALVES) * DB; c += 16) {
       uint32_t v[16] = {};
       if (n > 0) {
         __syncwarp();
-        tmem_load(tmem + lane_base + 384 + c, v);
+        tmem_load(tmem + lane_base + Q_AT + c, v);
       }
       if (t < p.a.T) store_row16(o, c, p.a.D, v, n > 0 ? p.a.scale : 0.f);
     }
@@ -282,25 +293,26 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dq_kernel(const __gri
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  if (warp == 2) tmem_dealloc(tmem, 512);
+  if (warp == 2) tmem_dealloc(tmem, COLUMNS);
 }
 
 // ---------------------------------------------------------------------------------------------------------------- keys, values
 // Stages of query tiles: what shared memory holds
-__host__ __device__ constexpr int key_stages(int db) { return db == 1 ? 3 : 2; }
+__host__ __device__ constexpr int key_stages(int db, bool two) { return two ? 4 : db == 1 ? 3 : 2; }
 
-template <int DB>
-__global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
+template <int DB, bool TWO>
+__global__ void __launch_bounds__(bwd_threads(TWO), TWO ? 2 : 1) attention_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
                                                                       const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                                                                       const BwdParams p) {
-  constexpr int TILE = DB * AT_BOX, STATS = 2 * AT_M * 4, NQ = key_stages(DB);  // lse and delta of a query tile
-  // TMEM columns: S 0-127, dP (dS over it) 128-255, P where it fits (APART, else over S), and the sums
-  constexpr bool APART = DB == 1;
-  constexpr uint32_t P_AT = 256, V_AT = APART ? 384 : 256, K_AT = APART ? 448 : 384;
+  constexpr int BN = bwd_tile(TWO), HALVES = BN / 64, BOX = BN * 128, TILE = DB * AT_BOX, QTILE = DB * BOX, NQ = key_stages(DB, TWO);
+  constexpr int STATS = 2 * BN * 4;  // lse and delta of a query tile
+  // TMEM columns: S 0 .., dP (dS over it), weights where they fit (APART, else over S), and the sums
+  constexpr bool APART = DB == 1 && !TWO;
+  constexpr uint32_t D_AT = BN, W_AT = APART ? 2 * BN : 0, V_AT = APART ? 3 * BN : 2 * BN, K_AT = V_AT + 64 * DB, COLUMNS = 4 * BN;
   extern __shared__ __align__(1024) uint8_t smem[];  // no other shared memory: it starts on a tile's boundary, which is looked at below
-  uint8_t *sK = smem, *sV = sK + TILE, *sQ = sV + TILE, *sG = sQ + NQ * TILE;
-  float* sStat = reinterpret_cast<float*>(sG + NQ * TILE);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sStat + NQ * 2 * AT_M);
+  uint8_t *sK = smem, *sV = sK + TILE, *sQ = sV + TILE, *sG = sQ + NQ * QTILE;
+  float* sStat = reinterpret_cast<float*>(sG + NQ * QTILE);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sStat + NQ * 2 * BN);
   uint64_t *kv_full = bars, *s_full = bars + 1, *p_ready = bars + 2, *dp_full = bars + 3, *ds_ready = bars + 4, *done = bars + 5, *s_read = bars + 6,
            *p_free = bars + 7, *q_full = bars + 8, *q_empty = q_full + NQ;
   uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(q_empty + NQ);
@@ -313,7 +325,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
   const int k0 = blockIdx.y * AT_M;  // with a causal mask the first keys are seen by the most queries
   const Visible vis(p.a, b);
   const int first = vis.first(k0), last = vis.last(min(p.a.S, k0 + AT_M) - 1, p.a.T);
-  const int i0 = first / AT_M, per = k0 < vis.length && last >= first ? last / AT_M + 1 - i0 : 0, n = per * rep;
+  const int i0 = first / BN, per = k0 < vis.length && last >= first ? last / BN + 1 - i0 : 0, n = per * rep;
   const int padded = (p.a.T + AT_M - 1) / AT_M * AT_M;
 
   if (threadIdx.x == 0) {
@@ -323,22 +335,24 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
       mbar_init(q_empty + i, 1);
     }
     mbar_init(s_full, 1);
-    mbar_init(p_ready, 256);
+    mbar_init(p_ready, 128 * HALVES);
     mbar_init(dp_full, 1);
-    mbar_init(ds_ready, 256);
+    mbar_init(ds_ready, 128 * HALVES);
     mbar_init(done, 1);
-    mbar_init(s_read, 256);
+    mbar_init(s_read, 128 * HALVES);
     mbar_init(p_free, 1);
     mbar_fence_init();
   }
   if (warp == 2) {
-    tmem_alloc(&tmem_slot, 512);
+    tmem_alloc(&tmem_slot, COLUMNS);
     tmem_relinquish();
   }
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = uniform(tmem_slot);
 
+  if (warp < 4) {
+  if constexpr (TWO) registers_down<BW_FEW>();
   if (warp == 0) {
     if (lane == 0 && n > 0) {
       prefetch_tmap(&tmQ);
@@ -353,18 +367,18 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
       bool ok = true;
       int i = 0, head = 0;
       for (int u = 0; u < n && ok; ++u) {
-        const int s = u % NQ, h = kvh * rep + head, t0 = (i0 + i) * AT_M;
+        const int s = u % NQ, h = kvh * rep + head, t0 = (i0 + i) * BN;
         if (++i == per) i = 0, ++head;
         if (u >= NQ) ok = mbar_wait(q_empty + s, ((u / NQ) & 1) ^ 1);
         if (!ok) break;
-        mbar_expect_tx(q_full + s, 2 * TILE + STATS);
+        mbar_expect_tx(q_full + s, 2 * QTILE + STATS);
         for (int d = 0; d < DB; ++d) {
-          tma_load_4d(sQ + s * TILE + d * AT_BOX, &tmQ, q_full + s, d * 64, t0, h, b);
-          tma_load_4d(sG + s * TILE + d * AT_BOX, &tmG, q_full + s, d * 64, t0, h, b);
+          tma_load_4d(sQ + s * QTILE + d * BOX, &tmQ, q_full + s, d * 64, t0, h, b);
+          tma_load_4d(sG + s * QTILE + d * BOX, &tmG, q_full + s, d * 64, t0, h, b);
         }
         const long long at = ((long long)b * p.a.H + h) * padded + t0;
-        bulk_load(sStat + s * 2 * AT_M, p.lse + at, AT_M * 4, q_full + s);
-        bulk_load(sStat + s * 2 * AT_M + AT_M, p.delta + at, AT_M * 4, q_full + s);
+        bulk_load(sStat + s * 2 * BN, p.lse + at, BN * 4, q_full + s);
+        bulk_load(sStat + s * 2 * BN + BN, p.delta + at, BN * 4, q_full + s);
       }
       for (int u = max(0, n - NQ); u < n && ok; ++u) ok = mbar_wait(q_empty + u % NQ, (u / NQ) & 1);
       if (!ok && p.status) *p.status = ST_TIMEOUT_EMPTY;
@@ -380,13 +394,13 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
         tc_fence_after_sync();
         auto scores = [&](int u) {
           issue([&] {
-            scores_product<DB>(tmem, k, q + u % NQ * TILE, ks);
+            scores_product<DB, BN>(tmem, k, q + u % NQ * QTILE, ks);
             umma_commit(s_full);
           });
         };
         auto slopes = [&](int u) {
           issue([&] {
-            scores_product<DB>(tmem + 128, v, g + u % NQ * TILE, ks);
+            scores_product<DB, BN>(tmem + D_AT, v, g + u % NQ * QTILE, ks);
             umma_commit(dp_full);
           });
         };
@@ -405,8 +419,8 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
           if (!ok) break;
           tc_fence_after_sync();
           issue([&] {
-            if constexpr (APART) rows_product<DB, 0, 8>(tmem + V_AT, tmem + P_AT, g + s * TILE, u > 0, [](int k) { return k * 8; });
-            else rows_product<DB, 0, 8>(tmem + V_AT, tmem, g + s * TILE, u > 0, half_column);
+            if constexpr (APART) rows_product<DB, 0, BN / 16>(tmem + V_AT, tmem + W_AT, g + s * QTILE, u > 0, [](int k) { return k * 8; });
+            else rows_product<DB, 0, BN / 16>(tmem + V_AT, tmem, g + s * QTILE, u > 0, half_column);
             if (APART) umma_commit(p_free);
           });
           if (!APART && next) {  // behind the product that reads P from the same columns
@@ -418,7 +432,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
           if (!ok) break;
           tc_fence_after_sync();
           issue([&] {
-            rows_product<DB, 0, 8>(tmem + K_AT, tmem + 128, q + s * TILE, u > 0, half_column);
+            rows_product<DB, 0, BN / 16>(tmem + K_AT, tmem + D_AT, q + s * QTILE, u > 0, half_column);
             umma_commit(q_empty + s);
           });
           if (next) slopes(u + 1);  // behind the product that reads dS from the same columns
@@ -427,17 +441,19 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
       }
       if (!ok && p.status) *p.status = ST_TIMEOUT_FULL;
     }
-  } else if (warp >= 4) {
+  }
+  } else {
+    if constexpr (TWO) registers_up<BW_MANY>();
     const int half = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane, key = k0 + row;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-    const uint32_t tS = tmem + lane_base + half * 64, tP = tS + 128;
+    const uint32_t tS = tmem + lane_base + half * 64, tP = tS + D_AT;
     const bool inside = key < vis.length;
     const int lo = inside ? vis.first(key) : p.a.T, hi = inside ? vis.last(key, p.a.T) : -1;  // queries that see this key
     bool ok = true;
     const uint64_t cc = pack_f2(p.scale2, p.scale2);
     auto tile = [&](auto some, int u, int c_lo, int c_hi) {  // as for the queries
       constexpr bool MASKED = decltype(some)::value;
-      const float4 *lse = reinterpret_cast<const float4*>(sStat + u % NQ * 2 * AT_M + half * 64), *delta = lse + AT_M / 4;
+      const float4 *lse = reinterpret_cast<const float4*>(sStat + u % NQ * 2 * BN + half * 64), *delta = lse + BN / 4;
       uint32_t x[32], y[32];
       tmem_load(tS, x, y);
       tc_fence_before_sync();
@@ -467,7 +483,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
           o[i / 2] = pack_bf16x2(a[0], a[1]);
           o[i / 2 + 1] = pack_bf16x2(a[2], a[3]);
         }
-        tmem_st_32x32b_x16((APART ? tmem + lane_base + P_AT + half * 32 : tS) + c0 / 2, o);
+        tmem_st_32x32b_x16((APART ? tmem + lane_base + W_AT + half * 32 : tS) + c0 / 2, o);
       };
       weights(x, 0);
       weights(y, 32);
@@ -506,31 +522,33 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
       return true;
     };
     for (int u = 0, i = 0; u < n; ++u) {
-      const int t0 = (i0 + i) * AT_M;
+      const int t0 = (i0 + i) * BN;
       if (++i == per) i = 0;
       ok = warp_wait(q_full + u % NQ, (u / NQ) & 1) && warp_wait(s_full, u & 1);
       if (!ok) break;
       tc_fence_after_sync();
-      if (vis.whole(t0, t0 + AT_M - 1, k0)) ok = tile(std::false_type{}, u, 0, 0);
+      if (vis.whole(t0, t0 + BN - 1, k0)) ok = tile(std::false_type{}, u, 0, 0);
       else ok = tile(std::true_type{}, u, lo - t0 - half * 64, hi - t0 - half * 64);
       if (!ok) break;
     }
     if (ok && n > 0) ok = warp_wait(done, 0);
     tc_fence_after_sync();
     // the first half of the warps writes dV, the second dK
-    __nv_bfloat16* o = (half == 0 ? p.dv : p.dk) + (((long long)b * p.a.S + key) * p.a.G + kvh) * p.a.D;
-    const float f = half == 0 ? 1.f : p.a.scale;
-    for (int c = 0; c < 64 * DB; c += 16) {
-      uint32_t v[16] = {};
-      if (n > 0) {
-        __syncwarp();
-        tmem_load(tmem + lane_base + (half == 0 ? V_AT : K_AT) + c, v);
-      }
-      if (!inside) {  // what keys past the length hold does not count
+    for (int which = half; which < 2; which += HALVES) {
+      __nv_bfloat16* o = (which == 0 ? p.dv : p.dk) + (((long long)b * p.a.S + key) * p.a.G + kvh) * p.a.D;
+      const float f = which == 0 ? 1.f : p.a.scale;
+      for (int c = 0; c < 64 * DB; c += 16) {
+        uint32_t v[16] = {};
+        if (n > 0) {
+          __syncwarp();
+          tmem_load(tmem + lane_base + (which == 0 ? V_AT : K_AT) + c, v);
+        }
+        if (!inside) {  // what keys past the length hold does not count
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = 0;
+          for (int i = 0; i < 16; ++i) v[i] = 0;
+        }
+        if (key < p.a.S) store_row16(o, c, p.a.D, v, n > 0 ? f : 0.f);
       }
-      if (key < p.a.S) store_row16(o, c, p.a.D, v, n > 0 ? f : 0.f);
     }
     if (!ok && p.status) *p.status = ST_TIMEOUT_TMEM;
   }
@@ -538,35 +556,65 @@ __global__ void __launch_bounds__(BW_THREADS, 1) attention_dkv_kernel(const __gr
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  if (warp == 2) tmem_dealloc(tmem, 512);
+  if (warp == 2) tmem_dealloc(tmem, COLUMNS);
 }
 
-template <int DB>
-void run_bwd(const AttentionBwd& f, cudaStream_t s) {
+int multiprocessors() {
+  static int count[PerDeviceOnce::kMaxDevices] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= PerDeviceOnce::kMaxDevices) return 148;
+  if (count[dev] == 0) cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev);
+  return count[dev];
+}
+
+template <int DB, bool TWO>
+void run_queries(const AttentionBwd& f, const BwdParams& p, unsigned tiles, cudaStream_t s) {
+  constexpr int BN = bwd_tile(TWO), NK = DB == 1 ? 4 : 3, NV = DB == 1 ? 3 : 2, smem = 2 * DB * AT_BOX + (NK + NV) * DB * BN * 128 + 1024;
+  static_assert(smem + 1280 <= 227 * 1024 / (TWO ? 2 : 1), "shared memory of a block");
   const AttentionShape& a = f.a;
-  constexpr int NQ = key_stages(DB), NK = DB == 1 ? 4 : 3, NV = DB == 1 ? 3 : 2;
-  constexpr int smem = (2 + NK + NV) * DB * AT_BOX + 1024;
-  constexpr int smem_kv = (2 + 2 * NQ) * DB * AT_BOX + NQ * 2 * AT_M * 4 + (9 + 2 * NQ) * 8;
-  static_assert(smem + 1280 <= 227 * 1024 && smem_kv <= 227 * 1024, "shared memory of a block");
-  const CUtensorMap tq = attention_map(f.q, a.D, a.T, a.H, a.B), tg = attention_map(f.dout, a.D, a.T, a.H, a.B),
-                    tk = attention_map(f.k, a.D, a.S, a.G, a.B), tv = attention_map(f.v, a.D, a.S, a.G, a.B);
-  const BwdParams p{a, f.out, f.rest, f.dout, f.lse, f.delta, f.dq, f.dk, f.dv, a.scale * LOG2E, f.status};
+  static PerDeviceOnce once;
+  if (once.first_use()) cudaFuncSetAttribute(attention_dq_kernel<DB, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  attention_dq_kernel<DB, TWO><<<dim3(a.B * a.H, tiles), bwd_threads(TWO), smem, s>>>(
+      attention_map(f.q, a.D, a.T, a.H, a.B), attention_map(f.dout, a.D, a.T, a.H, a.B), attention_map(f.k, a.D, a.S, a.G, a.B, BN),
+      attention_map(f.v, a.D, a.S, a.G, a.B, BN), p);
+  attention_check_launch("attention_dq");
+}
+template <int DB, bool TWO>
+void run_keys(const AttentionBwd& f, const BwdParams& p, unsigned tiles, cudaStream_t s) {
+  constexpr int BN = bwd_tile(TWO), NQ = key_stages(DB, TWO), smem = 2 * DB * AT_BOX + NQ * (2 * DB * BN * 128 + 2 * BN * 4) + (9 + 2 * NQ) * 8;
+  static_assert(smem + 1024 <= 227 * 1024 / (TWO ? 2 : 1), "shared memory of a block");
+  const AttentionShape& a = f.a;
   static PerDeviceOnce once;
   if (once.first_use()) {
-    cudaFuncSetAttribute(attention_dq_kernel<DB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    cudaFuncSetAttribute(attention_dkv_kernel<DB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_kv);
+    cudaFuncSetAttribute(attention_dkv_kernel<DB, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaFuncAttributes x{};
+    if (TWO && (cudaFuncGetAttributes(&x, attention_dkv_kernel<DB, TWO>) != cudaSuccess ||
+                x.numRegs * bwd_threads(TWO) < 128 * BW_FEW + (bwd_threads(TWO) - 128) * BW_MANY))
+      throw std::runtime_error("attention_dkv: built with too few registers for its warps' shares");
   }
-  attention_dq_kernel<DB><<<dim3(a.B * a.H, (a.T + AT_M - 1) / AT_M), BW_THREADS, smem, s>>>(tq, tg, tk, tv, p);
-  attention_check_launch("attention_dq");
-  attention_dkv_kernel<DB><<<dim3(a.B * a.G, (a.S + AT_M - 1) / AT_M), BW_THREADS, smem_kv, s>>>(tq, tg, tk, tv, p);
+  attention_dkv_kernel<DB, TWO><<<dim3(a.B * a.G, tiles), bwd_threads(TWO), smem, s>>>(
+      attention_map(f.q, a.D, a.T, a.H, a.B, BN), attention_map(f.dout, a.D, a.T, a.H, a.B, BN), attention_map(f.k, a.D, a.S, a.G, a.B),
+      attention_map(f.v, a.D, a.S, a.G, a.B), p);
   attention_check_launch("attention_dkv");
 }
 
 }  // namespace
 
+// Heads of up to 64 with two CTAs per SM where all SMs get two: a CTA that is left by itself on an SM takes longer than one with tiles of
+// 128. Both kernels, two per SM against one: 16 x 2048 tokens, 6 heads (1536 CTAs) 265 and 314 us, 8 x 1024 (384) 64 and 71; 3000 tokens,
+// 8 heads (192) 93 and 68; 8192 tokens, 8 heads on 2 (512 and 128) 583 and 398.
 void launch_attention_bwd(const AttentionBwd& f, cudaStream_t s) {
-  if (f.a.D <= 64) run_bwd<1>(f, s);
-  else run_bwd<2>(f, s);
+  const AttentionShape& a = f.a;
+  const BwdParams p{a, f.out, f.rest, f.dout, f.lse, f.delta, f.dq, f.dk, f.dv, a.scale * LOG2E, f.status};
+  const unsigned tq = (a.T + AT_M - 1) / AT_M, tk = (a.S + AT_M - 1) / AT_M;
+  const long long many = 2ll * multiprocessors();
+  if (a.D > 64) run_queries<2, false>(f, p, tq, s);
+  else if ((long long)a.B * a.H * tq >= many) run_queries<1, true>(f, p, tq, s);
+  else run_queries<1, false>(f, p, tq, s);
+  if (a.D > 64) run_keys<2, false>(f, p, tk, s);
+  else if ((long long)a.B * a.G * tk >= many) run_keys<1, true>(f, p, tk, s);
+  else run_keys<1, false>(f, p, tk, s);
 }
 
 }  // namespace tb

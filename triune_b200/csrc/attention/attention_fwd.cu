@@ -1,10 +1,15 @@
 // Forward pass: o_i = sum_j p_ij v_j with p the softmax over the visible keys, on the tensor cores.
 //
-// A CTA has two groups of four softmax warps, each with a tile of 128 queries by 128 keys under way, so that one group's
+// An SM has two groups of four softmax warps, each with a tile of 128 queries by 128 keys under way, so that one group's
 // exponentials run under the other group's products:
-//   * pairs (PAIR): the groups have two neighbouring query tiles and walk the same keys;
+//   * pairs (PAIR): the groups have two neighbouring query tiles and walk the same keys. With heads of up to 64 (ALONE) they are CTAs of
+//     their own, each with half of the SM's tensor memory, so that one's start and end (6 us of setting up, first loads and writing) run
+//     under the other's work: 16 x 2048 tokens, 6 heads 131 -> 117 us, 8 x 512 26.6 -> 18.4; walks over 16384 keys lose 7 % (203 -> 218);
 //   * halves: both have the same query tile, one the even and one the odd key tiles, and are added up at the end. Taken where
 //     pairs would leave SMs idle; the keys may then also be split over CTAs (`splits`), whose parts a second kernel adds up.
+// Bound by the softmax warps' arithmetic and exponentials: a tile of 128 x 128 takes 1430 (heads of 64) and 1910 clocks (of 128) of an SM
+// in a long walk, of which its products need 700 and 1400 at the rate that a large product reaches here, and its exponentials 770.
+// Whole calls with a cold L2: 8192 tokens, 16 heads on 4 of 128, causal: 240 us (1150 TFLOP/s); 1024 queries after 15360: 141 us.
 // Warp roles:
 //   warp 0      TMA producer: query tiles once, then two-stage rings of key and value tiles
 //   warp 1      tcgen05.mma: S_w = Q_w K^T into TMEM, O_w += P_w V with P_w read from TMEM
@@ -15,7 +20,7 @@
 // with one; with wider heads, whose sums take the room, weights lie over the scores, and the next scores wait for the product.
 // P is bf16 (every weight is off by 2^-8 of itself at most, which averages out over the keys); fp32 sums take the weights before
 // rounding. The running maximum is lazy: sums are rescaled only when it has grown by more than 2^8.
-// TMEM: S_0 0-127, S_1 128-255, O_0 and O_1 from 256 on, P_0 384-447, P_1 448-511 or over the scores.
+// TMEM: S_0 0-127, S_1 128-255, O_0 and O_1 from 256 on, P_0 384-447, P_1 448-511 or over the scores; ALONE: S 0-127, O 128-191, P 192-255.
 #include <algorithm>
 #include <type_traits>
 
@@ -25,9 +30,15 @@
 namespace tb {
 namespace {
 
-constexpr int FW_THREADS = 384;
+// PAIR with heads of up to 64: one group and one query tile, two CTAs per SM
+constexpr bool alone(int db, bool pair) { return pair && db == 1; }
+constexpr int fwd_threads(int db, bool pair) { return alone(db, pair) ? 256 : 384; }
+// registers of a thread of the first four warps and of the others; 128 + 200 is twice the 128 that 256 threads are launched with, and
+// 88 + 2 * 208 three times the 168 of 384
+constexpr int fwd_few(int db, bool pair) { return alone(db, pair) ? 56 : 88; }
+constexpr int fwd_many(int db, bool pair) { return alone(db, pair) ? 200 : 208; }
 constexpr float FW_LAZY = 8.f;
-constexpr int FW_POLY = 4;  // of so many pairs of exponentials one is a polynomial
+constexpr int FW_POLY = 4;  // of so many pairs of exponentials one is a polynomial (2: 5 to 10 % slower, 3: the same)
 
 struct FwdParams {
   AttentionShape a;
@@ -49,12 +60,14 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 template <int DB, bool PAIR, bool SCALED>
-__global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+__global__ void __launch_bounds__(fwd_threads(DB, PAIR), alone(DB, PAIR) ? 2 : 1) attention_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                                                                       const __grid_constant__ CUtensorMap tmV, const FwdParams p) {
-  constexpr int QT = PAIR ? 2 : 1, TILE = DB * AT_BOX;
+  constexpr bool ALONE = alone(DB, PAIR);
+  constexpr int QT = PAIR && !ALONE ? 2 : 1, TILE = DB * AT_BOX;
   // TMEM columns of the groups' scores, weights and sums. APART: weights do not lie over the scores
   constexpr bool APART = DB == 1;
-  constexpr int S_AT[2] = {0, 128}, P_AT[2] = {APART ? 384 : 0, APART ? 448 : 128}, O_AT[2] = {256, 256 + 64 * DB};
+  constexpr int S_AT[2] = {0, 128}, P_AT[2] = {ALONE ? 192 : APART ? 384 : 0, APART ? 448 : 128}, O_AT[2] = {ALONE ? 128 : 256, 256 + 64 * DB};
+  constexpr uint32_t COLUMNS = ALONE ? 256 : 512;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   uint8_t *sQ = smem, *sK = sQ + QT * TILE, *sV = sK + 2 * TILE;
@@ -76,7 +89,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __gr
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
       const int t0 = q0 + w * AT_M;
-      range[w] = t0 < p.a.T ? vis.tiles(t0, min(p.a.T, t0 + AT_M) - 1) : make_int2(0, 0);
+      range[w] = t0 < p.a.T && w < QT ? vis.tiles(t0, min(p.a.T, t0 + AT_M) - 1) : make_int2(0, 0);
     }
     const bool e0 = range[0].x == range[0].y, e1 = range[1].x == range[1].y;
     j0 = e0 ? range[1].x : e1 ? range[0].x : min(range[0].x, range[1].x);
@@ -118,15 +131,14 @@ __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __gr
     special = 0;
   }
   if (warp == 2) {
-    tmem_alloc(&tmem_slot, 512);
+    tmem_alloc(&tmem_slot, COLUMNS);
     tmem_relinquish();
   }
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = uniform(tmem_slot);
-  // 128 threads of 88 registers and 256 of 208 are 64512, the 384 * 168 that the block is launched with
   if (warp < 4) {
-  registers_down<88>();
+  registers_down<fwd_few(DB, PAIR)>();
   if (warp == 0) {
     if (lane == 0 && j1 > j0) {
       prefetch_tmap(&tmQ);
@@ -198,7 +210,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __gr
       bool ok = warp_wait(q_full, 0) && k_arrived(j0);
       if constexpr (PAIR) {
         if (takes(0, j0)) ok = ok && scores(g0, j0);
-        if (takes(1, j0)) ok = ok && scores(g1, j0);
+        if (!ALONE && takes(1, j0)) ok = ok && scores(g1, j0);
         commit(k_empty);
       } else {
         ok = ok && scores(g0, j0);
@@ -221,7 +233,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __gr
         const bool next = jn < j1;
         if (next) ok = k_arrived(jn);
         if (PAIR || s == 0) ok = ok && turn(g0, j, jn);
-        if (PAIR || s == 1) ok = ok && turn(g1, j, jn);
+        if (!ALONE && (PAIR || s == 1)) ok = ok && turn(g1, j, jn);
         if (next) commit(k_empty + ((jn - j0) & 1));
         commit(v_empty + s);
       }
@@ -263,7 +275,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __gr
     if (!ok && p.status) *p.status = ST_TIMEOUT_FULL;
   }
   } else {
-    registers_up<208>();
+    registers_up<fwd_many(DB, PAIR)>();
     const int w = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const int first = q0 + (PAIR ? w : 0) * AT_M, t = first + row;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
@@ -473,7 +485,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) attention_fwd_kernel(const __gr
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  if (warp == 2) tmem_dealloc(tmem, 512);
+  if (warp == 2) tmem_dealloc(tmem, COLUMNS);
 }
 
 // Parts of rows whose keys were split over CTAs: a warp per row.
@@ -523,12 +535,13 @@ int multiprocessors() {
   return count[dev];
 }
 
-// Pairs where they give every SM a CTA; else halves, with the keys split so far that the CTAs fill the SMs once, each with two key
+// Pairs where they give every SM a CTA (ALONE: where there are more tiles than SMs: 150 tiles of 640 keys 22.5 us as halves, 16.4 as
+// pairs; 192 causal ones of up to 3000 keys 37 and 39); else halves, with the keys split so far that the CTAs fill the SMs once, each with two key
 // tiles at least.
 int fwd_splits(const AttentionShape& a, bool& pair) {
   const int sms = multiprocessors();
   const long long heads = (long long)a.B * a.H, tiles = (a.T + AT_M - 1) / AT_M;
-  pair = heads * ((tiles + 1) / 2) >= sms;
+  pair = a.D <= 64 ? heads * tiles > sms : heads * ((tiles + 1) / 2) >= sms;
   if (pair) return 1;
   const long long most = std::max(1, (a.S + AT_M - 1) / AT_M / 2);
   return (int)std::max<long long>(1, std::min({sms / (heads * tiles), most, 32ll}));
@@ -536,11 +549,16 @@ int fwd_splits(const AttentionShape& a, bool& pair) {
 
 template <int DB, bool PAIR, bool SCALED>
 void run(const FwdParams& p, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t s) {
-  constexpr int QT = PAIR ? 2 : 1, smem = (QT + 4) * DB * AT_BOX + 1024;
+  constexpr int QT = PAIR && !alone(DB, PAIR) ? 2 : 1, smem = (QT + 4) * DB * AT_BOX + 1024, threads = fwd_threads(DB, PAIR);
   static PerDeviceOnce once;
   auto kern = attention_fwd_kernel<DB, PAIR, SCALED>;
-  if (once.first_use()) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  kern<<<dim3(p.a.B * p.a.H, (p.a.T + QT * AT_M - 1) / (QT * AT_M), p.splits), FW_THREADS, smem, s>>>(tq, tk, tv, p);
+  if (once.first_use()) {
+    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaFuncAttributes f{};
+    if (cudaFuncGetAttributes(&f, kern) != cudaSuccess || f.numRegs * threads < 128 * fwd_few(DB, PAIR) + (threads - 128) * fwd_many(DB, PAIR))
+      throw std::runtime_error("attention_fwd: built with too few registers for its warps' shares");
+  }
+  kern<<<dim3(p.a.B * p.a.H, (p.a.T + QT * AT_M - 1) / (QT * AT_M), p.splits), threads, smem, s>>>(tq, tk, tv, p);
   attention_check_launch("attention_fwd");
 }
 

@@ -36,13 +36,13 @@ struct Visible {  // of one sequence
   // queries first(j) .. last(j, T) see key j
   __device__ __forceinline__ int first(int j) const { return causal ? max(0, j - start) : 0; }
   __device__ __forceinline__ int last(int j, int T) const { return window ? min(T - 1, j - before) : T - 1; }
-  // tiles [x, y) of keys that queries t0 .. t1 see
-  __device__ __forceinline__ int2 tiles(int t0, int t1) const {
+  // tiles [x, y) of so many keys that queries t0 .. t1 see
+  __device__ __forceinline__ int2 tiles(int t0, int t1, int keys = AT_M) const {
     const int lo = low(t0), hi = high(t1);
-    return hi < lo ? make_int2(0, 0) : make_int2(lo / AT_M, hi / AT_M + 1);
+    return hi < lo ? make_int2(0, 0) : make_int2(lo / keys, hi / keys + 1);
   }
-  // whether all of queries t0 .. t1 see all of the 128 keys from key on
-  __device__ __forceinline__ bool whole(int t0, int t1, int key) const { return low(t1) <= key && high(t0) >= key + AT_M - 1; }
+  // whether all of queries t0 .. t1 see all of so many keys from key on
+  __device__ __forceinline__ bool whole(int t0, int t1, int key, int keys = AT_M) const { return low(t1) <= key && high(t0) >= key + keys - 1; }
 };
 
 // Bits lo .. hi of 32, whichever of them there are
@@ -102,10 +102,11 @@ __device__ __forceinline__ void issue(F f) {
   if (elect_one()) f();
   __syncwarp();
 }
-// D = A B^T over the head dimension, `steps` times 16 columns; tiles of DB boxes of 64 columns.
-template <int DB>
+// D = A B^T over the head dimension, `steps` times 16 columns; tiles of DB boxes of 64 columns, A of 128 rows and B of N.
+template <int DB, int N = AT_M>
 __device__ __forceinline__ void scores_product(uint32_t d, uint32_t a, uint32_t b, int steps) {
-  constexpr uint32_t idesc = make_idesc(AT_M, AT_M, 1, 1, 0, 0);
+  constexpr uint32_t idesc = make_idesc(AT_M, N, 1, 1, 0, 0);
+  static_assert(N == AT_M || DB == 1, "the boxes of a tile are equally far apart in A and B");
   const uint64_t da = make_smem_desc(a, 16, 1024), db = make_smem_desc(b, 16, 1024);
 #pragma unroll
   for (int k = 0; k < 4 * DB; ++k)

@@ -302,7 +302,7 @@ class SoftmaxAttention(nn.Module):
         if T > 1 and (rep > 1 or past is not None) and ops.attention_supported(q) and k.dtype == q.dtype == v.dtype:
             # Measured on one B200 against the library with repeated heads and a [T, P + T] mask, forward and backward: 1024 tokens after
             # 4096, 16 heads on 4 of 128: 171 against 506 us; whole prompts of 8 x 2048: 673 against 754 us. With a key/value head
-            # per query head and no prefix the library is ahead (16 x 2048, 6 heads of 64: 302 against 426 us) and stays.
+            # per query head and no prefix the library is ahead (16 x 2048, 6 heads of 64: 302 against 397 us) and stays.
             o = ops.attention(q, k, v)
         else:
             kk, vv = (k.repeat_interleave(rep, dim=2), v.repeat_interleave(rep, dim=2)) if rep > 1 else (k, v)

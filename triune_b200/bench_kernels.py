@@ -114,6 +114,35 @@ def case_gla(a):
     report(f"gla fwd+bwd B{B} T{T} H{H}", ms2, nbytes=2.0 * 14 * B * T * H * D)
 
 
+def case_attention(a):
+    """Causal softmax attention, forward alone and with its gradient (4 and 14 D operations a visible pair and head)."""
+    from . import ops
+
+    B, T, H, G, D = a.batch, a.seq, a.heads, a.kv_heads or a.heads, a.head_dim
+    q, k, v = (torch.randn(B, T, h, D, device="cuda").to(torch.bfloat16).requires_grad_(True) for h in (H, G, G))
+    do, pairs = torch.randn_like(q), B * H * T * (T + 1) / 2
+    name = f"B{B} T{T} H{H}/{G} D{D}"
+    with torch.no_grad():
+        report(f"attention fwd {name}", timeit(lambda: ops.attention(q, k, v), a.iters, a.warmup), flops=4 * D * pairs)
+    report(f"attention fwd+bwd {name}", timeit(lambda: torch.autograd.grad(ops.attention(q, k, v), (q, k, v), do), a.iters, a.warmup), flops=14 * D * pairs)
+
+
+@torch.no_grad()
+def case_kv8(a):
+    """The 8-bit key/value cache: a prompt into it and out of it, and a decoding step after ``--seq`` tokens."""
+    from . import ops
+
+    B, T, H, G, D = a.batch, a.seq, a.heads, a.kv_heads or a.heads, a.head_dim
+    k, v = (torch.randn(B, T, G, D, device="cuda").to(torch.bfloat16) for _ in range(2))
+    q, nk, nv = (torch.randn(B, 1, h, D, device="cuda").to(torch.bfloat16) for h in (H, G, G))
+    for kind in ("int8", "e4m3"):
+        name, cache = f"{kind} B{B} T{T} H{H}/{G} D{D}", ops.kv8_cache(B, G, T + 1, D, kind, "cuda")
+        held = 2.0 * B * G * T * (D + 4 / ops.KV8_BLOCK)
+        report(f"kv8 append {name}", timeit(lambda: ops.kv8_append(cache, k, v, 0), a.iters, a.warmup), nbytes=4.0 * B * G * T * D + held)
+        report(f"kv8 expand {name}", timeit(lambda: ops.kv8_expand(cache, T, D), a.iters, a.warmup), nbytes=4.0 * B * G * T * D + held)
+        report(f"kv8 decode {name}", timeit(lambda: ops.kv8_attention(q, cache, T, nk, nv), a.iters, a.warmup), nbytes=held)
+
+
 def case_gdn(a):
     """Gated DeltaNet: the recurrence kernel (no gradient) and forward + backward of the chunk-parallel training form."""
     from . import ops
@@ -452,7 +481,7 @@ def case_small(a):
         run(name, b)
 
 
-CASES = {"small": case_small, "tp": case_tp, "dp": case_dp, "mlp": case_mlp, "moe_route": case_moe_route, "fp8": case_fp8, "nvfp4": case_nvfp4, "gemm": case_gemm, "wgrad": case_wgrad, "gla": case_gla, "gdn": case_gdn, "swiglu": case_swiglu, "rmsnorm": case_rmsnorm, "ce": case_ce}
+CASES = {"attention": case_attention, "kv8": case_kv8, "small": case_small, "tp": case_tp, "dp": case_dp, "mlp": case_mlp, "moe_route": case_moe_route, "fp8": case_fp8, "nvfp4": case_nvfp4, "gemm": case_gemm, "wgrad": case_wgrad, "gla": case_gla, "gdn": case_gdn, "swiglu": case_swiglu, "rmsnorm": case_rmsnorm, "ce": case_ce}
 
 
 def main():
@@ -464,7 +493,8 @@ def main():
     ap.add_argument("--batch", type=int, default=16)
     ap.add_argument("--seq", type=int, default=2048)
     ap.add_argument("--heads", type=int, default=6)
-    ap.add_argument("--head-dim", type=int, default=64, help="head dimension of the gdn case (64 or 128)")
+    ap.add_argument("--head-dim", type=int, default=64, help="head dimension of the gdn case (64 or 128) and of attention and kv8")
+    ap.add_argument("--kv-heads", type=int, default=0, help="key/value heads of attention and kv8 (0: as many as heads)")
     ap.add_argument("--iters", type=int, default=10)
     ap.add_argument("--warmup", type=int, default=3)
     a = ap.parse_args()

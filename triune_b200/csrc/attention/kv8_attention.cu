@@ -14,6 +14,10 @@
 //
 // A CTA is one warp-group of four warps that take units of 32 keys in turn, each with statistics and sums of its own, joined at the
 // end through shared memory. Keys of a head are split over `splits` CTAs; a second kernel joins their parts.
+// Measured with a cold L2, with the append and the join: 32 sequences of 8191 tokens, 16 heads on 8 of 128 in int8 (537 MB of codes) 122 us, this
+// kernel 100 to 105 (0.8 of a copy's rate, issue slots 49 % busy); one of 131000 tokens, 16 heads on 4 of 128 in e4m3 48 us. Fetching
+// the next units into L2 ahead of their loads gains 2 to 4 % there and loses 2 % where L2 holds part of the cache; four CTAs per SM, at
+// 128 registers a thread, take 135 us instead of 122.
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 

@@ -156,6 +156,24 @@ def test_padding_may_hold_anything(what):
     assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, (q, k, v), grad), want))
 
 
+@pytest.mark.parametrize("D", [40, 64])
+@pytest.mark.parametrize("causal,window", [(True, None), (False, None), (True, 70)])
+def test_many_short_sequences_that_end_anywhere(D, causal, window):
+    """More tiles of heads of up to 64 than twice the SMs, of sequences that end at, before and behind the tiles' ends."""
+    lengths = [0, 1, 2, 31, 63, 64, 65, 100, 127, 128, 129, 191, 192, 193, 255, 256, 257, 298, 299, 300]
+    qkv, grad = make(20, 300, 300, 8, 8, D, seed=13)
+    got = check(qkv, grad, lengths=lengths, causal=causal, window=window)
+    assert not got["o"][0].any() and not any(got["d" + n][0].any() for n in "qkv")
+    with torch.no_grad():
+        for b, n in enumerate(lengths):
+            qkv[1][b, n:] = float("nan")
+            qkv[2][b, n:] = float("inf")
+    out = ops.attention(*qkv, key_lengths=torch.tensor(lengths, device="cuda"), causal=causal, window=window)
+    assert torch.equal(out, got["o"])
+    for n, x in zip("qkv", torch.autograd.grad(out, qkv, grad)):
+        assert torch.equal(x, got["d" + n])
+
+
 def test_gradients_against_differences():
     (q, k, v), grad = make(1, 140, 140, 2, 1, 64, seed=10)
     out = ops.attention(q, k, v)

@@ -96,7 +96,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
 
     What keys and values past ``key_lengths`` hold does not matter, whatever it is. A value that is an infinity or NaN reaches the
     outputs of the queries that see it and of no others; gradients are not kept apart in this way. On CUDA, weights and their gradients are rounded to bf16 for
-    the matrix products, sums and statistics are fp32, and results do not depend on the order in which blocks run."""
+    the matrix products, sums and statistics are fp32, and results do not depend on the order in which blocks run. Forward and backward
+    can be captured into a CUDA graph; as with any operator, PyTorch ends the capture of a backward pass with an error where a graph of the
+    same leaves that was not captured is still alive."""
     B, T, S, D = _shapes(q, k, v)
     scale = _scale(scale, D)
     if window is not None and (int(window) != window or window < 1):

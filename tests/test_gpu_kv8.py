@@ -137,6 +137,31 @@ def test_portions_of_prompts(kind, T):
             near(out[b : b + 1], attention64(q[b : b + 1], K, V)["o"], f"sequence {b}")
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D", [40, 64, 72, 128])
+@pytest.mark.parametrize("starts", [[0, 130, -1, 77, 400, 63, 64, 65, 1, 250], [300]])
+def test_portions_of_many_sequences_and_of_one(kind, D, starts):
+    """More tiles of queries than SMs, and fewer (keys are split then); sums over the blocks as above."""
+    B, G, rep, T = len(starts), 4, 4, 130
+    longest = max(starts) + T
+    _, k, v = filled(B, G, D, longest, kind)
+    cache = ops.kv8_cache(B, G, longest + 40, D, kind, device="cuda")
+    for b, n in enumerate(starts):
+        one = ops.kv8_cache(1, G, longest + 40, D, kind, device="cuda")
+        ops.kv8_append(one, k[b : b + 1, : max(n, 0)], v[b : b + 1, : max(n, 0)], 0)
+        for x in cache:
+            cache[x].view(torch.uint8)[b] = one[x].view(torch.uint8)[0]
+    q = rows(B, T, G * rep, D, 5, False) * 0.25
+    at = lambda x: torch.stack([x[b, max(n, 0) : max(n, 0) + T] for b, n in enumerate(starts)])  # noqa: E731
+    out = ops.kv8_attention(q, cache, torch.tensor(starts, device="cuda"), at(k), at(v))
+    for b, n in enumerate(starts):
+        if n < 0:
+            assert not out[b].any()
+            continue
+        K, V = (cache64(x[b].transpose(0, 1), kind, n + T).transpose(0, 1)[None] for x in (k, v))
+        near(out[b : b + 1], attention64(q[b : b + 1], K, V)["o"], f"sequence {b}")
+
+
 def test_appending_first_is_the_same_and_scale_and_bound_are_the_callers():
     a = attend(3, 2, 2, 64, 3, [10, 61, 300], "int8")
     assert torch.equal(a, attend(3, 2, 2, 64, 3, [10, 61, 300], "int8", append=False))

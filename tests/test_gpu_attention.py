@@ -174,6 +174,21 @@ def test_many_short_sequences_that_end_anywhere(D, causal, window):
         assert torch.equal(x, got["d" + n])
 
 
+@pytest.mark.parametrize("shape", [(1, 520, 520, 16, 2, 64), (2, 400, 400, 10, 2, 40), (1, 1100, 1100, 16, 2, 128), (2, 300, 700, 24, 3, 72), (1, 1025, 129, 1, 1, 64)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_keys_whose_queries_are_walked_by_two_blocks(shape, causal):
+    """Fewer tiles of keys than half of the SMs, and eight tiles of queries or more of all heads that share them; some keys are seen by none."""
+    qkv, grad = make(*shape, seed=14)
+    got = check(qkv, grad, causal=causal)
+    for _ in range(10):
+        again = torch.autograd.grad(ops.attention(*qkv, causal=causal), qkv, grad)
+        assert all(torch.equal(x, got["d" + n]) for n, x in zip("qkv", again))
+    check(qkv, grad, lengths=[shape[2] - 130 if shape[2] > 130 else 1] * shape[0], causal=causal)
+    if causal:
+        check(qkv, grad, causal=True, window=shape[2])
+        check(qkv, grad, causal=True, start=-3 if shape[1] < 1000 else 1)
+
+
 def test_gradients_against_differences():
     (q, k, v), grad = make(1, 140, 140, 2, 1, 64, seed=10)
     out = ops.attention(q, k, v)

@@ -15,6 +15,7 @@
 // Bound by the chain from scores to slopes and, with heads of 128, by the products (1.26 and 1.37 PFLOP/s). With a cold L2, dQ and dK, dV:
 // 8192 tokens, 16 heads on 4 of 128, causal: 332 and 407 us, of which the last 50 have SMs without work (the first keys' tile of a shared
 // head is seen by 256 query tiles, the mean of an SM is 225).
+#include <algorithm>
 #include <type_traits>
 
 #include "../common/per_device.h"
@@ -300,7 +301,8 @@ __global__ void __launch_bounds__(bwd_threads(TWO), TWO ? 2 : 1) attention_dq_ke
 // Stages of query tiles: what shared memory holds
 __host__ __device__ constexpr int key_stages(int db, bool two) { return two ? 4 : db == 1 ? 3 : 2; }
 
-template <int DB, bool TWO>
+// SHARE: two neighbouring CTAs (a cluster) have the same keys and one half of their queries each; the second hands its sums to the first.
+template <int DB, bool TWO, bool SHARE>
 __global__ void __launch_bounds__(bwd_threads(TWO), TWO ? 2 : 1) attention_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
                                                                       const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                                                                       const BwdParams p) {
@@ -321,11 +323,14 @@ __global__ void __launch_bounds__(bwd_threads(TWO), TWO ? 2 : 1) attention_dkv_k
     return;
   }
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int kvh = blockIdx.x % p.a.G, b = blockIdx.x / p.a.G, rep = p.a.H / p.a.G;
+  const int member = SHARE ? blockIdx.x & 1 : 0, head_at = SHARE ? blockIdx.x >> 1 : blockIdx.x;
+  const int kvh = head_at % p.a.G, b = head_at / p.a.G, rep = p.a.H / p.a.G;
   const int k0 = blockIdx.y * AT_M;  // with a causal mask the first keys are seen by the most queries
   const Visible vis(p.a, b);
   const int first = vis.first(k0), last = vis.last(min(p.a.S, k0 + AT_M) - 1, p.a.T);
-  const int i0 = first / BN, per = k0 < vis.length && last >= first ? last / BN + 1 - i0 : 0, n = per * rep;
+  const int i0 = first / BN, per = k0 < vis.length && last >= first ? last / BN + 1 - i0 : 0, all = per * rep;
+  const int half_of_all = SHARE ? (all + 1) / 2 : all, n = member == 0 ? half_of_all : all - half_of_all;  // query tiles of all heads, head by head
+  const int skip = member == 0 || n == 0 ? 0 : half_of_all;
   const int padded = (p.a.T + AT_M - 1) / AT_M * AT_M;
 
   if (threadIdx.x == 0) {
@@ -365,7 +370,7 @@ __global__ void __launch_bounds__(bwd_threads(TWO), TWO ? 2 : 1) attention_dkv_k
         tma_load_4d(sV + d * AT_BOX, &tmV, kv_full, d * 64, k0, kvh, b);
       }
       bool ok = true;
-      int i = 0, head = 0;
+      int i = skip > 0 ? skip % per : 0, head = skip > 0 ? skip / per : 0;
       for (int u = 0; u < n && ok; ++u) {
         const int s = u % NQ, h = kvh * rep + head, t0 = (i0 + i) * BN;
         if (++i == per) i = 0, ++head;
@@ -521,7 +526,7 @@ __global__ void __launch_bounds__(bwd_threads(TWO), TWO ? 2 : 1) attention_dkv_k
       mbar_arrive(ds_ready);
       return true;
     };
-    for (int u = 0, i = 0; u < n; ++u) {
+    for (int u = 0, i = skip > 0 ? skip % per : 0; u < n; ++u) {
       const int t0 = (i0 + i) * BN;
       if (++i == per) i = 0;
       ok = warp_wait(q_full + u % NQ, (u / NQ) & 1) && warp_wait(s_full, u & 1);
@@ -533,6 +538,30 @@ __global__ void __launch_bounds__(bwd_threads(TWO), TWO ? 2 : 1) attention_dkv_k
     }
     if (ok && n > 0) ok = warp_wait(done, 0);
     tc_fence_after_sync();
+    if (!ok && p.status) *p.status = ST_TIMEOUT_TMEM;
+  }
+  const int half = (warp - 4) >> 2, row = (warp & 3) * 32 + lane, key = k0 + row;
+  const uint32_t sums = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+  float* other = reinterpret_cast<float*>(smem);  // [2][64 DB][128]
+  if constexpr (SHARE) {
+    __syncwarp();
+    cluster_sync_all();  // nothing reads or writes the tiles any more
+    if (member == 1 && warp >= 4 && n > 0) {
+      for (int which = half; which < 2; which += HALVES)
+        for (int c = 0; c < 64 * DB; c += 16) {
+          uint32_t v[16];
+          __syncwarp();
+          tmem_load(sums + (which == 0 ? V_AT : K_AT) + c, v);
+          const uint32_t to = mapa_shared(smem_u32(other + (which * 64 * DB + c) * AT_M + row), 0);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to + i * AT_M * 4), "r"(v[i]) : "memory");
+        }
+    }
+    __syncwarp();
+    cluster_sync_all();
+  }
+  if (warp >= 4 && member == 0) {
+    const bool inside = key < vis.length;
     // the first half of the warps writes dV, the second dK
     for (int which = half; which < 2; which += HALVES) {
       __nv_bfloat16* o = (which == 0 ? p.dv : p.dk) + (((long long)b * p.a.S + key) * p.a.G + kvh) * p.a.D;
@@ -541,7 +570,11 @@ __global__ void __launch_bounds__(bwd_threads(TWO), TWO ? 2 : 1) attention_dkv_k
         uint32_t v[16] = {};
         if (n > 0) {
           __syncwarp();
-          tmem_load(tmem + lane_base + (which == 0 ? V_AT : K_AT) + c, v);
+          tmem_load(sums + (which == 0 ? V_AT : K_AT) + c, v);
+        }
+        if (SHARE && all > n) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + other[(which * 64 * DB + c + i) * AT_M + row]);
         }
         if (!inside) {  // what keys past the length hold does not count
 #pragma unroll
@@ -550,7 +583,6 @@ __global__ void __launch_bounds__(bwd_threads(TWO), TWO ? 2 : 1) attention_dkv_k
         if (key < p.a.S) store_row16(o, c, p.a.D, v, n > 0 ? f : 0.f);
       }
     }
-    if (!ok && p.status) *p.status = ST_TIMEOUT_TMEM;
   }
   __syncwarp();  // the block's barrier counts warps, not threads
   tc_fence_before_sync();
@@ -580,22 +612,33 @@ void run_queries(const AttentionBwd& f, const BwdParams& p, unsigned tiles, cuda
       attention_map(f.v, a.D, a.S, a.G, a.B, BN), p);
   attention_check_launch("attention_dq");
 }
-template <int DB, bool TWO>
+template <int DB, bool TWO, bool SHARE>
 void run_keys(const AttentionBwd& f, const BwdParams& p, unsigned tiles, cudaStream_t s) {
   constexpr int BN = bwd_tile(TWO), NQ = key_stages(DB, TWO), smem = 2 * DB * AT_BOX + NQ * (2 * DB * BN * 128 + 2 * BN * 4) + (9 + 2 * NQ) * 8;
   static_assert(smem + 1024 <= 227 * 1024 / (TWO ? 2 : 1), "shared memory of a block");
   const AttentionShape& a = f.a;
   static PerDeviceOnce once;
   if (once.first_use()) {
-    cudaFuncSetAttribute(attention_dkv_kernel<DB, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaFuncSetAttribute(attention_dkv_kernel<DB, TWO, SHARE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     cudaFuncAttributes x{};
-    if (TWO && (cudaFuncGetAttributes(&x, attention_dkv_kernel<DB, TWO>) != cudaSuccess ||
+    if (TWO && (cudaFuncGetAttributes(&x, attention_dkv_kernel<DB, TWO, SHARE>) != cudaSuccess ||
                 x.numRegs * bwd_threads(TWO) < 128 * BW_FEW + (bwd_threads(TWO) - 128) * BW_MANY))
       throw std::runtime_error("attention_dkv: built with too few registers for its warps' shares");
   }
-  attention_dkv_kernel<DB, TWO><<<dim3(a.B * a.G, tiles), bwd_threads(TWO), smem, s>>>(
-      attention_map(f.q, a.D, a.T, a.H, a.B, BN), attention_map(f.dout, a.D, a.T, a.H, a.B, BN), attention_map(f.k, a.D, a.S, a.G, a.B),
-      attention_map(f.v, a.D, a.S, a.G, a.B), p);
+  static_assert(!SHARE || 2 * 64 * DB * AT_M * 4 <= 2 * DB * AT_BOX + NQ * 2 * DB * BN * 128, "the sums take the tiles' place");
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.B * a.G * (SHARE ? 2 : 1), tiles);
+  cfg.blockDim = dim3(bwd_threads(TWO));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = SHARE ? 1 : 0;
+  cudaLaunchKernelEx(&cfg, attention_dkv_kernel<DB, TWO, SHARE>, attention_map(f.q, a.D, a.T, a.H, a.B, BN), attention_map(f.dout, a.D, a.T, a.H, a.B, BN),
+                     attention_map(f.k, a.D, a.S, a.G, a.B), attention_map(f.v, a.D, a.S, a.G, a.B), p);
   attention_check_launch("attention_dkv");
 }
 
@@ -604,6 +647,10 @@ void run_keys(const AttentionBwd& f, const BwdParams& p, unsigned tiles, cudaStr
 // Heads of up to 64 with two CTAs per SM where all SMs get two: a CTA that is left by itself on an SM takes longer than one with tiles of
 // 128. Both kernels, two per SM against one: 16 x 2048 tokens, 6 heads (1536 CTAs) 265 and 314 us, 8 x 1024 (384) 64 and 71; 3000 tokens,
 // 8 heads (192) 93 and 68; 8192 tokens, 8 heads on 2 (512 and 128) 583 and 398.
+// Keys shared by two CTAs where there are fewer of them than SMs and their walks over the queries of all heads are long. Both kernels, in tiles
+// of 128 without and with it: 8192 tokens, 8 heads on 2 of 64 (128 CTAs, 256 tiles) 411 and 282 us; 4096, 12 on 4 of 128 (128, 96) 251 and 195; 600
+// twice, 8 on 2 of 64 (20, 20) 46 and 38; 1024, 8 of 128 (64, 8) 48 and 46; but 2048, 8 of 128 (128, 16) 69 and 73; 1001, 12 of 80 (96, 8) 44 and
+// 52; 4096, 4 of 128 with a window of 600 (128, 6) 46 and 62; 8192, 16 on 4 of 128 (256, 256) 759 and 753; 4 x 2048, 16 on 4 (256, 64) 286 and 310.
 void launch_attention_bwd(const AttentionBwd& f, cudaStream_t s) {
   const AttentionShape& a = f.a;
   const BwdParams p{a, f.out, f.rest, f.dout, f.lse, f.delta, f.dq, f.dk, f.dv, a.scale * LOG2E, f.status};
@@ -612,9 +659,11 @@ void launch_attention_bwd(const AttentionBwd& f, cudaStream_t s) {
   if (a.D > 64) run_queries<2, false>(f, p, tq, s);
   else if ((long long)a.B * a.H * tq >= many) run_queries<1, true>(f, p, tq, s);
   else run_queries<1, false>(f, p, tq, s);
-  if (a.D > 64) run_keys<2, false>(f, p, tk, s);
-  else if ((long long)a.B * a.G * tk >= many) run_keys<1, true>(f, p, tk, s);
-  else run_keys<1, false>(f, p, tk, s);
+  const long long ctas = (long long)a.B * a.G * tk, walk = (a.window > 0 ? std::min<long long>(tq, a.window / AT_M + 2) : tq) * (a.H / a.G);
+  const bool few = ctas < multiprocessors() && walk >= (2 * ctas <= multiprocessors() ? 8 : 32);
+  if (a.D > 64) few ? run_keys<2, false, true>(f, p, tk, s) : run_keys<2, false, false>(f, p, tk, s);
+  else if ((long long)a.B * a.G * tk >= many) run_keys<1, true, false>(f, p, tk, s);
+  else few ? run_keys<1, false, true>(f, p, tk, s) : run_keys<1, false, false>(f, p, tk, s);
 }
 
 }  // namespace tb

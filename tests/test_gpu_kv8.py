@@ -312,3 +312,46 @@ def test_captured_steps_follow_positions_on_the_device(T):
             g.replay()
             assert torch.equal(out, want[i])
     assert all(torch.equal(a, bits(caches[0])[x]) for x, a in bits(cache).items())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T", [128, 300])
+@pytest.mark.parametrize("starts", [[0], [64, 130, -1, 0]])
+@pytest.mark.parametrize("what", [float("nan"), -float("inf")])
+def test_queries_before_a_block_that_reads_as_none_do_not_see_it(kind, D, T, starts, what):
+    """A token of the portion is no number, and so its whole block once it is full. Queries before the block (before the token, where
+    the block is open) are, bit for bit, what they are without it; the others are no numbers in all columns of a full block."""
+    B, G, rep, longest = len(starts), 2, 2, max(starts) + T
+    _, k, v = filled(B, G, D, longest, kind)
+    q = rows(B, T, G * rep, D, 5, False) * 0.25
+    at = lambda x: torch.stack([x[b, max(n, 0) : max(n, 0) + T] for b, n in enumerate(starts)])  # noqa: E731
+
+    def call(new_k, new_v, on_device):
+        cache = ops.kv8_cache(B, G, longest, D, kind, device="cuda")
+        for b, n in enumerate(starts):  # each sequence as it was before its new tokens
+            one = ops.kv8_cache(1, G, longest, D, kind, device="cuda")
+            ops.kv8_append(one, k[b : b + 1, : max(n, 0)], v[b : b + 1, : max(n, 0)], 0)
+            for x in cache:
+                cache[x].view(torch.uint8)[b] = one[x].view(torch.uint8)[0]
+        return ops.kv8_attention(q, cache, torch.tensor(starts, device="cuda") if on_device else starts[0], new_k, new_v)
+
+    for on_device in (True, False)[: 1 + (B == 1)]:
+        clean = call(at(k), at(v), on_device)
+        for side in range(2):
+            for token in (T // 2 + 36, T - 1):
+                new = [at(k), at(v)]
+                new[side][:, token, :, 7] = what
+                out = call(*new, on_device)
+                for b, n in enumerate(starts):
+                    if n < 0:
+                        assert not out[b].any()
+                        continue
+                    block = (n + token) // BLOCK * BLOCK
+                    full = block + BLOCK <= n + T
+                    first = max(0, block - n) if full else token
+                    assert torch.equal(out[b, :first], clean[b, :first]), (b, side, token)
+                    if full:
+                        assert bool(torch.isnan(out[b, first:]).all())
+                    elif side:
+                        assert not torch.isfinite(out[b, first:, :, 7]).any()

@@ -372,6 +372,11 @@ __global__ void __launch_bounds__(fwd_threads(DB, PAIR), alone(DB, PAIR) ? 2 : 1
           }
           sum2 = add2(sum2, e);
           if constexpr (SCALED) e = mul2(e, c < 2 ? v0 : v1);
+          if constexpr (MASKED && SCALED) {  // and a value scale that is no number must not reach queries that do not see its block
+            float a, z;
+            unpack_f2(e, a, z);
+            e = pack_f2(see >> (2 * i) & 1 ? a : 0.f, see >> (2 * i + 1) & 1 ? z : 0.f);
+          }
           q[i] = f2_to_bf16x2(e);
         }
         tmem_st_32x32b_x16(tP + 16 * c, q);

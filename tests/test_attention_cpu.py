@@ -212,3 +212,16 @@ def test_training_a_model_with_shared_heads():
     block = DenseTransformerBlock(32, 4, num_kv_heads=2)
     y, state = block(rand(1, 5, 32), state=(None, 0))
     assert y.shape == (1, 5, 32) and state[0][0].shape == (1, 5, 2, 8)
+
+
+def test_the_status_word_is_no_inference_tensor():
+    from triune_b200.ops import hybrid
+
+    kept = dict(hybrid._STATUS)
+    hybrid._STATUS.clear()
+    try:
+        with torch.inference_mode():
+            assert not hybrid.status_word("cpu").is_inference()
+    finally:
+        hybrid._STATUS.clear()
+        hybrid._STATUS.update(kept)

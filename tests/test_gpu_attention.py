@@ -273,3 +273,24 @@ def test_second_derivatives_and_tangents_are_refused():
 
     with fw.dual_level(), pytest.raises(NotImplementedError):
         ops.attention(fw.make_dual(q.detach(), torch.ones_like(q)), k.detach(), v.detach())
+
+
+def test_training_after_a_first_call_in_inference_mode():
+    """The word that a kernel's expired wait sets is made by whichever call comes first, also one that keeps nothing for a backward pass."""
+    from triune_b200.ops import hybrid
+
+    (q, k, v), grad = make(1, 50, 50, 2, 1, 64)
+    want = torch.autograd.grad(ops.attention(q, k, v), (q, k, v), grad)
+    kept = dict(hybrid._STATUS)
+    hybrid._STATUS.clear()
+    try:
+        with torch.inference_mode():
+            ops.attention(q, k, v)
+        out = ops.attention(q, k, v)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, (q, k, v), grad), want))
+        out = ops.attention(q, k, v)
+        for word in hybrid._STATUS.values():  # what looks at it may write it between the passes
+            word.zero_()
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, (q, k, v), grad), want))
+    finally:
+        hybrid._STATUS.update(kept)

@@ -179,7 +179,8 @@ class AttentionNode : public torch::autograd::Function<AttentionNode> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, double scale, bool causal, int64_t window,
                         const OptTensor& lengths, const OptTensor& starts, int64_t start, const Tensor& status) {
     std::vector<Tensor> r = attention_fwd(q, k, v, scale, causal, window, lengths, starts, start, true, status);
-    ctx->save_for_backward({q, k, v, r[0], r[2], r[1], has(lengths) ? *lengths : Tensor(), has(starts) ? *starts : Tensor(), status});
+    ctx->save_for_backward({q, k, v, r[0], r[2], r[1], has(lengths) ? *lengths : Tensor(), has(starts) ? *starts : Tensor()});
+    ctx->saved_data["status"] = status;  // kept for the process, and written by whoever looks at it: no value that a version is checked of
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["window"] = window;
@@ -189,7 +190,7 @@ class AttentionNode : public torch::autograd::Function<AttentionNode> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     const auto x = ctx->get_saved_variables();
     std::vector<Tensor> r = attention_bwd(x[0], x[1], x[2], x[3], x[4], grads[0].to(x[0].scalar_type()), x[5], ctx->saved_data["scale"].toDouble(),
-                                          ctx->saved_data["causal"].toBool(), ctx->saved_data["window"].toInt(), x[6], x[7], ctx->saved_data["start"].toInt(), x[8]);
+                                          ctx->saved_data["causal"].toBool(), ctx->saved_data["window"].toInt(), x[6], x[7], ctx->saved_data["start"].toInt(), ctx->saved_data["status"].toTensor());
     if (torch::GradMode::is_enabled()) {  // a graph of the gradients is asked for: they have none, and say so when it is used
       torch::autograd::variable_list leaves;
       for (Tensor& t : r) leaves.push_back(t.detach().requires_grad_(true));

@@ -37,7 +37,8 @@ def status_word(device) -> torch.Tensor:
     """The device's int32 word that a kernel sets when one of its bounded waits expires (0 = none did)."""
     key = torch.device(device)
     if key not in _STATUS:
-        _STATUS[key] = torch.zeros(1, dtype=torch.int32, device=key)
+        with torch.inference_mode(False):  # it outlives the call that comes first, and serves calls that train
+            _STATUS[key] = torch.zeros(1, dtype=torch.int32, device=key)
     return _STATUS[key]
 
 

@@ -225,3 +225,15 @@ def test_the_status_word_is_no_inference_tensor():
     finally:
         hybrid._STATUS.clear()
         hybrid._STATUS.update(kept)
+
+
+@pytest.mark.parametrize("mixer", ["sdpa", "gla"])
+def test_a_model_evaluated_in_inference_mode_can_be_trained_afterwards(mixer):
+    torch.manual_seed(0)
+    m = UniversalDenseTransformer.from_config(ModelConfig(family="universal", vocab_size=61, hidden_dim=32, num_layers=2, num_heads=4, head_dim=8,
+                                                          mixer=mixer, ffn="swiglu", dense_hidden=48).validate())
+    ids = torch.randint(0, 61, (2, 40), generator=torch.Generator().manual_seed(5))
+    with torch.inference_mode():
+        m.eval()(ids)
+    m.train().forward_loss(ids[:, :-1], ids[:, 1:]).backward()
+    assert all(torch.isfinite(p.grad).all() for p in m.parameters())

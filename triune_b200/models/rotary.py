@@ -59,8 +59,8 @@ class RotaryEmbedding(nn.Module):
         return self._sin
 
     def _build(self, length: int, device):
-        cos, sin = ops.rope_tables(length, self.head_dim, self.base, 0, device)
-        self._cos, self._sin = cos, sin
+        with torch.inference_mode(False):  # they outlive the call that wants them first, and serve calls that train
+            self._cos, self._sin = ops.rope_tables(length, self.head_dim, self.base, 0, device)
 
     def tables(self, seq_len: int, device, offset=0):
         """The whole tables [rows, head_dim], grown to cover ``offset + seq_len`` positions where ``offset`` is a number. A

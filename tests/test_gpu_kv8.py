@@ -355,3 +355,58 @@ def test_queries_before_a_block_that_reads_as_none_do_not_see_it(kind, D, T, sta
                         assert bool(torch.isnan(out[b, first:]).all())
                     elif side:
                         assert not torch.isfinite(out[b, first:, :, 7]).any()
+
+
+def by_contributions(q, k, v, kind, pos):
+    """As ``kv8_attention64``, but weights that are small are off by what half a step of fp16's smallest is next to the largest
+    CONTRIBUTION (weight times the block's scale): a power of two of at most twice that is the unit of the weights times scales,
+    which are rounded to fp16, 2^-25 at most below 2^-14."""
+    T, H, D = q.shape
+    G, n = k.shape[0], pos + T
+    full = n // BLOCK
+    K, V = cache64(k, kind, n), cache64(v, kind, n)
+    value, bound = (torch.zeros(T, H, D, dtype=torch.float64, device=q.device) for _ in "ab")
+    see = torch.arange(n, device=q.device) <= torch.arange(pos, n, device=q.device)[:, None]
+    for h in range(H):
+        g = h // (H // G)
+        scale = coded64(v[g, : full * BLOCK].unflatten(0, (full, BLOCK)), kind)[1].repeat_interleave(BLOCK)
+        p = torch.softmax((D ** -0.5 * q[:, h].double() @ K[g].T).masked_fill(~see, float("-inf")), -1)
+        value[:, h] = p @ V[g]
+        codes = (V[g, : full * BLOCK] / scale.masked_fill(scale == 0, 1.0)[:, None]).abs().sum(0)
+        largest = (p[:, : full * BLOCK] * scale).amax(-1, keepdim=True)
+        off = (2.0 ** -11 + 3e-5) * (p @ V[g].abs()) + 2.0 ** -24 * largest * codes
+        bound[:, h] = 2.0 ** -8 * value[:, h].abs() + (1 + 2.0 ** -8) * off
+    return value, bound
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D,T,n", [(64, 1, 2047), (128, 1, 2060), (64, 4, 2100), (128, 12, 20000)])
+@pytest.mark.parametrize("factor", [1e3, 1e5, 1e8, 1e20, 1e34])
+def test_a_loud_block_that_hardly_counts_leaves_the_others_their_digits(kind, D, T, n, factor):
+    """Values of one block are larger by a factor than all others, and its scores lower by so much that its weight next to nothing is: what the
+    other blocks give has its digits all the same. With the largest factor it outweighs them, and they are what is lost."""
+    B, G, H = 1, 1, 2
+    q, k, v = rows(B, T, H, D, 3, False), rows(B, n + T, G, D, 1, False), rows(B, n + T, G, D, 2, False)
+    q[:] = q[:, :1, :1]  # one direction, which the loud keys point away from
+    loud = slice(BLOCK * 5, BLOCK * 6)
+    x = q[0, 0, 0].float()
+    k[0, loud, 0] = (-60 * D ** 0.5 * x / (x @ x)).bfloat16()
+    v[0, loud] = (v[0, loud].float() * factor).bfloat16()
+    cache = ops.kv8_cache(B, G, n + T, D, kind, device="cuda")
+    ops.kv8_append(cache, k[:, :n], v[:, :n], 0)
+    out = ops.kv8_attention(q, cache, n, k[:, n:], v[:, n:])
+    near(out[0], by_contributions(q[0], k[0].transpose(0, 1), v[0].transpose(0, 1), kind, n))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("order", [(1e-36, 1.0, 1e30, 0.0, 1e-20), (1e30, 1e-36, 0.0, 1.0, 1e-38), (0.0, 0.0, 1e-38, 1e-39, 0.0), (1e36, 1e-30, 1e36, 0.0, 1e-36)])
+def test_scales_from_the_smallest_to_the_largest(kind, order):
+    q, k, v = rows(1, 1, 3, 64, 3, False), rows(1, 330, 1, 64, 1, False), rows(1, 330, 1, 64, 2, False)
+    for m, f in enumerate(order):
+        v[:, 64 * m : 64 * m + 64] = (v[:, 64 * m : 64 * m + 64].double() * f).bfloat16()
+    v[:, 320:] = 0
+    cache = ops.kv8_cache(1, 1, 400, 64, kind, device="cuda")
+    ops.kv8_append(cache, k, v, 0)
+    value, bound = by_contributions(q[0], k[0].transpose(0, 1), v[0].transpose(0, 1), kind, 329)
+    # numbers below the least normal one (2^-126) are off by half a step of the subnormal ones, 2^-134 in bf16, or flushed
+    near(ops.kv8_attention(q, cache, 329)[0], (value, bound + 2.0 ** -125))

@@ -7,9 +7,11 @@
 //   scores^T = K Q^T: A = 16 keys. The head dimension is put in such an order that a thread's fragments are 16 consecutive bytes.
 //   out^T = V^T P^T: A = 16 columns of V by 16 keys; columns are put in such an order that a thread's are 16 consecutive bytes;
 //   neighbouring keys are paired by byte permutes, P^T comes from the scores by an 8x8 transpose (movmatrix).
-// Scales: a block's key scale multiplies its scores; its value scale, over the largest one so far, the weights (which stay within
-// fp16's range), sums are in units of that largest. Queries are scaled by powers of two to fit fp16 (exact but for parts below 2^-24
-// of a row's largest). Weights lose 2^-11 of themselves to fp16 at most (2^-24 absolutely, where they are small); scores, statistics and sums are fp32.
+// Scales: a block's key scale multiplies its scores; its value scale the weights, in units of a power of two of each query's own that is no
+// less than its largest weight times value scale (but for the scale's fraction) so far. So it is by what they contribute that blocks are measured: a block of large values that
+// a query hardly looks at takes no digits from the others. Queries are scaled by powers of two to fit fp16 (exact but for parts below 2^-24
+// of a row's largest). Weights times scales lose 2^-11 of themselves to fp16 at most (2^-24 of the largest of them, where they are small); scores,
+// statistics and sums are fp32.
 // The open block is read from the ring in bf16, weights in two bf16 parts (2^-16).
 //
 // A CTA is one warp-group of four warps that take units of 32 keys in turn, each with statistics and sums of its own, joined at the
@@ -33,6 +35,9 @@ namespace {
 
 constexpr int DW = 4, UNIT = 32;  // warps of a CTA, keys of a unit
 constexpr int MOST_SPLITS = 512;
+// CTAs of an SM, which registers are kept to. Columns of 64, up to 8 queries: with four CTAs (115 registers) instead of five, four drafted tokens on
+// 8 x 2047, 30 heads take 24.6 us instead of 22.5, a step on 32 x 8191, 6 heads 58 (int8) and 61 (e4m3) instead of 62 and 69.
+constexpr int resident(int P, int NT) { return P == 64 ? (NT == 1 ? 5 : 3) : (NT == 1 ? 3 : 2); }
 constexpr int step_smem(int P, int NT) { return DW * NT * 8 * (P + 4) * 4; }
 
 struct StepParams {
@@ -77,6 +82,13 @@ __device__ __forceinline__ void numbers(uint32_t w, uint32_t& lo, uint32_t& hi) 
     hi = *reinterpret_cast<const uint32_t*>(&y);
   }
 }
+// A scale (>= 0, or NaN) as a fraction from 1 to 2 (0 and NaN: themselves) times a power of two, whose exponent is returned
+__device__ __forceinline__ float exponent_of(float s, float& fraction) {
+  const bool small = s < 0x1p-100f;  // subnormal numbers among them
+  const uint32_t bits = __float_as_uint(small ? s * 0x1p64f : s);
+  fraction = s > 0.f ? __uint_as_float((bits & 0x7fffffu) | 0x3f800000u) : s;
+  return (float)((int)(bits >> 23) - (small ? 191 : 127));
+}
 template <int BYTES>
 __device__ __forceinline__ void load_codes(const uint8_t* at, uint32_t* w) {
   if constexpr (BYTES == 16) {
@@ -89,7 +101,7 @@ __device__ __forceinline__ void load_codes(const uint8_t* at, uint32_t* w) {
 }
 
 template <int P, bool E4M3, int NT>
-__global__ void __launch_bounds__(DW * 32) kv8_attention_kernel(const StepParams p) {
+__global__ void __launch_bounds__(DW * 32, resident(P, NT)) kv8_attention_kernel(const StepParams p) {
   constexpr int KS = P / 16, VW = P / 32;  // products of a tile; words of a thread's part of a value row
   __shared__ float2 stat[DW][NT * 8];
   extern __shared__ float sums[];  // [DW][NT * 8][P + 4]
@@ -148,16 +160,17 @@ __global__ void __launch_bounds__(DW * 32) kv8_attention_kernel(const StepParams
     for (int k = 0; k < 2; ++k) seen[n][k] = pos + (row0 + n * 8 + 2 * t + k) / p.rep;
 
   float m[NT][2], l[NT][2], o[NT][KS][4];
-  float unit = 0.f;  // of the sums: the largest value scale so far
+  float unit[NT][2];  // the sums are in units of two to this power (of weights as they are now)
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    m[n][0] = m[n][1] = -INFINITY;
+    m[n][0] = m[n][1] = unit[n][0] = unit[n][1] = -INFINITY;
     l[n][0] = l[n][1] = 0.f;
 #pragma unroll
     for (int i = 0; i < KS; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
   }
-  // statistics of TILES tiles of 16 keys whose scores (base 2) are in s; s becomes the weights. -> factors of the sums so far
-  auto softmax = [&](auto& s, int tiles, float (&f)[NT][2]) {
+  // statistics of so many tiles of 16 keys whose scores (base 2) are in s; s becomes the weights. -> the logarithms of the tiles' largest
+  // weights, and of what weights so far have shrunk to
+  auto softmax = [&](auto& s, int tiles, float (&top)[NT][2], float (&less)[NT][2]) {
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -169,11 +182,13 @@ __global__ void __launch_bounds__(DW * 32) kv8_attention_kernel(const StepParams
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        const float here = mx;
         mx = fmaxf(mx, m[n][k]);
         const float ref = mx == -INFINITY ? 0.f : mx;
-        f[n][k] = m[n][k] == mx ? 1.f : ex2(m[n][k] - ref);
+        top[n][k] = here - ref;
+        less[n][k] = m[n][k] == mx ? 0.f : m[n][k] - ref;
         m[n][k] = mx;
-        l[n][k] *= f[n][k];
+        l[n][k] *= ex2(less[n][k]);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
           if (i < tiles) {
@@ -254,17 +269,21 @@ __global__ void __launch_bounds__(DW * 32) kv8_attention_kernel(const StepParams
           s[i][n][k] *= back[n][k & 1] * here;
           if (masked && key + 16 * i + 8 * (k >> 1) > seen[n][k & 1]) s[i][n][k] = -INFINITY;
         }
-    float f[NT][2];
-    softmax(s, 2, f);
-    float more = 1.f;
-    if (!(vs <= unit)) {  // larger, or no number
-      more = unit / vs;
-      unit = vs;
-    }
-    const float ratio = unit > 0.f || unit != unit ? vs / unit : 0.f;
+    float top[NT][2], less[NT][2], ratio[NT][2];
+    softmax(s, 2, top, less);
+    float fraction;
+    const float power = exponent_of(vs, fraction);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const float f0 = f[n][0] * more, f1 = f[n][1] * more;
+      float f[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float old = unit[n][k] + less[n][k], now = fmaxf(old, top[n][k] + power);
+        f[k] = old == now ? 1.f : ex2(old - now);
+        unit[n][k] = now;
+        ratio[n][k] = fraction * ex2(fminf(power - now, 126.f));  // past 126 there are no weights, or none that fp32 holds
+      }
+      const float f0 = f[0], f1 = f[1];
       if (__any_sync(0xffffffffu, f0 != 1.f || f1 != 1.f))
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
@@ -279,8 +298,8 @@ __global__ void __launch_bounds__(DW * 32) kv8_attention_kernel(const StepParams
       uint32_t w0[NT], w1[NT];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        w0[n] = transpose8(half2_bits(s[i][n][0] * ratio, s[i][n][1] * ratio));
-        w1[n] = transpose8(half2_bits(s[i][n][2] * ratio, s[i][n][3] * ratio));
+        w0[n] = transpose8(half2_bits(s[i][n][0] * ratio[n][0], s[i][n][1] * ratio[n][1]));
+        w1[n] = transpose8(half2_bits(s[i][n][2] * ratio[n][0], s[i][n][3] * ratio[n][1]));
       }
 #pragma unroll
       for (int w = 0; w < VW; ++w) {
@@ -298,11 +317,13 @@ __global__ void __launch_bounds__(DW * 32) kv8_attention_kernel(const StepParams
     }
   }
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+  for (int n = 0; n < NT; ++n) {
+    const float f[2] = {exp2f(unit[n][0]), exp2f(unit[n][1])};  // from here on in weights
 #pragma unroll
     for (int i = 0; i < KS; ++i)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) o[n][i][k] *= unit;
+      for (int k = 0; k < 4; ++k) o[n][i][k] *= f[k & 1];
+  }
 
   // ---- the open block: a tile of 16 keys per warp, by the CTA of the last part
   const int k0 = full + 16 * warp;
@@ -333,17 +354,18 @@ __global__ void __launch_bounds__(DW * 32) kv8_attention_kernel(const StepParams
         const int key = k0 + g + 8 * (k >> 1);
         s[0][n][k] = key <= seen[n][k & 1] && key < total ? s[0][n][k] * p.scale2 : -INFINITY;
       }
-    float f[NT][2];
-    softmax(s, 1, f);
+    float top[NT][2], less[NT][2];
+    softmax(s, 1, top, less);
     uint32_t hi[NT][2], lo[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
+      const float f0 = ex2(less[n][0]), f1 = ex2(less[n][1]);
 #pragma unroll
       for (int i = 0; i < KS; ++i) {
-        o[n][i][0] *= f[n][0];
-        o[n][i][1] *= f[n][1];
-        o[n][i][2] *= f[n][0];
-        o[n][i][3] *= f[n][1];
+        o[n][i][0] *= f0;
+        o[n][i][1] *= f1;
+        o[n][i][2] *= f0;
+        o[n][i][3] *= f1;
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {

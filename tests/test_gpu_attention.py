@@ -294,3 +294,18 @@ def test_training_after_a_first_call_in_inference_mode():
         assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, (q, k, v), grad), want))
     finally:
         hybrid._STATUS.update(kept)
+
+
+@pytest.mark.parametrize("T,S,H", [(1, 4096, 1), (3, 9000, 2), (200, 200, 200)])
+@pytest.mark.parametrize("what", [float("nan"), float("inf")])
+def test_values_that_are_no_numbers_reach_queries_whose_weight_for_them_is_zero(T, S, H, what):
+    """Where keys are split over blocks, a part whose scores are far below the others' counts for nothing, unless its sums are no numbers."""
+    (q, k, v), _ = make(1, T, S, H, 1, 64, seed=15, grad=False)
+    q[:] = q[:, :1, :1]
+    x = q[0, 0, 0].float()
+    k[0, : S // 2, 0] = (-300 * 8.0 * x / (x @ x)).bfloat16()
+    v[0, 10, 0, 5] = what
+    out = ops.attention(q, k, v, query_start=S)
+    assert not torch.isfinite(out[..., 5]).any()
+    keep = torch.arange(64, device="cuda") != 5
+    assert torch.isfinite(out[..., keep]).all()

@@ -410,3 +410,18 @@ def test_scales_from_the_smallest_to_the_largest(kind, order):
     value, bound = by_contributions(q[0], k[0].transpose(0, 1), v[0].transpose(0, 1), kind, 329)
     # numbers below the least normal one (2^-126) are off by half a step of the subnormal ones, 2^-134 in bf16, or flushed
     near(ops.kv8_attention(q, cache, 329)[0], (value, bound + 2.0 ** -125))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n,low", [(270, 256), (6000, 3000)])
+@pytest.mark.parametrize("T", [1, 3])
+def test_a_block_that_is_no_number_reaches_queries_whose_weight_for_it_is_zero(kind, n, low, T):
+    """Scores so much lower than others that the weights are zero in 32 bits: zero times what is no number is none."""
+    q, k, v = rows(1, T, 2, 64, 3, False), rows(1, n + T, 1, 64, 1, False), rows(1, n + T, 1, 64, 2, False)
+    q[:] = q[:, :1, :1]
+    x = q[0, 0, 0].float()
+    k[0, :low, 0] = (-300 * 8.0 * x / (x @ x)).bfloat16()
+    v[0, 70, 0, 5] = float("inf")
+    cache = ops.kv8_cache(1, 1, n + T, 64, kind, device="cuda")
+    ops.kv8_append(cache, k[:, :n], v[:, :n], 0)
+    assert bool(torch.isnan(ops.kv8_attention(q, cache, n, k[:, n:], v[:, n:])).all())

@@ -505,8 +505,8 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const FwdParams p) 
   float l = 0.f, acc[2 * DB] = {};
   for (int s = 0; s < p.splits; ++s) {
     const float2 x = ml[s * rows + row];
-    const float f = x.x == -INFINITY ? (x.y == x.y ? 0.f : 1.f) : ex2(x.x - m);
-    if (f == 0.f && x.y == x.y) continue;  // nothing visible there (its sums may not have been formed), or nothing that counts
+    if (x.x == -INFINITY && x.y == x.y) continue;  // nothing visible there: its sums may not have been formed
+    const float f = x.x == -INFINITY ? 1.f : ex2(x.x - m);  // zero times sums that are no numbers is none
     l += x.y * f;
 #pragma unroll
     for (int i = 0; i < 2 * DB; ++i) acc[i] += p.part[(s * rows + row) * 64 * DB + lane + 32 * i] * f;

@@ -451,8 +451,8 @@ __global__ void __launch_bounds__(DW * 32, resident(P, NT)) kv8_attention_kernel
 #pragma unroll
     for (int w = 0; w < DW; ++w) {
       const float2 st = stat[w][q];
-      f[w] = st.x == -INFINITY ? (st.y == st.y ? 0.f : 1.f) : ex2(st.x - mx);
-      if (f[w] == 0.f && st.y == st.y) continue;
+      if (st.x == -INFINITY && st.y == st.y) continue;  // no visible key
+      f[w] = st.x == -INFINITY ? 1.f : ex2(st.x - mx);  // zero times sums that are no numbers is none
       sum += st.y * f[w];
       const float4 y = *reinterpret_cast<const float4*>(sums + (w * NT * 8 + q) * (P + 4) + d);
       x.x += y.x * f[w];
@@ -490,9 +490,10 @@ __global__ void __launch_bounds__(128) kv8_join_kernel(const StepParams p) {
   for (int i = 16; i > 0; i >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, i));
   for (int s = threadIdx.x; s < p.splits; s += 128) {
     const float2 x = st[s * all + row];
-    const float f = x.x == -INFINITY ? (x.y == x.y ? 0.f : 1.f) : ex2(x.x - mx);
-    weight[s] = f;
-    l += f == 0.f && x.y == x.y ? 0.f : x.y * f;
+    const bool none = x.x == -INFINITY && x.y == x.y;  // no visible key
+    const float f = x.x == -INFINITY ? 1.f : ex2(x.x - mx);
+    weight[s] = none ? -1.f : f;
+    l += none ? 0.f : x.y * f;
   }
 #pragma unroll
   for (int i = 16; i > 0; i >>= 1) l += __shfl_xor_sync(0xffffffffu, l, i);
@@ -504,7 +505,7 @@ __global__ void __launch_bounds__(128) kv8_join_kernel(const StepParams p) {
     const float f = weight[s];
     const float* part = p.a.part + (s * all + row) * P + COLS * lane;
 #pragma unroll
-    for (int i = 0; i < COLS; ++i) x[i] += f == 0.f ? 0.f : part[i] * f;  // a part without visible keys, or with none that counts
+    for (int i = 0; i < COLS; ++i) x[i] += f < 0.f ? 0.f : part[i] * f;  // zero times sums that are no numbers is none
   }
 #pragma unroll
   for (int i = 0; i < COLS; ++i) acc[warp][COLS * lane + i] = x[i];

@@ -425,3 +425,16 @@ def test_a_block_that_is_no_number_reaches_queries_whose_weight_for_it_is_zero(k
     cache = ops.kv8_cache(1, 1, n + T, 64, kind, device="cuda")
     ops.kv8_append(cache, k[:, :n], v[:, :n], 0)
     assert bool(torch.isnan(ops.kv8_attention(q, cache, n, k[:, n:], v[:, n:])).all())
+
+
+@pytest.mark.parametrize("T", [1, 3, 100])
+def test_positions_at_the_ends_of_64_bits(T):
+    cache, k, v = filled(3, 2, 64, 100, "int8", capacity=128)
+    before = {n: t.clone() for n, t in bits(cache).items()}
+    q, nk, nv = rows(3, T, 4, 64, 3, False), rows(3, T, 2, 64, 4), rows(3, T, 2, 64, 5)
+    far = torch.tensor([2 ** 63 - 1, -(2 ** 63), 2 ** 63 - 50], device="cuda")
+    out = ops.kv8_attention(q, cache, far, nk, nv)
+    assert bool(torch.isnan(out[0]).all()) and not out[1].any() and bool(torch.isnan(out[2]).all())
+    assert all(torch.equal(before[n], t) for n, t in bits(cache).items())
+    got = ops.kv8_expand(cache, torch.tensor([2 ** 63 - 1, -(2 ** 63), 100], device="cuda"), 64, 100)
+    assert torch.equal(got[0][2], ops.kv8_expand(cache, 100, 64)[0][2]) and not got[0][1].any()

@@ -17,8 +17,6 @@ struct AppendParams {
   Kv8Pos pos;
 };
 
-__device__ __forceinline__ long long pos_at(const Kv8Pos& p, int b) { return p.dev != nullptr ? p.dev[(long long)b * p.step] : p.host; }
-
 template <bool E4M3>
 __device__ __forceinline__ uint32_t code_of(float y) {
   if constexpr (E4M3) return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
@@ -75,7 +73,7 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const AppendParams p) {
   const int side = at & 1;
   at >>= 1;
   const int g = at % p.c.G, b = at / p.c.G;
-  const long long start = pos_at(p.pos, b);
+  const long long start = p.pos.at(b);
   if (start < 0 || start >= p.c.C) return;
   const int begin = (int)start, end = (int)min((long long)p.c.C, start + p.T);
   const int m = begin / KV8_BLOCK + i, base = m * KV8_BLOCK;
@@ -151,7 +149,7 @@ __global__ void __launch_bounds__(256) kv8_expand_kernel(const ExpandParams p) {
   at /= p.blocks;
   const int side = at & 1;
   at >>= 1;  // head
-  const long long start = pos_at(p.pos, at / p.c.G), given = start < 0 ? 0 : start + p.T;
+  const long long start = p.pos.at(at / p.c.G), given = start < 0 ? 0 : start + p.T;
   const int n = (int)min(given, (long long)p.c.C), base = m * KV8_BLOCK;
   const bool full = base + KV8_BLOCK <= n;
   __nv_bfloat16* out = (side ? p.to.v : p.to.k) + (at * p.rows + base) * p.D;
@@ -201,7 +199,7 @@ __global__ void __launch_bounds__(256) kv8_expand_kernel(const ExpandParams p) {
 }
 
 __global__ void __launch_bounds__(128) kv8_outside_kernel(__nv_bfloat16* out, int T, int width, int C, const Kv8Pos pos) {
-  const long long row = blockIdx.x, start = pos_at(pos, row / T);
+  const long long row = blockIdx.x, start = pos.at(row / T);
   if (start < 0 || start + row % T < C) return;
   for (int i = threadIdx.x; i < width; i += 128) out[row * width + i] = __float2bfloat16(__int_as_float(0x7fc00000));
 }

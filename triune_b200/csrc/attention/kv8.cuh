@@ -30,6 +30,11 @@ struct Kv8Pos {  // position per sequence: dev[b * step], or host where dev is n
   long long host;
   const long long* dev;
   int step;
+  // positions past 2^62 are taken for that: tokens may be added to it
+  __device__ __forceinline__ long long at(int b) const {
+    const long long x = dev != nullptr ? dev[(long long)b * step] : host;
+    return x < (1ll << 62) ? x : 1ll << 62;
+  }
 };
 
 // k, v [B, T, G, D] (16-byte aligned rows) at positions pos .. pos + T - 1

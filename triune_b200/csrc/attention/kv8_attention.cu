@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(DW * 32, resident(P, NT)) kv8_attention_kernel
   const int tile = at % p.tiles;
   at /= p.tiles;
   const int kvh = at % c.G, b = at / c.G;
-  const long long start = p.a.pos.dev != nullptr ? p.a.pos.dev[(long long)b * p.a.pos.step] : p.a.pos.host;
+  const long long start = p.a.pos.at(b);
   const int row0 = tile * NT * 8, D = p.a.D;
   const bool idle = start < 0, outside = start >= c.C;
   const int pos = idle || outside ? 0 : (int)start, total = idle || outside ? 0 : (int)min((long long)c.C, start + p.a.T);
@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(128) kv8_join_kernel(const StepParams p) {
   const int d = threadIdx.x;
   if (d >= p.a.D) return;
   const float total = sum[0] + sum[1] + sum[2] + sum[3];
-  const long long start = p.a.pos.dev != nullptr ? p.a.pos.dev[(long long)b * p.a.pos.step] : p.a.pos.host;
+  const long long start = p.a.pos.at(b);
   const int tok = r / p.rep, h = kvh * p.rep + r % p.rep;
   float y = total == 0.f ? 0.f : (acc[0][d] + acc[1][d] + acc[2][d] + acc[3][d]) / total;
   if (start >= 0 && start + tok >= c.C) y = __int_as_float(0x7fc00000);

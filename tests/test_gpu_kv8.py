@@ -438,3 +438,11 @@ def test_positions_at_the_ends_of_64_bits(T):
     assert all(torch.equal(before[n], t) for n, t in bits(cache).items())
     got = ops.kv8_expand(cache, torch.tensor([2 ** 63 - 1, -(2 ** 63), 100], device="cuda"), 64, 100)
     assert torch.equal(got[0][2], ops.kv8_expand(cache, 100, 64)[0][2]) and not got[0][1].any()
+
+
+@pytest.mark.parametrize("T", [1, 3, 100])
+def test_caches_without_room(T):
+    q, nk, nv = rows(3, T, 4, 64, 3, False), rows(3, T, 2, 64, 4), rows(3, T, 2, 64, 5)
+    empty = ops.kv8_cache(3, 2, 0, 64, "int8", device="cuda")
+    out = ops.kv8_attention(q, empty, torch.tensor([0, -1, 5], device="cuda"), nk, nv)
+    assert bool(torch.isnan(out[0]).all()) and not out[1].any() and bool(torch.isnan(out[2]).all())

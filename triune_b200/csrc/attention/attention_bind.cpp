@@ -265,7 +265,11 @@ Tensor kv8_attention(const Tensor& k8, const Tensor& v8, const Tensor& ks, const
   }
   // a portion of a prompt: codes as bf16 numbers once, then attention on the tensor cores, which applies the blocks' scales
   const int64_t rows = a.most, blocks = (rows + tb::KV8_BLOCK - 1) / tb::KV8_BLOCK;
-  if (rows == 0) return torch::zeros(q.sizes(), q.options());
+  if (rows == 0) {  // no room, or none that is to be looked at
+    out = torch::zeros(q.sizes(), q.options());
+    if (a.pos.dev != nullptr) tb::launch_kv8_outside(c, reinterpret_cast<__nv_bfloat16*>(out.data_ptr()), a.T, a.H * a.D, a.pos, cur_stream());
+    return out;
+  }
   Tensor codes = torch::empty({2, c.B, c.G, rows, a.D}, q.options()), scales = torch::empty({2, c.B, c.G, blocks}, q.options().dtype(at::kFloat));
   tb::Kv8Codes to{reinterpret_cast<__nv_bfloat16*>(codes.data_ptr()), nullptr, scales.data_ptr<float>(), nullptr, nullptr, nullptr};
   to.v = to.k + codes.numel() / 2;

@@ -237,3 +237,87 @@ def test_a_model_evaluated_in_inference_mode_can_be_trained_afterwards(mixer):
         m.eval()(ids)
     m.train().forward_loss(ids[:, :-1], ids[:, 1:]).backward()
     assert all(torch.isfinite(p.grad).all() for p in m.parameters())
+
+
+def one_by_one(layer, x, kind):
+    cache, out = (kv8_state(x.shape[0], layer.kv_heads, layer.head_dim, kind), 0), []
+    for t in range(x.shape[1]):
+        y, cache = layer(x[:, t : t + 1], cache=cache)
+        out.append(y)
+    return torch.cat(out, 1), cache
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("first", [0, 1, 61, 63, 64, 127])
+@torch.no_grad()
+def test_drafted_tokens_that_cross_the_end_of_a_block_are_single_steps(kind, first):
+    """Outputs of the attention are rounded to bf16 (2^-8 of themselves at most), from sums in another order, before the layer's last product."""
+    torch.manual_seed(2)
+    layer = SoftmaxAttention(64, 8, 8, 2)
+    for n in (2, 5, 40, 64):
+        x = rand(2, first + n, 64, seed=n)
+        want, held = one_by_one(layer, x, kind)
+        _, cache = one_by_one(layer, x[:, :first], kind) if first else (None, (kv8_state(2, 2, 8, kind), 0))
+        got, cache = layer(x[:, first:], cache=cache)
+        assert float((got - want[:, first:]).norm() / want[:, first:].norm()) < 2.0 ** -8
+        assert cache[1] == first + n and all(cache[0][name].shape == t.shape for name, t in held[0].tensors.items())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("first,n", [(0, 64), (0, 200), (3, 61), (40, 100), (63, 2), (130, 130)])
+@torch.no_grad()
+def test_outputs_do_not_depend_on_later_tokens(kind, first, n):
+    """The last token of a call is another, and much larger: the others' outputs stay."""
+    torch.manual_seed(3)
+    layer = SoftmaxAttention(64, 8, 8, 2)
+    x = rand(1, first + n, 64)
+    y = x.clone()
+    y[:, -1] *= -1000.0
+    outs = []
+    for z in (x, y):
+        cache = (kv8_state(1, 2, 8, kind), 0)
+        if first:
+            _, cache = layer(z[:, :first], cache=cache)
+        outs.append(layer(z[:, first:], cache=cache)[0])
+    assert torch.equal(outs[0][:, :-1], outs[1][:, :-1]) and not torch.equal(outs[0][:, -1], outs[1][:, -1])
+
+
+@pytest.mark.parametrize("kind,limit", [("int8", 0.02), ("e4m3", 0.08)])
+@torch.no_grad()
+def test_portions_of_a_prompt_of_several_sizes(kind, limit):
+    """The first layer's cache is the same whatever the portions, but for the few numbers that a product of another shape rounds otherwise; logits, and later layers' caches, differ by what codes round off (1 / 254 of a
+    block's largest, or 2^-4 of each number) in averages over what is seen."""
+    m = model(kind)
+    ids = torch.randint(0, 61, (1, 150), generator=torch.Generator().manual_seed(3))
+    want, held = m(ids, cache=m.init_cache(1))
+    for chunk in (50, 64, 65, 7, 1):
+        cache, out = m.init_cache(1), []
+        for part in ids.split(chunk, 1):
+            y, cache = m(part, cache=cache)
+            out.append(y)
+        assert float((torch.cat(out, 1) - want).norm() / want.norm()) < limit, chunk
+        n = 150 // ops.KV8_BLOCK
+        for name in ("k8", "v8"):
+            a, b = (c[0][0][name][:, :, : n * ops.KV8_BLOCK].float() for c in (cache, held))
+            assert float((a != b).float().mean()) < 1e-2, (chunk, name)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_new_tokens_as_given(kind):
+    B, G, H, D, n, T = 3, 2, 4, 64, 100, 150
+    k, v, q = rows(B, n + T, G, D), rows(B, n + T, G, D, seed=1), rand(B, T, H, D, seed=2).bfloat16()
+    cache, same = (ops.kv8_cache(B, G, 256, D, kind) for _ in range(2))
+    for c in (cache, same):
+        ops.kv8_append(c, k[:, :n], v[:, :n], 0)
+    starts = torch.tensor([n, -1, 64])  # the third sequence goes back
+    new = [torch.stack([x[b, max(0, s) : max(0, s) + T] for b, s in enumerate(starts.tolist())]) for x in (k, v)]
+    out = ops.kv8_attention(q, cache, starts, *new, as_given=True)
+    ops.kv8_append(same, *new, starts)
+    assert all(torch.equal(cache[x].view(torch.uint8), same[x].view(torch.uint8)) for x in cache) and not out[1].any()
+    for b in (0, 2):
+        p = int(starts[b])
+        K, V = (torch.cat((cache64(x[b].transpose(0, 1), kind, p), y[b].double().transpose(0, 1)), 1).transpose(0, 1)[None] for x, y in zip((k, v), new))
+        value, bound = attention64(q[b : b + 1], K, V)["o"]
+        assert bool(((out[b : b + 1].double() - value).abs() <= bound).all())
+    with pytest.raises(ValueError, match="as_given"):
+        ops.kv8_attention(q, cache, 0, as_given=True)

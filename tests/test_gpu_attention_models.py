@@ -94,3 +94,37 @@ def test_a_cache_on_another_stream_and_one_that_grows():
         torch.cuda.current_stream().wait_stream(stream)
         assert cache[1] == 700 and cache[0].capacity >= 700
     assert torch.equal(*outs)
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("heads,kv_heads,head_dim", [(8, 2, 64), (4, 4, 128), (16, 1, 72)])
+@pytest.mark.parametrize("first,n", [(0, 64), (0, 200), (3, 61), (40, 100), (317, 5), (63, 2), (1000, 700)])
+@torch.no_grad()
+def test_outputs_on_an_8_bit_cache_do_not_depend_on_later_tokens(kind, heads, kv_heads, head_dim, first, n):
+    """The last token of a call is another, and much larger: the others' outputs stay, bit for bit."""
+    m = layer(heads, kv_heads, head_dim, seed=4)
+    x = torch.randn(1, first + n, m.dim, device="cuda").bfloat16()
+    y = x.clone()
+    y[:, -1] *= -1000.0
+    outs = []
+    for z in (x, y):
+        cache = (kv8_state(1, kv_heads, head_dim, kind, "cuda"), 0)
+        if first:
+            _, cache = m(z[:, :first], cache=cache)
+        outs.append(m(z[:, first:], cache=cache)[0])
+    assert torch.equal(outs[0][:, :-1], outs[1][:, :-1]) and not torch.equal(outs[0][:, -1], outs[1][:, -1])
+
+
+@torch.no_grad()
+def test_a_prompt_at_once_and_in_portions_is_near_the_prompt_in_16_bits():
+    """Outputs against the layer without a cache: codes are off by 1 / 254 of a block's largest (some 3.5 times a value's size), and bf16 on the way."""
+    m = layer(8, 2, 128, seed=5)
+    x = torch.randn(2, 900, m.dim, device="cuda").bfloat16()
+    want, _ = m(x)
+    for chunk in (900, 256, 100, 64, 3):
+        cache, out = (kv8_state(2, 2, 128, "int8", "cuda"), 0), []
+        for part in x.split(chunk, 1):
+            y, cache = m(part, cache=cache)
+            out.append(y)
+        assert rel(torch.cat(out, 1), want) < 3e-2, chunk
+        assert cache[1] == 900

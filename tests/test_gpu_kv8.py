@@ -446,3 +446,50 @@ def test_caches_without_room(T):
     empty = ops.kv8_cache(3, 2, 0, 64, "int8", device="cuda")
     out = ops.kv8_attention(q, empty, torch.tensor([0, -1, 5], device="cuda"), nk, nv)
     assert bool(torch.isnan(out[0]).all()) and not out[1].any() and bool(torch.isnan(out[2]).all())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D", [40, 64, 128])
+@pytest.mark.parametrize("T", [1, 3, 64, 130, 300])
+@pytest.mark.parametrize("starts", [[0], [130], [0, 130, -1, 77, 64, 63, 200, 1]])
+def test_new_tokens_as_given(kind, D, T, starts):
+    """Earlier full blocks are codes, the open block and the call's own tokens as they came; the cache is the same afterwards."""
+    B, G, rep = len(starts), 2, 2
+    longest = max(starts) + T
+    _, k, v = filled(B, G, D, longest, kind)
+    caches = [ops.kv8_cache(B, G, longest + 70, D, kind, device="cuda") for _ in range(2)]
+    for b, n in enumerate(starts):
+        one = ops.kv8_cache(1, G, longest + 70, D, kind, device="cuda")
+        ops.kv8_append(one, k[b : b + 1, : max(n, 0)], v[b : b + 1, : max(n, 0)], 0)
+        for c in caches:
+            for x in c:
+                c[x].view(torch.uint8)[b] = one[x].view(torch.uint8)[0]
+    q = rows(B, T, G * rep, D, 5, False) * 0.25
+    at = lambda x: torch.stack([x[b, max(n, 0) : max(n, 0) + T] for b, n in enumerate(starts)])  # noqa: E731
+    for pos in (torch.tensor(starts, device="cuda"), starts[0])[: 1 + (B == 1)]:
+        cache = {x: t.clone() for x, t in caches[0].items()}
+        out = ops.kv8_attention(q, cache, pos, at(k), at(v), as_given=True)
+        for b, n in enumerate(starts):
+            if n < 0:
+                assert not out[b].any()
+                continue
+            K, V = (torch.cat((cache64(x[b].transpose(0, 1), kind, n), x[b, n : n + T].double().transpose(0, 1)), 1).transpose(0, 1)[None] for x in (k, v))
+            near(out[b : b + 1], attention64(q[b : b + 1], K, V)["o"], f"sequence {b}")
+    ops.kv8_append(caches[1], at(k), at(v), pos)
+    assert all(torch.equal(t, bits(caches[1])[x]) for x, t in bits(cache).items())
+
+
+def test_new_tokens_as_given_at_the_edges():
+    cache, k, v = filled(3, 2, 64, 100, "int8", capacity=128)
+    q, nk, nv = rows(3, 100, 4, 64, 3, False), rows(3, 100, 2, 64, 4), rows(3, 100, 2, 64, 5)
+    before = {n: t.clone() for n, t in bits(cache).items()}
+    out = ops.kv8_attention(q, cache, torch.tensor([100, 2 ** 63 - 1, -7], device="cuda"), nk, nv, as_given=True)
+    assert torch.isfinite(out[0, :28]).all() and bool(torch.isnan(out[0, 28:]).all()) and bool(torch.isnan(out[1]).all()) and not out[2].any()
+    assert all(torch.equal(before[n][1:], t[1:]) for n, t in bits(cache).items())
+    assert not ops.kv8_attention(q, cache, -3, nk, nv, as_given=True).any()
+    cache = filled(1, 2, 64, 100, "int8", capacity=512)[0]  # what is no number reaches the queries that see it, and no others
+    same = {n: t.clone() for n, t in cache.items()}
+    clean = ops.kv8_attention(q[:1], same, 100, nk[:1], nv[:1], as_given=True)
+    nv[0, 20, 1, 5] = float("inf")
+    out = ops.kv8_attention(q[:1], cache, 100, nk[:1], nv[:1], as_given=True)
+    assert torch.equal(out[:, :20], clean[:, :20]) and torch.equal(out[:, :, :2], clean[:, :, :2]) and not torch.isfinite(out[:, 20:, 2:, 5]).any()

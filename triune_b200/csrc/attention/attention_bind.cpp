@@ -6,6 +6,7 @@
 #include <torch/extension.h>
 
 #include <cmath>
+#include <optional>
 
 #include "kv8.cuh"
 
@@ -93,13 +94,24 @@ void check_rows(const tb::Kv8Cache& c, const Tensor& x, int64_t heads, const cha
   TORCH_CHECK(x.size(1) < (1ll << 30), "kv8: too many tokens");
 }
 
-// `held`: copies that have to live until all that may run beside the append is launched; their memory is handed out again from then on
-void append_rows(const tb::Kv8Cache& c, const Tensor& k, const Tensor& v, const tb::Kv8Pos& pos, Tensor (&held)[2]) {
-  check_rows(c, k, c.G, "keys");
-  TORCH_CHECK(v.sizes() == k.sizes(), "kv8: keys and values differ in shape");
-  const tb::AttentionView kv = view_of(k, k, "keys", held[0]), vv = view_of(v, k, "values", held[1]);
-  if (k.numel() > 0) tb::launch_kv8_append(c, kv, vv, (int)k.size(1), (int)k.size(3), pos, cur_stream());
-}
+// New keys and values of a cache. `held`: copies that have to live until all that may run beside the append is launched; their memory
+// is handed out again from then on
+struct NewRows {
+  tb::AttentionView k{}, v{};
+  int T, D;
+  bool any;
+  Tensor held[2];
+  NewRows(const tb::Kv8Cache& c, const Tensor& keys, const Tensor& values) {
+    check_rows(c, keys, c.G, "keys");
+    TORCH_CHECK(values.sizes() == keys.sizes(), "kv8: keys and values differ in shape");
+    k = view_of(keys, keys, "keys", held[0]);
+    v = view_of(values, keys, "values", held[1]);
+    T = (int)keys.size(1), D = (int)keys.size(3), any = keys.numel() > 0;
+  }
+  void append(const tb::Kv8Cache& c, const tb::Kv8Pos& pos) const {
+    if (any) tb::launch_kv8_append(c, k, v, T, D, pos, cur_stream());
+  }
+};
 
 // Forward pass of f.a; -> out, and what the backward pass wants where it will come
 Tensor attend(tb::AttentionFwd& f, const Tensor& q, const Tensor& k, const Tensor& v, bool train, const Tensor& status, Tensor& lse, Tensor& rest) {
@@ -210,8 +222,7 @@ void kv8_append(const Tensor& k8, const Tensor& v8, const Tensor& ks, const Tens
                 int64_t host, const OptTensor& dev) {
   const tb::Kv8Cache c = cache_of(k8, v8, ks, vs, kt, vt, k);
   c10::cuda::CUDAGuard guard(k.device());
-  Tensor held[2];
-  append_rows(c, k, v, pos_of(host, dev, c.B, k), held);
+  NewRows(c, k, v).append(c, pos_of(host, dev, c.B, k));
 }
 
 // -> k, v [B, G, rows, D]
@@ -227,9 +238,10 @@ std::vector<Tensor> kv8_expand(const Tensor& k8, const Tensor& v8, const Tensor&
   return {k, v};
 }
 
-// Appends k and v (where given), then attends. `most`: a bound on the tokens a sequence holds then.
+// Appends k and v (where given), then attends. `most`: a bound on the tokens a sequence holds then. `as_given`: k and v are read as they are,
+// not as the cache holds them.
 Tensor kv8_attention(const Tensor& k8, const Tensor& v8, const Tensor& ks, const Tensor& vs, const Tensor& kt, const Tensor& vt, const Tensor& q,
-                     const OptTensor& k, const OptTensor& v, int64_t host, const OptTensor& dev, double scale, int64_t most, const Tensor& status) {
+                     const OptTensor& k, const OptTensor& v, int64_t host, const OptTensor& dev, double scale, int64_t most, bool as_given, const Tensor& status) {
   const tb::Kv8Cache c = cache_of(k8, v8, ks, vs, kt, vt, q);
   TORCH_CHECK(q.dim() == 4 && q.size(2) % c.G == 0, "kv8: query heads must be a multiple of the cache's");
   check_rows(c, q, q.size(2), "queries");
@@ -237,7 +249,8 @@ Tensor kv8_attention(const Tensor& k8, const Tensor& v8, const Tensor& ks, const
   c10::cuda::CUDAGuard guard(q.device());
   tb::Kv8Attention a{};
   a.c = c;
-  Tensor hq, held[2], part;
+  Tensor hq, part;
+  std::optional<NewRows> rows_in;
   a.q = view_of(q, q, "queries", hq);
   a.T = (int)q.size(1);
   a.H = (int)q.size(2);
@@ -249,12 +262,14 @@ Tensor kv8_attention(const Tensor& k8, const Tensor& v8, const Tensor& ks, const
   if (has(k)) {
     TORCH_CHECK(has(v) && k->dim() == 4 && k->size(1) == q.size(1) && k->size(3) == q.size(3) && k->get_device() == q.get_device(),
                 "kv8: new keys and values come with the queries' tokens");
-    append_rows(c, *k, *v, a.pos, held);
-    a.appended = k->numel() > 0;
+    rows_in.emplace(c, *k, *v);
+    if (!as_given) rows_in->append(c, a.pos);  // else once the open block's old tokens are no longer wanted
+    a.appended = rows_in->any;
   }
+  TORCH_CHECK(has(k) || !as_given, "kv8: new keys and values to read as given");
   if (q.numel() == 0) return torch::empty(q.sizes(), q.options());
   if (a.pos.dev == nullptr && host < 0) return torch::zeros(q.sizes(), q.options());  // idle
-  if (a.T * (a.H / c.G) < PORTION) {
+  if (!as_given && a.T * (a.H / c.G) < PORTION) {
     out = torch::empty(q.sizes(), q.options());
     a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
     const long long bytes = tb::kv8_attention_scratch(a);
@@ -263,15 +278,23 @@ Tensor kv8_attention(const Tensor& k8, const Tensor& v8, const Tensor& ks, const
     tb::launch_kv8_attention(a, cur_stream());
     return out;
   }
+  tb::AttentionFwd f{};
+  if (as_given && a.pos.dev == nullptr && host == 0) {  // nothing comes before them
+    rows_in->append(c, a.pos);
+    f.a = shape_of(q, *k, *v, scale, true, 0, c10::nullopt, c10::nullopt, 0);
+    return attend(f, q, *k, *v, false, status, part, part);
+  }
   // a portion of a prompt: codes as bf16 numbers once, then attention on the tensor cores, which applies the blocks' scales
   const int64_t rows = a.most, blocks = (rows + tb::KV8_BLOCK - 1) / tb::KV8_BLOCK;
   if (rows == 0) {  // no room, or none that is to be looked at
+    if (as_given) rows_in->append(c, a.pos);
     out = torch::zeros(q.sizes(), q.options());
     if (a.pos.dev != nullptr) tb::launch_kv8_outside(c, reinterpret_cast<__nv_bfloat16*>(out.data_ptr()), a.T, a.H * a.D, a.pos, cur_stream());
     return out;
   }
   Tensor codes = torch::empty({2, c.B, c.G, rows, a.D}, q.options()), scales = torch::empty({2, c.B, c.G, blocks}, q.options().dtype(at::kFloat));
-  tb::Kv8Codes to{reinterpret_cast<__nv_bfloat16*>(codes.data_ptr()), nullptr, scales.data_ptr<float>(), nullptr, nullptr, nullptr};
+  tb::Kv8Codes to{reinterpret_cast<__nv_bfloat16*>(codes.data_ptr()), nullptr, scales.data_ptr<float>()};
+  if (as_given) to.new_k = rows_in->k, to.new_v = rows_in->v;
   to.v = to.k + codes.numel() / 2;
   to.v_scales = to.k_scales + scales.numel() / 2;
   Tensor where;
@@ -281,8 +304,8 @@ Tensor kv8_attention(const Tensor& k8, const Tensor& v8, const Tensor& ks, const
     to.ends = to.starts + c.B;
   }
   tb::launch_kv8_codes(c, to, (int)rows, a.D, a.pos, a.T, cur_stream());
+  if (as_given) rows_in->append(c, a.pos);
   const Tensor kk = codes.select(0, 0).transpose(1, 2), vv = codes.select(0, 1).transpose(1, 2);
-  tb::AttentionFwd f{};
   f.a = shape_of(q, kk, vv, scale, true, 0, c10::nullopt, c10::nullopt, a.pos.host);
   if (a.pos.dev != nullptr) f.a.starts = to.starts, f.a.lengths = to.ends;
   f.k_scales = to.k_scales;

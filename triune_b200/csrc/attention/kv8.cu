@@ -149,8 +149,10 @@ __global__ void __launch_bounds__(256) kv8_expand_kernel(const ExpandParams p) {
   at /= p.blocks;
   const int side = at & 1;
   at >>= 1;  // head
+  const AttentionView& fresh = side ? p.to.new_v : p.to.new_k;
   const long long start = p.pos.at(at / p.c.G), given = start < 0 ? 0 : start + p.T;
-  const int n = (int)min(given, (long long)p.c.C), base = m * KV8_BLOCK;
+  const int end = (int)min(given, (long long)p.c.C), base = m * KV8_BLOCK;
+  const int n = CODES && fresh.p != nullptr ? (int)min(max(start, 0ll), (long long)end) : end;  // tokens that are read from the cache
   const bool full = base + KV8_BLOCK <= n;
   __nv_bfloat16* out = (side ? p.to.v : p.to.k) + (at * p.rows + base) * p.D;
   const uint2* codes = reinterpret_cast<const uint2*>((side ? p.c.v8 : p.c.k8) + (at * p.c.C + base) * P);
@@ -158,10 +160,10 @@ __global__ void __launch_bounds__(256) kv8_expand_kernel(const ExpandParams p) {
   float s = full ? (side ? p.c.vs : p.c.ks)[at * (p.c.C / KV8_BLOCK) + m] : 0.f;
   if constexpr (CODES) {
     if (threadIdx.x == 0) {
-      (side ? p.to.v_scales : p.to.k_scales)[at * p.blocks + m] = full ? s : base < n ? 1.f : 0.f;
+      (side ? p.to.v_scales : p.to.k_scales)[at * p.blocks + m] = full ? s : base < end ? 1.f : 0.f;
       if (p.to.ends != nullptr && m == 0 && side == 0 && at % p.c.G == 0) {
         p.to.starts[at / p.c.G] = start;
-        p.to.ends[at / p.c.G] = n;
+        p.to.ends[at / p.c.G] = end;
       }
     }
     s = 1.f;
@@ -169,7 +171,7 @@ __global__ void __launch_bounds__(256) kv8_expand_kernel(const ExpandParams p) {
 #pragma unroll
   for (int e = 0; e < PIECES; ++e) {
     const int i = threadIdx.x + 256 * e, row = i / ACROSS, piece = i % ACROSS;
-    if (base + row >= p.rows || piece * 8 >= p.D || (CODES && base + row >= n)) continue;
+    if (base + row >= p.rows || piece * 8 >= p.D || (CODES && base + row >= end)) continue;
     uint4 z = make_uint4(0, 0, 0, 0);
     if (full) {
       const uint2 c = codes[i];
@@ -193,6 +195,8 @@ __global__ void __launch_bounds__(256) kv8_expand_kernel(const ExpandParams p) {
       }
     } else if (base + row < n) {
       z = ring[i];
+    } else if (CODES && base + row < end) {
+      z = *reinterpret_cast<const uint4*>((const __nv_bfloat16*)fresh.p + at / p.c.G * fresh.sb + at % p.c.G * fresh.sh + (base + row - start) * fresh.sr + piece * 8);
     }
     *reinterpret_cast<uint4*>(out + (long long)row * p.D + piece * 8) = z;
   }
@@ -224,7 +228,7 @@ void launch_kv8_append(const Kv8Cache& c, const AttentionView& k, const Attentio
 }
 
 void launch_kv8_expand(const Kv8Cache& c, __nv_bfloat16* k, __nv_bfloat16* v, int rows, int D, const Kv8Pos& length, cudaStream_t s) {
-  expand<false>(ExpandParams{c, Kv8Codes{k, v, nullptr, nullptr, nullptr, nullptr}, rows, D, (rows + KV8_BLOCK - 1) / KV8_BLOCK, length, 0}, s);
+  expand<false>(ExpandParams{c, Kv8Codes{k, v}, rows, D, (rows + KV8_BLOCK - 1) / KV8_BLOCK, length, 0}, s);
 }
 
 void launch_kv8_codes(const Kv8Cache& c, const Kv8Codes& to, int rows, int D, const Kv8Pos& pos, int T, cudaStream_t s) {

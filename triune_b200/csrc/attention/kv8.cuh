@@ -45,10 +45,13 @@ void launch_kv8_expand(const Kv8Cache& c, __nv_bfloat16* k, __nv_bfloat16* v, in
 // For tensor-core attention over the cache: k, v [B, G, rows, D] hold codes (and the open block's tokens) as bf16 numbers, which they
 // are exactly, k_scales and v_scales [B, G, ceil(rows / 64)] what blocks are multiplied by (1 for the open one, 0 past the end); rows
 // past a sequence's end are left as they are. starts and ends [B] (or null): positions, and those plus T (0 for idle sequences).
+// new_k, new_v [B, T, G, D] (or null): tokens from the position on as they came, in place of what the cache holds of them; it need not hold
+// them yet, and must hold the open block before them (launch_kv8_append comes after).
 struct Kv8Codes {
   __nv_bfloat16 *k, *v;
   float *k_scales, *v_scales;
   long long *starts, *ends;
+  AttentionView new_k, new_v;
 };
 void launch_kv8_codes(const Kv8Cache& c, const Kv8Codes& to, int rows, int D, const Kv8Pos& pos, int T, cudaStream_t s);
 // out [B, T, width]: NaN at the positions past the capacity

@@ -257,8 +257,7 @@ class SoftmaxAttention(nn.Module):
 
     Shared key/value heads, and a portion of tokens after a prefix, run ``ops.attention``; whole prompts with a key/value head per
     query head, and single tokens on a cache in 16 bits, the library's. With a :func:`kv8_state` as the state of its cache the
-    layer keeps keys and values in 8 bits and runs ``ops.kv8_attention``, for prompts, portions and single tokens alike; such a
-    cache advances in place, and its position may be on the device.
+    layer keeps keys and values in 8 bits (:meth:`_attend_in_8_bits`); such a cache advances in place, and its position may be on the device.
 
     Reference: the ``use_sdpa`` branch of ``HybridAttention`` (``triune/model/attention.py:606-653``) and the
     dense model's attention (``triune/universal.py:200-266``).
@@ -277,11 +276,23 @@ class SoftmaxAttention(nn.Module):
         self.rope = RotaryEmbedding(self.head_dim, max_seq_len=rope_max_seq_len, base=rope_base)
 
     def _attend_in_8_bits(self, q, k, v, state: LayerState, offset):
-        """The tokens' keys and values go into the cache, then the queries attend to it. Reserves room where the position is a number."""
+        """Attention of new tokens that go into the cache. No output depends on a later token. Room is reserved where the position is a number:
+
+        * up to 64 tokens attend to the cache as if they came one by one: ``ops.kv8_attention`` reads a block that a call fills as codes, for the
+          queries before the block's last token too, so a call ends before such a token and the next begins with it;
+        * more (and several at a position on the device) attend to what the cache held before and to one another's keys and values as they are
+          given, in bf16. They see earlier portions as codes, so outputs depend on where portions begin, within what codes round off."""
+        T, dtype = q.shape[1], q.dtype
+        q, k, v = (x.to(torch.bfloat16) for x in (q, k, v))
+        ends = [T]
         if not torch.is_tensor(offset):
-            state.reserve(offset + q.shape[1])
-        narrow = [x.to(torch.bfloat16) for x in (q, k, v)]
-        return ops.kv8_attention(narrow[0], state, offset, narrow[1], narrow[2]).to(q.dtype)
+            state.reserve(offset + T)
+            first = ops.KV8_BLOCK - 1 - offset % ops.KV8_BLOCK  # the token that fills the open block
+            if 0 < first < T <= ops.KV8_BLOCK:
+                ends = [first, T]
+        as_given = T > ops.KV8_BLOCK or T > 1 and torch.is_tensor(offset)
+        outs = [ops.kv8_attention(q[:, a:b], state, offset + a, k[:, a:b], v[:, a:b], as_given=as_given) for a, b in zip([0] + ends, ends)]
+        return (torch.cat(outs, 1) if len(outs) > 1 else outs[0]).to(dtype)
 
     def forward(self, x, cache=None):
         B, T, _ = x.shape

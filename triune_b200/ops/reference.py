@@ -818,7 +818,8 @@ def kv8_expand(cache, length, head_dim: int, rows: int):
     return tuple(out)
 
 
-def kv8_attention(q, cache, pos, scale: float):
+def kv8_attention(q, cache, pos, scale: float, new_k=None, new_v=None):
+    """With ``new_k`` and ``new_v``, the tokens from the position on are these, and the cache need not hold them."""
     out = torch.zeros_like(q)
     T, D, room = q.shape[1], q.shape[3], cache["k8"].shape[2]
     for b, p in enumerate(_per_sequence(pos, q.shape[0])):
@@ -826,7 +827,10 @@ def kv8_attention(q, cache, pos, scale: float):
             continue
         n = min(p + T, room)
         if p < n:
-            k, v = (_kv8_values(cache, name, b, n)[None, :, :, :D].transpose(1, 2) for name in ("k", "v"))
+            held = n if new_k is None else p
+            k, v = (_kv8_values(cache, name, b, held)[None, :, :, :D].transpose(1, 2) for name in ("k", "v"))
+            if new_k is not None:
+                k, v = (torch.cat((x, y[b : b + 1, : n - p].float()), 1) for x, y in ((k, new_k), (v, new_v)))
             out[b] = attention(q[b : b + 1].float(), k, v, query_start=p, scale=scale)[0].to(q.dtype)
         out[b, max(0, room - p) :] = float("nan")
     return out

@@ -216,10 +216,15 @@ def kv8_expand(cache: Mapping[str, torch.Tensor], length: Position, head_dim: in
 
 
 def kv8_attention(q: torch.Tensor, cache: Mapping[str, torch.Tensor], pos: Position, k: Optional[torch.Tensor] = None,
-                  v: Optional[torch.Tensor] = None, scale: Optional[float] = None, most: Optional[int] = None) -> torch.Tensor:
-    """Causal attention of ``q`` [B, T, H, D] at positions ``pos`` .. ``pos + T - 1`` over the cached keys up to each query's own ->
+                  v: Optional[torch.Tensor] = None, scale: Optional[float] = None, most: Optional[int] = None,
+                  as_given: bool = False) -> torch.Tensor:
+    """Attention of ``q`` [B, T, H, D] at positions ``pos`` .. ``pos + T - 1`` over the cached keys up to each query's own ->
     [B, T, H, D]. With ``k`` and ``v`` [B, T, G, D], the queries' tokens are appended first (:func:`kv8_append`, also on
-    ``pos``); without, the cache must hold them already. ``most`` is a bound on the tokens that any sequence holds after this call, by
+    ``pos``); without, the cache must hold them already. Keys and values are those that the cache holds once these tokens are in it: a block that the call
+    fills is read as codes by all its queries, also by those before the block's last token. Their outputs depend, by what codes round
+    off, on the rest of the block, and so on later tokens and on how tokens are portioned. A call is strictly causal where no token but its
+    first ends a block (position % 64 == 63), as single tokens are; and with ``as_given``, by which queries see the call's own ``k`` and ``v`` as
+    they are given, and earlier blocks that were full before as codes. ``most`` is a bound on the tokens that any sequence holds after this call, by
     default the capacity (or ``pos + T`` where ``pos`` is a number), for which the work is laid out; tokens past it are not promised to be seen.
 
     Idle sequences (negative positions) give zeros; a query past the capacity (positions on the device only) gives NaN."""
@@ -231,6 +236,8 @@ def kv8_attention(q: torch.Tensor, cache: Mapping[str, torch.Tensor], pos: Posit
         raise ValueError("queries of an 8-bit cache are bfloat16 on the cache's device")
     if (k is None) != (v is None):
         raise ValueError("new keys come with new values")
+    if as_given and k is None:
+        raise ValueError("as_given is about new keys and values, and there are none")
     _no_gradients(q, k, v)
     scale, T = _scale(scale, qs[3]), qs[1]
     if k is not None:
@@ -242,10 +249,15 @@ def kv8_attention(q: torch.Tensor, cache: Mapping[str, torch.Tensor], pos: Posit
     room = cs[2] if dev is not None else max(0, host + T)
     most = room if most is None else min(int(most), room)
     if not _kv8_kernels(cache):
+        at = host if dev is None else dev
+        if as_given:
+            out = ref.kv8_attention(q, cache, at, scale, k, v)
+            ref.kv8_append(cache, k, v, at)
+            return out
         if k is not None:
-            ref.kv8_append(cache, k, v, host if dev is None else dev)
-        return ref.kv8_attention(q, cache, host if dev is None else dev, scale)
-    out = _ext.ext().kv8_attention(*_parts(cache), q, k, v, host, dev, scale, most, status_word(q.device))
+            ref.kv8_append(cache, k, v, at)
+        return ref.kv8_attention(q, cache, at, scale)
+    out = _ext.ext().kv8_attention(*_parts(cache), q, k, v, host, dev, scale, most, as_given, status_word(q.device))
     _tick(2 + (k is not None))
     return out
 

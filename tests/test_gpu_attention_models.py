@@ -128,3 +128,28 @@ def test_a_prompt_at_once_and_in_portions_is_near_the_prompt_in_16_bits():
             out.append(y)
         assert rel(torch.cat(out, 1), want) < 3e-2, chunk
         assert cache[1] == 900
+
+
+@pytest.mark.parametrize("shape", [(2, 37, 8, 2, 64), (1, 700, 8, 2, 128), (1, 2500, 16, 4, 64), (3, 2048, 8, 2, 80), (1, 2048, 6, 1, 128)])
+@pytest.mark.parametrize("train", [True, False])
+def test_prompts_with_shared_heads_of_any_size(shape, train):
+    """Small and large prompts run on different attention; both follow the definition: outputs are rounded to bf16, weights on the way (2^-8 each), and
+    so are the gradients of shared heads, on the library's way before they are added up."""
+    from triune_b200.models.attention import _causal, _own_kernels
+
+    B, T, H, G, D = shape
+    q, k, v = (torch.randn(B, T, h, D, device="cuda", generator=torch.Generator("cuda").manual_seed(h)).bfloat16().requires_grad_(train) for h in (H, G, G + 1))
+    v = v[:, :, :G]
+    assert _own_kernels(q, k, v) == (B * H * T * T * D <= (1 << 32 if train else 1 << 27))
+    out = _causal(q, k, v)
+    kk, vv = (x.detach().double().repeat_interleave(H // G, 2).transpose(1, 2).requires_grad_() for x in (k, v))
+    qq = q.detach().double().transpose(1, 2).requires_grad_()
+    s = (qq @ kk.transpose(-1, -2)) * D ** -0.5
+    want = s.masked_fill(torch.ones(T, T, dtype=torch.bool, device="cuda").triu(1), float("-inf")).softmax(-1) @ vv
+    assert rel(out, want.transpose(1, 2)) < 2.0 ** -7
+    if train:
+        g = torch.randn_like(out)
+        got = torch.autograd.grad(out, (q, k, v), g)
+        dq, dk, dv = torch.autograd.grad(want, (qq, kk, vv), g.double().transpose(1, 2))
+        for a, b in zip(got, (dq.transpose(1, 2), *(x.transpose(1, 2).unflatten(2, (G, H // G)).sum(3) for x in (dk, dv)))):
+            assert rel(a, b) < 3 * 2.0 ** -7

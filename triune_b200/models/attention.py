@@ -245,6 +245,51 @@ class VectorisedGLA(nn.Module):
         return y, torch.stack(states)
 
 
+def _own_kernels(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> bool:
+    """Whether :func:`_causal` runs ``ops.attention`` rather than the library's attention: portions after a prefix, and whole prompts with shared heads
+    that are not too large.
+
+    Measured on one B200, microseconds with a cold L2 (in brackets: calls back to back), forward and backward | forward alone:
+
+        whole prompts, heads on key/value heads    ops.attention           library, shared heads   library, repeated heads
+        2 x 37, 16 on 4 of 64                       90 (95) | 12 (11)       155 (155) | 12 (20)     260 (241) | 43 (54)
+        8 x 512, 16 on 4 of 64                      92 (90) | 25 (21)       130 (136) | 23 (22)     214 (206) | 48 (40)
+        1 x 256, 16 on 4 of 128                     77 (88) | 18 (15)       135 (136) | 14 (20)     232 (220) | 23 (39)
+        8 x 512, 8 on 2 of 128                      95 (90) | 35 (30)       129 (136) | 19 (21)     215 (205) | 40 (39)
+        1 x 2048, 16 on 4 of 64                     120 (106) | 33 (28)     131 (137) | 32 (29)     214 (207) | 48 (42)
+        1 x 2048, 16 on 4 of 128                    152 (144) | 45 (39)     137 (136) | 35 (31)     206 (206) | 54 (52)
+        8 x 2048, 16 on 4 of 64                     445 (438) | 135 (130)   425 (407) | 113 (106)   503 (497) | 179 (172)
+        4 x 4096, 16 on 4 of 128                    1130 | 331              934 | 207               1098 | 331
+        1 x 8192, 16 on 4 of 128                    1012 | 267              821 | 198               908 | 267
+        1 x 32768, 8 on 2 of 128                    7918 | 1889             5805 | 1428             6613 | 1551
+
+        portions after a prefix                     ops.attention           library, mask           library, lower right causal
+        4 after 300, 16 on 4 of 64                  77 | 14                 283 | 69                155 | 21 (shared heads)
+        1024 after 15360, 16 on 4 of 128            513 | 137               1450 | 640              1672 | 486 (shared heads)
+        4096 twice after 4096, 8 of 64              570 | 172               2001 | 646              1408 | 412
+
+    Without shared heads and a prefix the library stays (16 x 2048, 6 heads of 64: 302 against 397)."""
+    (B, T, H, D), (_, S, G, _) = q.shape, k.shape
+    if T == 1 or not ops.attention_supported(q) or not q.dtype == k.dtype == v.dtype:
+        return False
+    return S > T or H > G and B * H * T * T * D <= (1 << 27 if ops.inference_call(q, k, v) else 1 << 32)
+
+
+def _causal(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
+    """Attention of the last T tokens, queries [B, T, H, D], over keys and values [B, S, G, D] up to each one's own."""
+    T, S, rep = q.shape[1], k.shape[1], q.shape[2] // k.shape[2]
+    if _own_kernels(q, k, v):
+        return ops.attention(q, k, v)
+    shared = rep > 1 and T > 1 and ops.attention_supported(q) and q.dtype == k.dtype == v.dtype  # by the library, which need not have them repeated
+    if rep > 1 and not shared:
+        k, v = k.repeat_interleave(rep, dim=2), v.repeat_interleave(rep, dim=2)
+    mask, causal = None, S == T and T > 1
+    if T > 1 and not causal:  # a multi-token chunk after a prefix: query i sees the whole prefix and chunk positions <= i
+        mask = torch.ones(T, S, dtype=torch.bool, device=q.device).tril(diagonal=S - T)
+    o = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), attn_mask=mask, is_causal=causal, enable_gqa=shared)
+    return o.transpose(1, 2)
+
+
 def kv8_state(batch: int, kv_heads: int, head_dim: int, kind: str, device=None) -> LayerState:
     """An empty key/value cache held in 8 bits (:func:`triune_b200.ops.kv8_cache`), which grows as tokens come. Its capacity is counted
     in codes; a scale stands for a block of them."""
@@ -255,8 +300,8 @@ def kv8_state(batch: int, kv_heads: int, head_dim: int, kind: str, device=None) 
 class SoftmaxAttention(nn.Module):
     """Causal softmax attention with RoPE, GQA and a KV cache.
 
-    Shared key/value heads, and a portion of tokens after a prefix, run ``ops.attention``; whole prompts with a key/value head per
-    query head, and single tokens on a cache in 16 bits, the library's. With a :func:`kv8_state` as the state of its cache the
+    A portion of tokens after a prefix, and prompts with shared key/value heads that are not large, run ``ops.attention``; other prompts,
+    and single tokens on a cache in 16 bits, the library's, whichever is faster (:func:`_own_kernels`). With a :func:`kv8_state` as the state of its cache the
     layer keeps keys and values in 8 bits (:meth:`_attend_in_8_bits`); such a cache advances in place, and its position may be on the device.
 
     Reference: the ``use_sdpa`` branch of ``HybridAttention`` (``triune/model/attention.py:606-653``) and the
@@ -309,22 +354,7 @@ class SoftmaxAttention(nn.Module):
             k = torch.cat((past[0], k), dim=1)
             v = torch.cat((past[1], v), dim=1)
         new_state = (k, v) if cache is not None else None
-        rep = self.heads // self.kv_heads
-        if T > 1 and (rep > 1 or past is not None) and ops.attention_supported(q) and k.dtype == q.dtype == v.dtype:
-            # Measured on one B200 against the library with repeated heads and a [T, P + T] mask, forward and backward: 1024 tokens after
-            # 4096, 16 heads on 4 of 128: 171 against 506 us; whole prompts of 8 x 2048: 673 against 754 us. With a key/value head
-            # per query head and no prefix the library is ahead (16 x 2048, 6 heads of 64: 302 against 397 us) and stays.
-            o = ops.attention(q, k, v)
-        else:
-            kk, vv = (k.repeat_interleave(rep, dim=2), v.repeat_interleave(rep, dim=2)) if rep > 1 else (k, v)
-            if past is None or T == 1:
-                mask, causal = None, (past is None and T > 1)
-            else:  # a multi-token chunk after a prefix: query i sees the whole prefix and chunk positions <= i
-                P = kk.shape[1] - T
-                mask = torch.ones(T, P + T, dtype=torch.bool, device=x.device).tril(diagonal=P)
-                causal = False
-            o = F.scaled_dot_product_attention(q.transpose(1, 2), kk.transpose(1, 2), vv.transpose(1, 2), attn_mask=mask,
-                                               is_causal=causal).transpose(1, 2)
+        o = _causal(q, k, v)
         o = o.reshape(B, T, self.heads * self.head_dim)
         return _project(self.out_proj, o), format_cache(new_state, cache, fmt, offset, T)
 

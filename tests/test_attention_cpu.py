@@ -321,3 +321,35 @@ def test_new_tokens_as_given(kind):
         assert bool(((out[b : b + 1].double() - value).abs() <= bound).all())
     with pytest.raises(ValueError, match="as_given"):
         ops.kv8_attention(q, cache, 0, as_given=True)
+
+
+def test_a_loss_that_is_no_number_because_a_wait_expired_says_so():
+    """Attention gives NaN where a kernel's wait expired; what trains raises with that reason. The status word is set here, on the host."""
+    from triune_b200.models.universal import TriuneUniversalEngine
+    from triune_b200.ops import hybrid
+    from triune_b200.trainer.trainer import Trainer
+
+    m = model()
+    ids = torch.randint(0, 61, (2, 20), generator=torch.Generator().manual_seed(5))
+    calls = [lambda e=TriuneUniversalEngine(m, optimizer=torch.optim.SGD(m.parameters(), lr=0.0)): e.train_step(ids)]
+    t = Trainer(m, {"optimizer": "adamw", "mode": "cortex"}, optimizer=torch.optim.SGD(m.parameters(), lr=0.0), device="cpu")
+    t.step_on_device = lambda *a: m.forward_loss(a[0], a[1]).detach()
+    calls.append(lambda: t.train_step(ids[:, :-1], ids[:, 1:]))
+    kept, weight = dict(hybrid._STATUS), m.norm.weight.detach().clone()
+    try:
+        word = hybrid.status_word("cpu")
+        for broken in (False, True):
+            with torch.no_grad():
+                m.norm.weight.copy_(weight * (float("nan") if broken else 1.0))
+            for status in (0, 3):
+                word.fill_(status)
+                for call in calls:
+                    if broken and status:
+                        with pytest.raises(RuntimeError, match="bounded wait expired"):
+                            call()
+                    else:
+                        assert torch.isfinite(torch.tensor(call())) != broken
+    finally:
+        word.zero_()
+        hybrid._STATUS.clear()
+        hybrid._STATUS.update(kept)

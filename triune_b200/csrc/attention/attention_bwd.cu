@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(bwd_threads(TWO), TWO ? 2 : 1) attention_dq_ke
         __syncwarp();
         tmem_load(tmem + lane_base + Q_AT + c, v);
       }
-      if (t < p.a.T) store_row16(o, c, p.a.D, v, n > 0 ? p.a.scale : 0.f);
+      if (t < p.a.T) store_row16(o, c, p.a.D, v, !ok ? __int_as_float(0x7fc00000) : n > 0 ? p.a.scale : 0.f);  // no numbers where a wait expired
     }
     if (!ok && p.status) *p.status = ST_TIMEOUT_TMEM;
   }
@@ -332,6 +332,7 @@ __global__ void __launch_bounds__(bwd_threads(TWO), TWO ? 2 : 1) attention_dkv_k
   const int half_of_all = SHARE ? (all + 1) / 2 : all, n = member == 0 ? half_of_all : all - half_of_all;  // query tiles of all heads, head by head
   const int skip = member == 0 || n == 0 ? 0 : half_of_all;
   const int padded = (p.a.T + AT_M - 1) / AT_M * AT_M;
+  bool finished = true;  // of the softmax warps: no wait expired
 
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
@@ -539,6 +540,7 @@ __global__ void __launch_bounds__(bwd_threads(TWO), TWO ? 2 : 1) attention_dkv_k
     if (ok && n > 0) ok = warp_wait(done, 0);
     tc_fence_after_sync();
     if (!ok && p.status) *p.status = ST_TIMEOUT_TMEM;
+    finished = ok;
   }
   const int half = (warp - 4) >> 2, row = (warp & 3) * 32 + lane, key = k0 + row;
   const uint32_t sums = tmem + ((uint32_t)((warp & 3) * 32) << 16);
@@ -554,7 +556,7 @@ __global__ void __launch_bounds__(bwd_threads(TWO), TWO ? 2 : 1) attention_dkv_k
           tmem_load(sums + (which == 0 ? V_AT : K_AT) + c, v);
           const uint32_t to = mapa_shared(smem_u32(other + (which * 64 * DB + c) * AT_M + row), 0);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to + i * AT_M * 4), "r"(v[i]) : "memory");
+          for (int i = 0; i < 16; ++i) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to + i * AT_M * 4), "r"(finished ? v[i] : 0x7fc00000u) : "memory");
         }
     }
     __syncwarp();
@@ -565,7 +567,7 @@ __global__ void __launch_bounds__(bwd_threads(TWO), TWO ? 2 : 1) attention_dkv_k
     // the first half of the warps writes dV, the second dK
     for (int which = half; which < 2; which += HALVES) {
       __nv_bfloat16* o = (which == 0 ? p.dv : p.dk) + (((long long)b * p.a.S + key) * p.a.G + kvh) * p.a.D;
-      const float f = which == 0 ? 1.f : p.a.scale;
+      const float f = !finished ? __int_as_float(0x7fc00000) : n == 0 ? 0.f : which == 0 ? 1.f : p.a.scale;
       for (int c = 0; c < 64 * DB; c += 16) {
         uint32_t v[16] = {};
         if (n > 0) {
@@ -580,7 +582,7 @@ __global__ void __launch_bounds__(bwd_threads(TWO), TWO ? 2 : 1) attention_dkv_k
 #pragma unroll
           for (int i = 0; i < 16; ++i) v[i] = 0;
         }
-        if (key < p.a.S) store_row16(o, c, p.a.D, v, n > 0 ? f : 0.f);
+        if (key < p.a.S) store_row16(o, c, p.a.D, v, f);
       }
     }
   }

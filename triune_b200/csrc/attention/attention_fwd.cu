@@ -403,6 +403,7 @@ __global__ void __launch_bounds__(fwd_threads(DB, PAIR), alone(DB, PAIR) ? 2 : 1
       if (!ok) break;
     }
     if (ok && n > 0) ok = warp_wait(o_done + w, (n - 1) & 1);
+    if (!ok) l = __int_as_float(0x7fc00000);  // a wait has expired: what is handed on is no number
     tc_fence_after_sync();
     float share = 1.f;  // of this group's sums in the row
     float* half = reinterpret_cast<float*>(sK);

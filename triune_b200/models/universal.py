@@ -17,6 +17,7 @@ import torch.nn.functional as F
 
 from .. import ops
 from ..config import ModelConfig
+from ..ops.hybrid import checked_loss
 from . import native_block
 from .attention import SoftmaxAttention, VectorisedGLA, kv8_state
 from .block import DenseFFN
@@ -249,7 +250,7 @@ class TriuneUniversalEngine:
         loss.backward()
         self.optimizer.step()
         self.optimizer.zero_grad(set_to_none=True)
-        return float(loss.detach())
+        return checked_loss(float(loss.detach()), self.device)
 
     @torch.no_grad()
     def generate(self, input_ids: torch.Tensor, max_new_tokens: int = 32, temperature: float = 0.0, top_k: int = 0):

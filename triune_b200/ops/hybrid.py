@@ -7,6 +7,7 @@ Positions are an ``int`` or, for graph-replayed decoding, a CUDA int64 tensor. N
 
 from __future__ import annotations
 
+import math
 from typing import Any, Dict, List, Optional, Tuple
 
 import torch
@@ -33,9 +34,14 @@ def _host_pos(pos) -> int:
 _STATUS: Dict[Any, torch.Tensor] = {}
 
 
+def _status_key(device) -> torch.device:
+    d = torch.device(device)
+    return torch.device("cuda", torch.cuda.current_device()) if d.type == "cuda" and d.index is None else d
+
+
 def status_word(device) -> torch.Tensor:
     """The device's int32 word that a kernel sets when one of its bounded waits expires (0 = none did)."""
-    key = torch.device(device)
+    key = _status_key(device)
     if key not in _STATUS:
         with torch.inference_mode(False):  # it outlives the call that comes first, and serves calls that train
             _STATUS[key] = torch.zeros(1, dtype=torch.int32, device=key)
@@ -44,9 +50,16 @@ def status_word(device) -> torch.Tensor:
 
 def check_status(device) -> None:
     """Raise if a bounded wait of a kernel on ``device`` has expired (reads the word: waits for the device)."""
-    word = _STATUS.get(torch.device(device))
+    word = _STATUS.get(_status_key(device))
     if word is not None and int(word.item()):
         raise RuntimeError(f"a kernel's bounded wait expired (status {int(word.item())}): its results are not valid")
+
+
+def checked_loss(loss: float, device) -> float:
+    """``loss``, unless it is no finite number and a kernel's bounded wait has expired (attention gives NaN then): raises with that reason."""
+    if not math.isfinite(loss):
+        check_status(device)
+    return loss
 
 
 def embed_rows(ids: torch.Tensor, table: torch.Tensor) -> torch.Tensor:

@@ -27,6 +27,7 @@ import torch
 import torch.nn.functional as F
 
 from ..models.moe import MoE_FFN
+from ..ops.hybrid import checked_loss
 from ..profiling import nvtx_range
 
 
@@ -221,7 +222,7 @@ class TrainingEngine:
             while self.step < total:
                 last = self.step_once()
                 if self.step % log_every == 0:
-                    loss = float(last["loss"])
+                    loss = checked_loss(float(last["loss"]), tr.device)
                     tr.logger.log({"step": self.step, "loss": loss, "lr": last["lr"],
                                    "elapsed_s": time.time() - t0}) if getattr(tr, "logger", None) else None
                 if eval_every and self.step % eval_every == 0 and hasattr(tr, "run_eval"):

@@ -16,6 +16,7 @@ from typing import Any, Dict, Iterable, Optional
 import torch
 
 from ..data.dataloader import AsyncDevicePrefetcher, CyclingDataLoader
+from ..ops.hybrid import checked_loss
 from ..optim.factory import build_optimizer
 from . import checkpoint as ckpt
 from .engine import TrainingEngine
@@ -106,7 +107,7 @@ class Trainer:
             n_valid = int(labels.numel())  # callers with ignored labels pass the exact count
         loss = self.step_on_device(input_ids, labels, n_valid)
         self.d2h_bytes += 4
-        return float(loss.item() if torch.is_tensor(loss) else loss)
+        return checked_loss(float(loss.item() if torch.is_tensor(loss) else loss), self.device)
 
     def step_on_device(self, input_ids: torch.Tensor, labels: torch.Tensor, n_valid: Optional[int] = None):
         """One optimizer step on device-resident tensors; returns the loss as a device tensor (no host sync)."""

@@ -353,3 +353,17 @@ def test_a_loss_that_is_no_number_because_a_wait_expired_says_so():
         word.zero_()
         hybrid._STATUS.clear()
         hybrid._STATUS.update(kept)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_what_a_full_cache_gives_for_fewer_tokens(kind):
+    """Multiples of a block, and up to 64 tokens back."""
+    k, v = rows(1, 300, 2, 64), rows(1, 300, 2, 64, seed=1)
+    cache = ops.kv8_cache(1, 2, 320, 64, kind)
+    ops.kv8_append(cache, k, v, 0)
+    q = rand(1, 2, 4, 64, seed=2).bfloat16()
+    for n in (64, 128, 192, 236, 237, 255, 256, 299):
+        fresh = ops.kv8_cache(1, 2, 320, 64, kind)
+        ops.kv8_append(fresh, k[:, :n], v[:, :n], 0)
+        assert all(torch.equal(a, b) for a, b in zip(ops.kv8_expand(cache, n, 64), ops.kv8_expand(fresh, n, 64))), n
+        assert torch.equal(ops.kv8_attention(q, cache, n - 2), ops.kv8_attention(q, fresh, n - 2)), n

@@ -493,3 +493,16 @@ def test_new_tokens_as_given_at_the_edges():
     nv[0, 20, 1, 5] = float("inf")
     out = ops.kv8_attention(q[:1], cache, 100, nk[:1], nv[:1], as_given=True)
     assert torch.equal(out[:, :20], clean[:, :20]) and torch.equal(out[:, :, :2], clean[:, :, :2]) and not torch.isfinite(out[:, 20:, 2:, 5]).any()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("T", [2, 64])
+def test_what_a_full_cache_gives_for_fewer_tokens(kind, T):
+    """Multiples of a block, and up to 64 tokens back."""
+    cache, k, v = filled(1, 2, 64, 300, kind)
+    q = rows(1, T, 4, 64, 3, False)
+    for n in (64, 128, 192, 236, 237, 255, 256, 299):
+        fresh = ops.kv8_cache(1, 2, 320, 64, kind, device="cuda")
+        ops.kv8_append(fresh, k[:, :n], v[:, :n], 0)
+        assert all(torch.equal(a, b) for a, b in zip(ops.kv8_expand(cache, n, 64), ops.kv8_expand(fresh, n, 64))), n
+        assert torch.equal(ops.kv8_attention(q, cache, n - T), ops.kv8_attention(q, fresh, n - T)), n

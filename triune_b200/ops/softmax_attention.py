@@ -202,7 +202,10 @@ def kv8_append(cache: Mapping[str, torch.Tensor], k: torch.Tensor, v: torch.Tens
 
 def kv8_expand(cache: Mapping[str, torch.Tensor], length: Position, head_dim: int, rows: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """The keys and values of the first ``length`` positions in bf16, [B, rows, G, D] each (``rows``: by default the length where it
-    is a number, else the capacity); zeros from the sequence's length on."""
+    is a number, else the capacity); zeros from the sequence's length on.
+
+    The block in which a length lies is read from the last 128 tokens that came: a length is a multiple of 64, or at most 64 less than what was appended.
+    For others the rows from their last multiple of 64 on are those of later tokens; the cache does not know what was appended, so this is not checked."""
     host, dev = _at(length, "length", cache)
     room, pitch = cache["k8"].shape[2:]
     rows = (max(0, host) if dev is None else room) if rows is None else int(rows)
@@ -220,7 +223,7 @@ def kv8_attention(q: torch.Tensor, cache: Mapping[str, torch.Tensor], pos: Posit
                   as_given: bool = False) -> torch.Tensor:
     """Attention of ``q`` [B, T, H, D] at positions ``pos`` .. ``pos + T - 1`` over the cached keys up to each query's own ->
     [B, T, H, D]. With ``k`` and ``v`` [B, T, G, D], the queries' tokens are appended first (:func:`kv8_append`, also on
-    ``pos``); without, the cache must hold them already. Keys and values are those that the cache holds once these tokens are in it: a block that the call
+    ``pos``); without, the cache must hold them already, and at most 64 behind them (or ``pos + T`` is a multiple of 64; :func:`kv8_expand`). Keys and values are those that the cache holds once these tokens are in it: a block that the call
     fills is read as codes by all its queries, also by those before the block's last token. Their outputs depend, by what codes round
     off, on the rest of the block, and so on later tokens and on how tokens are portioned. A call is strictly causal where no token but its
     first ends a block (position % 64 == 63), as single tokens are; and with ``as_given``, by which queries see the call's own ``k`` and ``v`` as

@@ -36,7 +36,8 @@ inline int attention_rows(int T) { return (T + 127) / 128 * 128; }
 // out [B, T, H, D] contiguous; lse (or null): minus the base-2 logarithm of the sum of the rows' exponentials; -inf for rows that see
 // no key and rows past T, whose weights are zero that way.
 // rest (or null): what the outputs lost when they were rounded, for the backward pass: the rows' sums of dout times out enter every
-// gradient, and with the rounded outputs alone those of short rows were off by up to 4e-3 of themselves instead of 2.4e-3.
+// gradient, and with the rounded outputs alone those of short rows were off by up to 4e-3 of themselves instead of 2.4e-3. It costs a tensor of
+// the outputs' size that is kept until the backward pass (queries, keys, values, outputs, this: a quarter more than without, where heads are not shared).
 // part (attention_fwd_scratch(a) bytes or null): where the keys of few queries are split over blocks.
 // k_scales, v_scales (or null): [B, G, blocks], what blocks of 64 keys and values are multiplied by.
 struct AttentionFwd {

@@ -18,7 +18,6 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "../common/per_device.h"
 #include "attention_tiles.cuh"
 
 namespace tb {
@@ -591,15 +590,6 @@ __global__ void __launch_bounds__(bwd_threads(TWO), TWO ? 2 : 1) attention_dkv_k
   __syncthreads();
   tc_fence_after_sync();
   if (warp == 2) tmem_dealloc(tmem, COLUMNS);
-}
-
-int multiprocessors() {
-  static int count[PerDeviceOnce::kMaxDevices] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= PerDeviceOnce::kMaxDevices) return 148;
-  if (count[dev] == 0) cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev);
-  return count[dev];
 }
 
 template <int DB, bool TWO>

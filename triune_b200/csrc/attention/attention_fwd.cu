@@ -9,7 +9,8 @@
 //     pairs would leave SMs idle; the keys may then also be split over CTAs (`splits`), whose parts a second kernel adds up.
 // Bound by the softmax warps' arithmetic and exponentials: a tile of 128 x 128 takes 1430 (heads of 64) and 1910 clocks (of 128) of an SM
 // in a long walk, of which its products need 700 and 1400 at the rate that a large product reaches here, and its exponentials 770.
-// Whole calls with a cold L2: 8192 tokens, 16 heads on 4 of 128, causal: 240 us (1150 TFLOP/s); 1024 queries after 15360: 141 us.
+// Whole calls with a cold L2: 8192 tokens, 16 heads on 4 of 128, causal: 240 to 267 us from card to card (1150 to 1030 TFLOP/s); 1024 queries after
+// 15360: 137 to 141 us.
 // Warp roles:
 //   warp 0      TMA producer: query tiles once, then two-stage rings of key and value tiles
 //   warp 1      tcgen05.mma: S_w = Q_w K^T into TMEM, O_w += P_w V with P_w read from TMEM
@@ -24,7 +25,6 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "../common/per_device.h"
 #include "attention_tiles.cuh"
 
 namespace tb {
@@ -530,15 +530,6 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const FwdParams p) 
     if (t == p.a.T - 1)
       for (int i = p.a.T; i < padded; ++i) at[i] = -INFINITY;
   }
-}
-
-int multiprocessors() {
-  static int count[PerDeviceOnce::kMaxDevices] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= PerDeviceOnce::kMaxDevices) return 148;
-  if (count[dev] == 0) cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev);
-  return count[dev];
 }
 
 // Pairs where they give every SM a CTA (ALONE: where there are more tiles than SMs: 150 tiles of 640 keys 22.5 us as halves, 16.4 as

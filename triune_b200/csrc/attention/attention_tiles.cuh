@@ -1,5 +1,6 @@
-// What the kernels of attention over bf16 keys share: which tiles of 128 keys a tile of 128 queries sees, and TMA maps.
+// What the kernels of attention over bf16 keys share: which tiles of 128 keys a tile of 128 queries sees, TMA maps, the number of SMs.
 #pragma once
+#include "../common/per_device.h"
 #include "../common/ptx.cuh"
 #include "../common/tma_desc.h"
 #include "attention.cuh"
@@ -70,6 +71,15 @@ __device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
   y = fma2(y, r, pack_f2(0.9999992847442627f, 0.9999992847442627f));
   unpack_f2(t, a, b);
   return mul2(y, pack_f2(__uint_as_float(__float_as_uint(a) * 0x800000u + 0x3f800000u), __uint_as_float(__float_as_uint(b) * 0x800000u + 0x3f800000u)));
+}
+
+inline int multiprocessors() {
+  static int count[PerDeviceOnce::kMaxDevices] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= PerDeviceOnce::kMaxDevices) return 148;
+  if (count[dev] == 0) cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev);
+  return count[dev];
 }
 
 // 64-wide boxes of 128 rows of one head: coordinates (column, row, head, batch); what is outside reads as zero

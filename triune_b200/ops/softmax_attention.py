@@ -1,7 +1,8 @@
 """Softmax attention of training batches and prompts, and attention from a key/value cache held in 8 bits.
 
-CUDA bf16 tensors with heads of up to 128 (a multiple of 8) run the kernels of ``csrc/attention``; other tensors run the statements
-in :mod:`triune_b200.ops.reference`. This is the role of the library call in the reference's ``use_sdpa`` branch
+CUDA bf16 tensors with heads of up to 128 (a multiple of 8) run the kernels of ``csrc/attention``; other tensors (fp16, fp32, other heads) run the statements
+in :mod:`triune_b200.ops.reference`, which hold the [B, H, T, S] scores and weights in fp32 several times over and repeat shared heads:
+2048 tokens, 16 heads: 268 MB a sequence each. ``attention_supported`` tells. This is the role of the library call in the reference's ``use_sdpa`` branch
 (``triune/model/attention.py:606-653``) and dense attention (``triune/universal.py:200-266``); the 8-bit cache has no counterpart there."""
 
 from __future__ import annotations

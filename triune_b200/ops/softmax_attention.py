@@ -99,7 +99,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     outputs of the queries that see it and of no others; gradients are not kept apart in this way. On CUDA, weights and their gradients are rounded to bf16 for
     the matrix products, sums and statistics are fp32, and results do not depend on the order in which blocks run. Forward and backward
     can be captured into a CUDA graph; as with any operator, PyTorch ends the capture of a backward pass with an error where a graph of the
-    same leaves that was not captured is still alive."""
+    same leaves that was not captured is still alive. Where a bounded wait of a kernel expires, what waited for it is NaN
+    (:func:`triune_b200.ops.hybrid.check_status` tells)."""
     B, T, S, D = _shapes(q, k, v)
     scale = _scale(scale, D)
     if window is not None and (int(window) != window or window < 1):

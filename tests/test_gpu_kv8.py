@@ -506,3 +506,49 @@ def test_what_a_full_cache_gives_for_fewer_tokens(kind, T):
         ops.kv8_append(fresh, k[:, :n], v[:, :n], 0)
         assert all(torch.equal(a, b) for a, b in zip(ops.kv8_expand(cache, n, 64), ops.kv8_expand(fresh, n, 64))), n
         assert torch.equal(ops.kv8_attention(q, cache, n - T), ops.kv8_attention(q, fresh, n - T)), n
+
+
+@pytest.mark.parametrize("T", [3, 80])
+def test_new_tokens_as_given_in_a_graph_on_a_stream_and_in_other_layouts(T):
+    n, steps = 100, 4
+    k, v, q = (rows(2, n + T * steps, h, 64, s, False) for h, s in ((2, 1), (2, 2), (4, 3)))
+
+    def fresh():
+        cache = ops.kv8_cache(2, 2, n + T * steps, 64, "int8", device="cuda")
+        ops.kv8_append(cache, k[:, :n], v[:, :n], 0)
+        return cache
+
+    def at_device(i):  # as captured: keys are split by the capacity then, not by the tokens that there are
+        return torch.tensor([n + T * i], device="cuda")
+
+    want, cache = [], fresh()
+    for i in range(steps):
+        at = slice(n + T * i, n + T * i + T)
+        want.append(ops.kv8_attention(q[:, at], cache, at_device(i), k[:, at], v[:, at], as_given=True))
+    graphs = []
+    for _ in range(2):  # two captures, replayed in turn
+        c, pos = fresh(), torch.tensor([n], device="cuda")
+        new = [x[:, n : n + T].clone() for x in (q, k, v)]
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = ops.kv8_attention(new[0], c, pos, new[1], new[2], as_given=True)
+        graphs.append((g, new, out, pos, c))
+    for i in range(steps):
+        for g, new, out, pos, _ in graphs:
+            pos.fill_(n + T * i)
+            for x, y in zip(new, (q, k, v)):
+                x.copy_(y[:, n + T * i : n + T * i + T])
+            g.replay()
+            assert torch.equal(out, want[i])
+    assert all(torch.equal(a, bits(graphs[0][4])[x]) for x, a in bits(cache).items())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = fresh()
+        for i in range(steps):  # heads first, and rows whose addresses are no multiples of 16 bytes: copied
+            new = [x[:, n + T * i : n + T * i + T] for x in (q, k, v)]
+            new[1] = new[1].transpose(1, 2).contiguous().transpose(1, 2)
+            new[2] = torch.zeros(2, T, 2, 72, device="cuda", dtype=torch.bfloat16)[..., 3:67].copy_(new[2])
+            assert torch.equal(ops.kv8_attention(new[0], other, at_device(i), new[1], new[2], as_given=True), want[i])
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, bits(other)[x]) for x, a in bits(cache).items())
